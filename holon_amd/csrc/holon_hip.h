@@ -545,6 +545,33 @@ int holon_bigram_embedding(const int32_t* ids, const int32_t* take_slot, const i
                            int vocab, int buckets, int64_t mul_prev, int64_t mul_cur, int state_slots, int dtype,
                            int rows_in_order, void* stream);
 
+// -- continuations of a context (cache_q8.hip, cache_attention.hip, verify_drafts.hip) ------------------------------------
+// The 8-bit cache: codes [pages, 2, kv_heads, P * D], keys as rows, values transposed, and scales [pages, 2, kv_heads, P], pages
+// page_stride and scale_stride bytes apart (see cache_q8.h). k, v: tokens `stride` values apart.
+int holon_kv_write_q8(const void* k, const void* v, int64_t stride, void* pages, void* scales, int64_t page_stride,
+                      int64_t scale_stride, const int32_t* write_page, const int32_t* write_off, int tokens, int kv_heads,
+                      int head_dim, int page_size, int num_pages, int dtype, void* stream);
+int holon_kv_read_q8(void* k, void* v, const void* pages, const void* scales, int64_t page_stride, int64_t scale_stride,
+                     const int32_t* read_page, const int32_t* read_off, int tokens, int kv_heads, int head_dim, int page_size,
+                     int num_pages, int dtype, void* stream);
+// Paged attention over it (scales given; dtype of q and out), or over bfloat16 pages (scales NULL), rows sharing their first tokens
+// by groups (n_groups 0: none). `room`: holon_cache_attention_room bytes of scratch, on a border of 16.
+int64_t holon_cache_attention_room(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len, int n_groups,
+                                   int max_group_query, int max_group_len, int n_tokens, int heads, int kv_heads, int head_dim,
+                                   int window, int dtype);
+int holon_cache_attention(const void* q, void* out, const void* pages, const void* scales, int64_t page_stride, int64_t scale_stride,
+                          int num_pages, const int32_t* table, int table_stride, int n_slots, const int32_t* slots,
+                          const int32_t* lens, const int32_t* qstart, const int32_t* decode_rows, int n_decode, int max_decode_len,
+                          const int32_t* chunk_rows, int n_chunk, int max_chunk_query, int max_chunk_len,
+                          const int32_t* group_start, const int32_t* group_lens, int n_groups, int max_group_query,
+                          int max_group_len, int n_tokens, int heads, int kv_heads, int head_dim, int page_size, float scale,
+                          int window, const float* sink, void* room, int dtype, void* stream);
+// Drafted tokens against softmax(logits / temperature): see verify_drafts.hip. `room`: holon_verify_drafts_room bytes.
+int64_t holon_verify_drafts_room(int rows, int requests, int vocab);
+int holon_verify_drafts(const float* logits, const int32_t* drafted, const float* draft_probs, const float* accept,
+                        const float* draw, const float* temperature, const int32_t* start, int32_t* tokens, int32_t* accepted,
+                        void* room, int rows, int requests, int vocab, int most, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,334 @@
+// Drafted tokens judged against the target's probabilities, from given random numbers. Request b owns rows start[b] ..
+// start[b + 1] - 1 of the logits; row i judges drafted[i], the last one has none behind it. With p = softmax(logits / T) and q the
+// distribution that the draft came from (given, or certainty):
+//
+//   row i takes its draft x when accept[i] q(x) <= p(x);   after the first that does not (or the last row) one token is drawn:
+//   from max(p - q, 0), renormalised, where a draft was turned down, from p where none was judged,
+//   the first x with sum_{y <= x} mass(y) > draw[b] * sum mass.
+//
+// So a token's law is p whatever q is. T = 0 takes the largest logit for p. The draw compares a running sum over up to hundreds
+// of thousands of masses with a given number: exponentials and sums are in 64 bits, where the order of a sum moves a border
+// between two tokens by 1e-16 of the whole, not by more than a token's own mass as in 32.
+//
+// Three launches over pieces of 4,096 values: every row's largest value and sum of exponentials; the judgement (each block of a
+// request works it out for itself from those) and its masses; the walk through the one piece that the drawn number falls into.
+#include "common.h"
+#include "holon_hip.h"
+
+namespace {
+
+constexpr int PIECE = 4096, THREADS = 256, EACH = PIECE / THREADS, MOST = 64;   // MOST: rows a request may have
+
+struct RowPart {        // of one piece of one row
+  double sum;           // of 2^((l - max) c), c = log2(e) / T
+  float max;
+  int at;               // the first place of `max`
+};
+struct Judged {         // of one request
+  double inv_z;         // 1 / sum of the end row
+  double heat;          // log2(e) / T; 0: T = 0
+  float max;            // of the end row
+  int row, accepted, draft;   // the end row, how many drafts were taken, the one that was not (-1: none was judged)
+  int token;            // T = 0: the token itself
+};
+struct Masses {
+  double left, all;     // of max(p - q, 0), of p
+};
+
+// 2^z for z <= 0: a whole power, and on [-1/2, 1/2] the sum of (r ln 2)^k / k! up to k = 12, whose next term is below 2e-16.
+__device__ __forceinline__ double exp2_of(double z) {
+  const double n = rint(z), r = z - n;
+  constexpr double C = 0.69314718055994530942;
+  const double x = r * C;
+  double p = 1.0 / 479001600.0;
+  p = fma(p, x, 1.0 / 39916800.0);
+  p = fma(p, x, 1.0 / 3628800.0);
+  p = fma(p, x, 1.0 / 362880.0);
+  p = fma(p, x, 1.0 / 40320.0);
+  p = fma(p, x, 1.0 / 5040.0);
+  p = fma(p, x, 1.0 / 720.0);
+  p = fma(p, x, 1.0 / 120.0);
+  p = fma(p, x, 1.0 / 24.0);
+  p = fma(p, x, 1.0 / 6.0);
+  p = fma(p, x, 0.5);
+  p = fma(p, x, 1.0);
+  p = fma(p, x, 1.0);
+  return z < -1000.0 ? 0.0 : ldexp(p, (int)fmax(n, -1100.0));
+}
+// exp((l - max) / T): 1 at the largest value, also where that is infinite; nothing for what is no number.
+__device__ __forceinline__ double weight_of(float l, float max, double c) {
+  if (l == max) return l == -INFINITY ? 0.0 : 1.0;
+  return l < max && max < INFINITY ? exp2_of(((double)l - (double)max) * c) : 0.0;
+}
+
+// The values of piece `lo` that a thread takes: 4 * (tid + 256 j) .. + 3, j < 4, in 16-byte loads where rows allow it.
+__device__ __forceinline__ void load_piece(const float* __restrict__ row, int lo, int vocab, bool wide, float fill, float (&x)[EACH]) {
+#pragma unroll
+  for (int j = 0; j < EACH / 4; ++j) {
+    const int at = lo + 4 * ((int)threadIdx.x + THREADS * j);
+    if (wide && at + 3 < vocab) {
+      const float4 v = *reinterpret_cast<const float4*>(row + at);
+      x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * j + e] = at + e < vocab ? row[at + e] : fill;
+    }
+  }
+}
+__device__ __forceinline__ int place_of(int lo, int i) { return lo + 4 * ((int)threadIdx.x + THREADS * (i / 4)) + i % 4; }
+
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += lane_xor<32>(v);
+  v += lane_xor<16>(v);
+  v += lane_xor<8>(v);
+  v += lane_xor<4>(v);
+  v += lane_xor<2>(v);
+  v += lane_xor<1>(v);
+  return v;
+}
+__device__ __forceinline__ double block_sum64(double v, double* part) {      // every thread gets it; `part`: 4 values of LDS
+  v = wave_sum64(v);
+  if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = v;
+  __syncthreads();
+  const double s = (part[0] + part[1]) + (part[2] + part[3]);
+  __syncthreads();
+  return s;
+}
+
+// The request that owns row i (-1: none): how many starts are at most i, by the lanes of a wave side by side.
+__device__ __forceinline__ int owner_of(const int32_t* __restrict__ start, int requests, int i) {
+  int before = 0;
+  for (int at = 0; at <= requests; at += WAVE) {
+    const int j = at + (int)(threadIdx.x % WAVE);
+    before += __popcll(__ballot(j <= requests && start[min(j, requests)] <= i));
+  }
+  return before >= 1 && before <= requests ? before - 1 : -1;
+}
+// log2(e) / T; 0 says T = 0 (an infinite T: all the same but what is -inf).
+__device__ __forceinline__ double heat_of(float t) { return t > 0.f ? fmax(1.4426950408889634074 / (double)t, 1e-300) : 0.0; }
+
+__global__ void __launch_bounds__(THREADS) verify_rows_kernel(const float* __restrict__ logits, const int32_t* __restrict__ start,
+                                                              const float* __restrict__ temperature, RowPart* __restrict__ parts,
+                                                              int requests, int vocab, int wide) {
+  __shared__ double sums[THREADS / WAVE];
+  __shared__ float tops[THREADS / WAVE];
+  __shared__ int ats[THREADS / WAVE];
+  const int piece = blockIdx.x, row = blockIdx.y, lo = piece * PIECE;
+  const int b = owner_of(start, requests, row);
+  if (b < 0) return;                                          // a row behind the last request's (the same for the whole block)
+  const double c = heat_of(temperature[b]);
+  float x[EACH];
+  load_piece(logits + (int64_t)row * vocab, lo, vocab, wide, -INFINITY, x);
+  float top = -INFINITY;
+  int at = 0x7fffffff;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)                              // (a thread's places grow with i; what is no number is never larger)
+    if (x[i] > top) { top = x[i]; at = place_of(lo, i); }
+#pragma unroll
+  for (int o = WAVE / 2; o > 0; o >>= 1) {
+    const float t2 = __shfl_xor(top, o, WAVE);
+    const int a2 = __shfl_xor(at, o, WAVE);
+    if (t2 > top || (t2 == top && a2 < at)) { top = t2; at = a2; }
+  }
+  if (threadIdx.x % WAVE == 0) { tops[threadIdx.x / WAVE] = top; ats[threadIdx.x / WAVE] = at; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / WAVE; ++w)
+    if (tops[w] > top || (tops[w] == top && ats[w] < at)) { top = tops[w]; at = ats[w]; }
+  double s = 0.0;
+  if (c > 0.0) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) s += weight_of(x[i], top, c);
+    s = block_sum64(s, sums);
+  }
+  if (threadIdx.x == 0) parts[(int64_t)row * gridDim.x + piece] = RowPart{s, top, at};
+}
+
+// One wave: a row's largest value, its first place and its sum of weights from its pieces, added in piece order by lanes and
+// then over the lanes: an order that the number of pieces alone decides.
+__device__ __forceinline__ RowPart whole_row(const RowPart* __restrict__ parts, int pieces, double c) {
+  const int lane = threadIdx.x % WAVE;
+  float top = -INFINITY;
+  int at = 0x7fffffff;
+  for (int i = lane; i < pieces; i += WAVE) {
+    const RowPart p = parts[i];
+    if (p.max > top || (p.max == top && p.at < at)) { top = p.max; at = p.at; }
+  }
+#pragma unroll
+  for (int o = WAVE / 2; o > 0; o >>= 1) {
+    const float t2 = __shfl_xor(top, o, WAVE);
+    const int a2 = __shfl_xor(at, o, WAVE);
+    if (t2 > top || (t2 == top && a2 < at)) { top = t2; at = a2; }
+  }
+  double s = 0.0;
+  if (c > 0.0)
+    for (int i = lane; i < pieces; i += WAVE) s += parts[i].sum * weight_of(parts[i].max, top, c);
+  return RowPart{wave_sum64(s), top, at};
+}
+
+__global__ void __launch_bounds__(THREADS) verify_masses_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
+                                                                const float* __restrict__ draft_probs, const float* __restrict__ accept,
+                                                                const float* __restrict__ temperature,
+                                                                const int32_t* __restrict__ start, const RowPart* __restrict__ parts,
+                                                                Judged* __restrict__ judged, Masses* __restrict__ masses, int rows,
+                                                                int vocab, int most, int wide) {
+  __shared__ RowPart whole[MOST];
+  __shared__ int verdict[MOST];                               // 1: taken, 0: turned down, -1: nothing to judge
+  __shared__ double sums[THREADS / WAVE];
+  const int piece = blockIdx.x, b = blockIdx.y, wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+  const int first = max(start[b], 0), n = min(min(start[b + 1], rows) - first, most + 1);
+  if (n <= 0) {
+    if (piece == 0 && threadIdx.x == 0) judged[b] = Judged{0.0, 0.0, 0.f, -1, 0, -1, -1};
+    return;
+  }
+  const double c = heat_of(temperature[b]);
+  for (int i = wave; i < n; i += THREADS / WAVE) {
+    const RowPart w = whole_row(parts + (int64_t)(first + i) * gridDim.x, gridDim.x, c);
+    if (lane == 0) {
+      whole[i] = w;
+      int v = -1;
+      const int x = drafted[first + i];
+      if (i + 1 < n && x >= 0 && x < vocab) {
+        const int64_t at = (int64_t)(first + i) * vocab + x;
+        if (c > 0.0) {
+          const double q = draft_probs != nullptr ? (double)draft_probs[at] : 1.0;
+          v = (double)accept[first + i] * q * w.sum <= weight_of(logits[at], w.max, c) ? 1 : 0;
+        } else {
+          v = x == (w.at == 0x7fffffff ? 0 : w.at) ? 1 : 0;
+        }
+      }
+      verdict[i] = v;
+    }
+  }
+  __syncthreads();
+  int end = 0;
+  while (end < n - 1 && verdict[end] == 1) ++end;
+  const bool turned_down = verdict[end] == 0;
+  const RowPart w = whole[end];
+  const int row = first + end, draft = turned_down ? drafted[row] : -1;
+  const double inv_z = w.sum > 0.0 ? 1.0 / w.sum : 0.0;
+  if (piece == 0 && threadIdx.x == 0)
+    judged[b] = Judged{inv_z, c, w.max, row, end, draft, w.at == 0x7fffffff ? 0 : w.at};
+  if (c == 0.0) return;
+  float x[EACH], q[EACH];
+  const int lo = piece * PIECE;
+  load_piece(logits + (int64_t)row * vocab, lo, vocab, wide, -INFINITY, x);
+  const bool by_probs = turned_down && draft_probs != nullptr;
+  if (by_probs) load_piece(draft_probs + (int64_t)row * vocab, lo, vocab, wide, 0.f, q);
+  double left = 0.0, all = 0.0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const double p = weight_of(x[i], w.max, c) * inv_z;
+    all += p;
+    left += by_probs ? fmax(p - (double)q[i], 0.0) : (place_of(lo, i) == draft ? 0.0 : p);
+  }
+  all = block_sum64(all, sums);
+  left = block_sum64(left, sums);
+  if (threadIdx.x == 0) masses[(int64_t)b * gridDim.x + piece] = Masses{left, all};
+}
+
+__global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
+                                                              const float* __restrict__ draft_probs, const float* __restrict__ draw,
+                                                              const Judged* __restrict__ judged, const Masses* __restrict__ masses,
+                                                              int32_t* __restrict__ tokens, int32_t* __restrict__ accepted,
+                                                              int pieces, int vocab, int most) {
+  __shared__ double upto[THREADS];
+  __shared__ int found, last, chosen;
+  __shared__ double target, base;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const Judged j = judged[b];
+  int token = j.token;
+  if (j.row >= 0 && j.heat > 0.0) {
+    const Masses* mine = masses + (int64_t)b * pieces;
+    if (tid == 0) {
+      double left = 0.0, all = 0.0;
+      for (int i = 0; i < pieces; ++i) { left += mine[i].left; all += mine[i].all; }
+      const bool use = left > 0.0;                            // (q = p everywhere leaves nothing: then from p)
+      const double want = (double)draw[b] * (use ? left : all);
+      double sum = 0.0, before = 0.0;
+      int pick = -1, heavy = -1;
+      for (int i = 0; i < pieces && pick < 0; ++i) {
+        const double m = use ? mine[i].left : mine[i].all;
+        if (m > 0.0) { heavy = i; before = sum; }
+        sum += m;
+        if (sum > want) pick = i;
+      }
+      chosen = pick >= 0 ? pick : heavy;                      // (a number so near one that rounding passed the last border)
+      base = before;
+      target = want;
+      found = 0x7fffffff;
+      last = use ? -1 : -2;
+    }
+    __syncthreads();
+    const bool use = last == -1;
+    if (chosen >= 0) {
+      const int lo = chosen * PIECE + tid * EACH;
+      const float* row = logits + (int64_t)j.row * vocab;
+      const float* qrow = draft_probs != nullptr && j.draft >= 0 ? draft_probs + (int64_t)j.row * vocab : nullptr;
+      double m[EACH], s = 0.0;
+      int heavy = -1;
+      for (int i = 0; i < EACH; ++i) {
+        const int x = lo + i;
+        double p = x < vocab ? weight_of(row[x], j.max, j.heat) * j.inv_z : 0.0;
+        if (use && x < vocab) p = qrow != nullptr ? fmax(p - (double)qrow[x], 0.0) : (x == j.draft ? 0.0 : p);
+        m[i] = p;
+        s += p;
+        if (p > 0.0) heavy = x;
+      }
+      upto[tid] = s;
+      __syncthreads();
+      if (tid == 0) {                                         // running sums in order
+        double sum = base;
+        for (int i = 0; i < THREADS; ++i) { const double v = upto[i]; upto[i] = sum; sum += v; }
+      }
+      __syncthreads();
+      double sum = upto[tid];
+      int first = 0x7fffffff;
+      for (int i = 0; i < EACH && first == 0x7fffffff; ++i) {
+        sum += m[i];
+        if (m[i] > 0.0 && sum > target) first = lo + i;
+      }
+      if (first != 0x7fffffff) atomicMin(&found, first);      // (whole numbers: in any order the same)
+      if (heavy >= 0) atomicMax(&last, heavy);
+      __syncthreads();
+      token = found != 0x7fffffff ? found : max(last, 0);
+    } else {
+      token = 0;                                              // no token has any mass
+    }
+  }
+  for (int i = tid; i <= most; i += THREADS)
+    tokens[(int64_t)b * (most + 1) + i] = j.row < 0 || i > j.accepted ? -1 : i == j.accepted ? token : drafted[j.row - j.accepted + i];
+  if (tid == 0) accepted[b] = j.accepted;
+}
+
+}  // namespace
+
+extern "C" int64_t holon_verify_drafts_room(int rows, int requests, int vocab) {
+  const int64_t pieces = ((int64_t)vocab + PIECE - 1) / PIECE;
+  return rows * pieces * (int64_t)sizeof(RowPart) + requests * (int64_t)sizeof(Judged) + requests * pieces * (int64_t)sizeof(Masses);
+}
+
+extern "C" int holon_verify_drafts(const float* logits, const int32_t* drafted, const float* draft_probs, const float* accept,
+                                   const float* draw, const float* temperature, const int32_t* start, int32_t* tokens,
+                                   int32_t* accepted, void* room, int rows, int requests, int vocab, int most, void* stream) {
+  HOLON_CHECK(rows >= 0 && requests >= 0 && vocab > 0 && vocab <= PIECE * 65535, "verify_drafts: bad sizes");
+  HOLON_CHECK(most >= 0 && most < MOST, "verify_drafts: %d drafted tokens a request (at most %d)", most, MOST - 1);
+  HOLON_CHECK(rows <= 65535 && requests <= 65535, "verify_drafts: %d rows of %d requests (at most 65,535)", rows, requests);
+  if (requests == 0) return 0;
+  const int pieces = (vocab + PIECE - 1) / PIECE;
+  RowPart* parts = (RowPart*)room;
+  Masses* masses = (Masses*)(parts + (int64_t)rows * pieces);
+  Judged* judged = (Judged*)(masses + (int64_t)requests * pieces);
+  const bool wide = vocab % 4 == 0 && ((uintptr_t)logits | (uintptr_t)draft_probs) % 16 == 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (rows > 0) {
+    verify_rows_kernel<<<dim3(pieces, rows), THREADS, 0, s>>>(logits, start, temperature, parts, requests, vocab, wide);
+    HOLON_LAUNCH_OK();
+  }
+  verify_masses_kernel<<<dim3(pieces, requests), THREADS, 0, s>>>(logits, drafted, draft_probs, accept, temperature, start, parts, judged,
+                                                                  masses, rows, vocab, most, wide);
+  HOLON_LAUNCH_OK();
+  verify_draw_kernel<<<requests, THREADS, 0, s>>>(logits, drafted, draft_probs, draw, judged, masses, tokens, accepted, pieces, vocab, most);
+  HOLON_LAUNCH_OK();
+  return 0;
+}

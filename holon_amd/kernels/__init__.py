@@ -1,7 +1,7 @@
 """Device kernels: the contract (`api`) and its HIP implementation (`hip`)."""
-from .api import AttnRows, Kernels
+from .api import AttnRows, Kernels, SharedPrefix
 
-__all__ = ["AttnRows", "Kernels", "load_hip"]
+__all__ = ["AttnRows", "Kernels", "SharedPrefix", "load_hip"]
 
 
 def load_hip(build_if_missing: bool = True):

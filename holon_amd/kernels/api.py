@@ -42,6 +42,18 @@ class AttnRows:
     in_order: bool = False               # every row is a decode row, and decode_rows[i] = query_start[i] = i
 
 
+@dataclasses.dataclass
+class SharedPrefix:
+    """Rows of a step that begin with the same tokens: group g is rows group_start[g] .. group_start[g + 1] - 1 (neighbours; a
+    row may be in none), whose first lens[g] tokens are the same ones in the same cache pages."""
+
+    group_start: torch.Tensor            # [G+1] int32, rising
+    lens: torch.Tensor                   # [G] int32
+    n_groups: int
+    max_queries: int                     # host bounds for launch shapes: the most query tokens of a group's rows together,
+    max_len: int                         # and the longest prefix
+
+
 class Kernels(Protocol):
     name: str
 
@@ -158,6 +170,37 @@ class Kernels(Protocol):
         h // s (several score maps over one set of values). `head_gate` [T, Hq] (there as well; columns of wider rows
         will do): head h's result of token t is multiplied by sigmoid(head_gate[t, h]) before it is rounded."""
 
+    def check_cache_q8(self, head_dim: int, page_size: int) -> None:
+        """Raise, with a message that names the limit, when no 8-bit cache of this head size and page size is served."""
+
+    def kv_write_q8(self, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, write_page: torch.Tensor,
+                    write_off: torch.Tensor, page_size: int) -> None:
+        """k, v [T, Hkv, D] into an 8-bit cache at (write_page[t], write_off[t]): pages [n, 2, Hkv, P * D] float8_e4m3fn in the
+        cache layout above, scales [n, 2, Hkv, P] float8_e8m0fnu (either may be a uint8 view; pages may lie apart, each in one
+        piece). A (token, head) row is held as round(x / 2^e) and the byte of 2^e, e the smallest power of two, at least -126,
+        that brings its largest finite value to 448 or less (a row of zeros: 0); a value that is not finite is held as NaN.
+        k and v may be columns of wider rows (equally far apart). A token whose place lies outside the pool or the page is not
+        written. Two tokens of one place: their bytes mix (the padding rows of a captured step share the null page)."""
+
+    def kv_read_q8(self, pages: torch.Tensor, scales: torch.Tensor, read_page: torch.Tensor, read_off: torch.Tensor, page_size: int,
+                   dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the places (read_page[t], read_off[t]) of an 8-bit cache stand for: (k, v), new tensors [T, Hkv, D], code * 2^e
+        in `dtype` (bfloat16 holds it exactly). Zeros for a place outside the pool or the page."""
+
+    def paged_attention_q8(self, q: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor, table: torch.Tensor, rows: AttnRows,
+                           page_size: int, scale: float, window: int = 0, sink: torch.Tensor | None = None) -> torch.Tensor:
+        """`paged_attention` over an 8-bit cache (see `kv_write_q8`): the softmax and its sums in float32 over the values that the
+        cache stands for. q [T, Hq, D] bfloat16 or float32 -> a new tensor of its type; heads of 64, 128 and 256, pages of a
+        multiple of 16 tokens; `scale` > 0. A query that sees no key gets zeros; what a query does not see, finite or not, does
+        not reach it. Tokens of no row are not written. A page or slot number out of range is not followed."""
+
+    def prefix_attention(self, q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, rows: AttnRows, prefix: SharedPrefix,
+                         page_size: int, scale: float, scales: torch.Tensor | None = None, sink: torch.Tensor | None = None
+                         ) -> torch.Tensor:
+        """`paged_attention` (window 0) of a batch whose rows share their first tokens by groups: a group's prefix is read once for
+        all of its rows' queries (through its first row's block table), each row's further keys by itself, and the two are joined.
+        pages bfloat16, or with `scales` an 8-bit cache. Sizes, types and masks as in `paged_attention_q8`."""
+
     def qkv_attention(self, qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
                       q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float,
                       rope_table: torch.Tensor | None, positions: torch.Tensor, pages: torch.Tensor | None,
@@ -186,6 +229,19 @@ class Kernels(Protocol):
         position of the token being drawn). Rows with temperature 0 take the argmax; the others draw by inverse CDF
         at the hashed uniform of (seed, position): in vocabulary order when the row has no filter (top_k 0, top_p 1,
         min_p 0), else in sorted order (scaled logit descending, equal ones by index)."""
+
+    def verify_drafts(self, logits: torch.Tensor, drafted: torch.Tensor, draft_probs: torch.Tensor | None, accept: torch.Tensor,
+                      draw: torch.Tensor, temperature: torch.Tensor, start: torch.Tensor, most: int
+                      ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Drafted tokens judged against the target's probabilities from given random numbers. Request b (of B) owns rows start[b]
+        .. start[b + 1] - 1 (start [B+1] int32) of logits [N, V] float32: row i judges drafted[i] ([N] int32), the last row none.
+        p = softmax(logits / temperature[b]), q = draft_probs[i] ([N, V] float32; None: the drafts were certain). Row i takes its
+        draft x when accept[i] q(x) <= p(x); behind the drafts taken one more token is drawn: from max(p - q, 0) where a draft was
+        turned down (where that leaves nothing: from p), from p otherwise: the first whose running sum exceeds draw[b] times the
+        whole. accept [N] and draw [B] float32 lie in [0, 1). Temperature 0 (or less): p is the first largest logit. A drafted id
+        outside the vocabulary is no draft: the row draws from p. Sums and exponentials in 64 bits; a logit that is NaN has no
+        mass; a row without any gives token 0. -> (tokens [B, most + 1] int32: those taken, the drawn one, then -1; how many were
+        taken [B] int32); a request of no rows gets -1 and 0, of its rows only the first most + 1 (at most 64) count."""
 
     def scatter_rows(self, dst: torch.Tensor, idx: torch.Tensor, src: torch.Tensor) -> None:
         """dst[idx[r]] = src[r] for int32 rows: dst [N, W], idx [n], src n * W values."""

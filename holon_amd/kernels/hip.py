@@ -15,6 +15,7 @@ import torch
 
 from . import build as _build
 from .api import AttnRows
+from .continuation import SYMBOLS as CONTINUATION_SYMBOLS, ContinuationOps
 from .registry import kernel_op
 from ..config.products import ProductPlan, row_bucket
 
@@ -79,7 +80,7 @@ def general_split_pays(blocks: int, head_dim: int, span: int) -> bool:
     return blocks <= 128 and blocks * head_dim <= 16384 and span > (128 if few and 64 < head_dim <= 128 else 256 if few else 384)
 
 
-class HipKernels:
+class HipKernels(ContinuationOps):
     name = "hip-gfx950"
     settled = False           # see `configured`
     _instance: "HipKernels | None" = None
@@ -177,6 +178,9 @@ class HipKernels:
         for name, args in sig.items():
             fn = getattr(lib, name)
             fn.argtypes, fn.restype = args, _I
+        for name, (args, result) in CONTINUATION_SYMBOLS.items():
+            fn = getattr(lib, name)
+            fn.argtypes, fn.restype = args, result
         self.plan = ProductPlan("own")            # which form a product takes where several serve it: see `configured`
         self._tiled_weights: dict[tuple, list] = {}   # weight shape -> weak (weight, tiled copy) pairs, see _alike
         self._f32_result: bool | None = None      # whether torch has a float32 result for a bfloat16 product (probed once)

@@ -39,6 +39,24 @@ def _mix32(x):
     return x ^ (x >> 16)
 
 
+def quantise_q8(x):
+    """x [..., D] -> (codes, e + 127), both uint8, of the 8-bit cache's rows."""
+    x = x.float()
+    finite = torch.where(torch.isfinite(x), x.abs(), 0.0).amax(-1)
+    mantissa, power = torch.frexp(finite)                     # finite = mantissa 2^power, 448 = 0.875 * 2^9
+    e = torch.where(finite == 0, 0, (power - 9 + (mantissa > 0.875).to(power.dtype)).clamp(min=-126))
+    y = torch.where(torch.isfinite(x), torch.ldexp(x, -e[..., None]), torch.nan)
+    return y.to(torch.float8_e4m3fn).view(torch.uint8), (e + 127).to(torch.uint8)
+
+
+def dequantise_q8(pages, scales, page_size):
+    """(keys [n, Hkv, P, D], values [n, Hkv, D, P]), float32, that the pages of an 8-bit cache stand for."""
+    n, _, hkv, wide = pages.shape
+    power = torch.ldexp(torch.ones((), device=pages.device), scales.view(torch.uint8).int() - 127)
+    x = pages.view(torch.uint8).view(torch.float8_e4m3fn).float()
+    return (x[:, 0].reshape(n, hkv, page_size, -1) * power[:, 0, :, :, None], x[:, 1].reshape(n, hkv, -1, page_size) * power[:, 1, :, None, :])
+
+
 class TorchKernels:
     name = "torch-plain"
 
@@ -230,6 +248,80 @@ class TorchKernels:
         q = self.qk_norm_rope_write(qkv, heads, kv_heads, head_dim, q_weight, k_weight, eps, rope_table, positions,
                                     pages if writes else None, write_page, write_off, page_size)
         return self.paged_attention(q, pages, table, rows, page_size, scale, window)
+
+    def check_cache_q8(self, head_dim, page_size):
+        return None
+
+    def kv_write_q8(self, k, v, pages, scales, write_page, write_off, page_size):
+        n, _, hkv, wide = pages.shape
+        codes, powers = pages.view(torch.uint8), scales.view(torch.uint8)
+        kp, vp = codes[:, 0].view(n, hkv, page_size, wide // page_size), codes[:, 1].view(n, hkv, wide // page_size, page_size)
+        page, off = write_page.long(), write_off.long()
+        there = (page >= 0) & (page < n) & (off >= 0) & (off < page_size)
+        page, off = page[there], off[there]
+        for part, x in enumerate((k[there], v[there])):
+            code, power = quantise_q8(x)
+            if part == 0:
+                kp[page, :, off] = code
+            else:
+                vp[page, :, :, off] = code
+            powers[page, part, :, off] = power
+
+    def kv_read_q8(self, pages, scales, read_page, read_off, page_size, dtype=torch.bfloat16):
+        n, _, hkv, wide = pages.shape
+        k, v = dequantise_q8(pages, scales, page_size)
+        page, off = read_page.long(), read_off.long()
+        there = ((page >= 0) & (page < n) & (off >= 0) & (off < page_size))[:, None, None]
+        page, off = page.clamp(0, n - 1), off.clamp(0, page_size - 1)
+        return tuple(torch.where(there, x, 0.0).to(dtype) for x in (k[page, :, off], v[page, :, :, off]))
+
+    def paged_attention_q8(self, q, pages, scales, table, rows, page_size, scale, window=0, sink=None):
+        k, v = dequantise_q8(pages, scales, page_size)
+        n, _, hkv, wide = pages.shape
+        held = torch.stack((k.reshape(n, hkv, wide), v.reshape(n, hkv, wide)), 1)
+        return self.paged_attention(q, held.to(_up(q).dtype), table, rows, page_size, scale, window, sink)
+
+    def prefix_attention(self, q, pages, table, rows, prefix, page_size, scale, scales=None, sink=None):
+        """The prefix is read through each row's own table: the pages are the same ones."""
+        if scales is None:
+            return self.paged_attention(q, pages, table, rows, page_size, scale, 0, sink)
+        return self.paged_attention_q8(q, pages, scales, table, rows, page_size, scale, 0, sink)
+
+    def verify_drafts(self, logits, drafted, draft_probs, accept, draw, temperature, start, most):
+        vocab, at = logits.shape[1], start.tolist()
+        tokens = torch.full((len(at) - 1, most + 1), -1, dtype=torch.int32, device=logits.device)
+        accepted = torch.zeros(len(at) - 1, dtype=torch.int32, device=logits.device)
+        for b in range(len(at) - 1):
+            heat, rows, taken = float(temperature[b]), range(at[b], min(at[b + 1], at[b] + most + 1)), 0
+            for i in rows:
+                x = logits[i].double()
+                x = torch.where(torch.isnan(x), -torch.inf, x)
+                if heat > 0:
+                    z = torch.where(x == x.max(), 0.0, (x - x.max()) / heat)
+                    e = torch.where(x == -torch.inf, 0.0, z.exp())
+                    p = e / e.sum() if e.sum() > 0 else e
+                else:
+                    p = torch.nn.functional.one_hot(x.argmax(), vocab).double()
+                draft = int(drafted[i])
+                judged = i + 1 < rows.stop and 0 <= draft < vocab
+                q = draft_probs[i].double() if draft_probs is not None else torch.nn.functional.one_hot(
+                    torch.tensor(max(0, min(draft, vocab - 1))), vocab).to(p)
+                good = judged and (float(accept[i]) * float(q[draft]) <= float(p[draft]) if heat > 0 else float(p[draft]) == 1)
+                if good:
+                    tokens[b, taken] = draft
+                    taken += 1
+                    continue
+                mass = p
+                if judged and heat > 0:
+                    left = (p - q).clamp(min=0) if draft_probs is not None else torch.where(q > 0, 0.0, p)
+                    mass = left if left.sum() > 0 else p
+                c = mass.cumsum(-1)
+                over = torch.nonzero((c > float(draw[b]) * c[-1]) & (mass > 0))
+                some = torch.nonzero(mass > 0)
+                tokens[b, taken] = int(x.argmax()) if heat <= 0 else int(over[0]) if len(over) else int(some[-1]) if len(some) else 0
+                break
+            accepted[b] = taken
+        return tokens, accepted
 
     def scatter_rows(self, dst, idx, src):
         dst[idx.long()] = src.view(idx.shape[0], dst.shape[1])

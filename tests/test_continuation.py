@@ -1,0 +1,520 @@
+"""The operators for many continuations of a context: the 8-bit paged cache written, read back and attended over, attention over
+prefixes that rows share, the verification of drafted tokens. What is exact is held to equality, attention to a bound that is
+derived from the formula's own roundings (`_bound`), the verification's whole numbers to the definition in 64 bits."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from holon_amd.kernels.api import AttnRows, SharedPrefix
+from holon_amd.kernels.continuation import ContinuationOps
+from holon_amd.kernels.hip import KernelError
+from tests.plain.ops import TorchKernels, dequantise_q8, quantise_q8
+
+PLAIN = TorchKernels()
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+# -- the format -------------------------------------------------------------------------------------------------------------
+
+def test_a_row_of_the_format():
+    """The smallest power of two that brings the largest value to 448 or less; values to half a step of four significant bits."""
+    for largest, power in ((448.0, 0), (448.5, 1), (1.0, -8), (1.75, -8), (1.7500001, -7), (0.0, 0), (2.0 ** -140, -126), (3e38, 120)):
+        x = torch.zeros(64, dtype=torch.float32)
+        x[3] = -largest
+        codes, byte = quantise_q8(x)
+        assert int(byte) - 127 == power, (largest, int(byte) - 127)
+    x = torch.randn(500, 128, generator=torch.Generator().manual_seed(1)) * torch.exp2(torch.linspace(-60, 60, 500))[:, None]
+    codes, byte = quantise_q8(x)
+    held = codes.view(E4M3).double() * torch.exp2(byte.double() - 127)[:, None]
+    step = torch.maximum(x.double().abs() * 2.0 ** -4, torch.exp2(byte.double() - 127)[:, None] * 2.0 ** -10)
+    assert ((held - x.double()).abs() <= step).all()
+    x[7, 5], x[8, 6] = float("nan"), float("inf")
+    again, byte2 = quantise_q8(x)
+    gone = torch.isnan(again.view(E4M3).float())
+    assert gone.sum() == 2 and gone[7, 5] and gone[8, 6]
+
+
+# -- steps to attend in -----------------------------------------------------------------------------------------------------
+
+def _step(rows, heads, kv, d, page, *, seed=0, shared=(), dtype=torch.bfloat16, q8=True, device="cpu", spare=3, gap=0):
+    """rows: (tokens already held, query tokens); shared: (first row, last row, prefix tokens). Pages lie about the pool in any
+    order, slots too; what no row holds is NaN."""
+    rng, g = np.random.default_rng(seed), torch.Generator().manual_seed(seed)
+    counts, lens = np.array([n for _, n in rows]), np.array([s + n for s, n in rows])
+    need = [-(-int(n) // page) for n in lens]
+    wide = max(need + [1]) + 1
+    total = sum(need) + spare
+    order = list(rng.permutation(total))
+    slots = rng.permutation(len(rows) + 2)[: len(rows)]
+    table = np.full((len(rows) + 2, wide), total, dtype=np.int64)       # the null page is the last one
+    for i, n in enumerate(need):
+        table[slots[i], :n] = [order.pop() for _ in range(n)]
+    for lo, hi, prefix in shared:
+        whole = -(-prefix // page)
+        for i in range(lo + 1, hi + 1):
+            if prefix % page:                                           # the page in which the prefix ends is copied
+                table[slots[i], : whole - 1] = table[slots[lo], : whole - 1]
+            else:
+                table[slots[i], :whole] = table[slots[lo], :whole]
+    n_pages = total + 1
+    k = torch.randn(n_pages, kv, page, d, generator=g) * torch.exp(0.6 * torch.randn(n_pages, kv, page, 1, generator=g))
+    v = torch.randn(n_pages, kv, d, page, generator=g) * torch.exp(0.6 * torch.randn(n_pages, kv, 1, page, generator=g))
+    for lo, hi, prefix in shared:
+        if prefix % page:
+            at = prefix // page
+            for i in range(lo + 1, hi + 1):
+                k[table[slots[i], at], :, : prefix % page] = k[table[slots[lo], at], :, : prefix % page]
+                v[table[slots[i], at], :, :, : prefix % page] = v[table[slots[lo], at], :, :, : prefix % page]
+    held = torch.zeros(n_pages, page, dtype=torch.bool)
+    for i, n in enumerate(lens):
+        pos = np.arange(n)
+        held[table[slots[i], pos // page], pos % page] = True
+    k[~held[:, None, :].expand(n_pages, kv, page)] = float("nan")
+    v.transpose(2, 3)[~held[:, None, :].expand(n_pages, kv, page)] = float("nan")
+    i32 = lambda a: torch.as_tensor(np.asarray(a, dtype=np.int32)).to(device)              # noqa: E731
+    dec, chk = np.flatnonzero(counts == 1), np.flatnonzero(counts > 1)
+    attn = AttnRows(slots=i32(slots), lens=i32(lens), query_start=i32(np.concatenate([[0], np.cumsum(counts)])), decode_rows=i32(dec),
+                    chunk_rows=i32(chk), n_decode=len(dec), n_chunk=len(chk), max_decode_len=int(lens[dec].max()) if len(dec) else 0,
+                    max_chunk_query=int(counts[chk].max()) if len(chk) else 0, max_chunk_len=int(lens[chk].max()) if len(chk) else 0)
+    q = (torch.randn(int(counts.sum()), heads, d, generator=g) * 1.5).to(dtype).to(device)
+    if q8:
+        kc, ke = quantise_q8(k)
+        vc, ve = quantise_q8(v.transpose(2, 3))
+        pages = torch.stack((kc.reshape(n_pages, kv, -1), vc.transpose(2, 3).reshape(n_pages, kv, -1)), 1)
+        scales = torch.stack((ke, ve), 1)
+        if gap:                                                         # a page's codes and scales in one piece of a wider row
+            both = torch.zeros(n_pages, pages[0].numel() + scales[0].numel() + gap, dtype=torch.uint8)
+            both[:, : pages[0].numel()] = pages.reshape(n_pages, -1)
+            both[:, pages[0].numel(): pages[0].numel() + scales[0].numel()] = scales.reshape(n_pages, -1)
+            both = both.to(device)
+            pages = both[:, : pages[0].numel()].view(pages.shape)
+            scales = both[:, pages[0].numel(): pages[0].numel() + scales[0].numel()].view(scales.shape)
+        pages, scales = pages.to(device).view(E4M3), scales.to(device).view(E8M0)
+    else:
+        pages, scales = torch.stack((k.reshape(n_pages, kv, -1), v.reshape(n_pages, kv, -1)), 1).to(dtype).to(device), None
+    prefix = None
+    if shared:
+        start = [lo for lo, _, _ in shared] + [shared[-1][1] + 1]
+        assert all(shared[i][1] + 1 == shared[i + 1][0] for i in range(len(shared) - 1))
+        prefix = SharedPrefix(i32(start), i32([p for _, _, p in shared]), len(shared),
+                              int(max(counts[lo: hi + 1].sum() for lo, hi, _ in shared)), max(p for _, _, p in shared))
+    return q, pages, scales, i32(table), attn, prefix
+
+
+def _want(q, pages, scales, table, rows, page, scale, window=0, sink=None):
+    """softmax(scale q k^T) v in 64 bits, and beside it sum_j w_j |v_j| and the largest sum_d |q_d k_d| a query meets: what the
+    bound is made of. Keys that a query does not see take no part, whatever they hold."""
+    d = q.shape[2]
+    if scales is not None:
+        k, v = dequantise_q8(pages.cpu(), scales.cpu(), page)
+    else:
+        n, _, hkv, wide = pages.shape
+        k, v = pages[:, 0].cpu().float().reshape(n, hkv, page, d), pages[:, 1].cpu().float().reshape(n, hkv, d, page)
+    hkv = k.shape[1]
+    group = q.shape[1] // hkv
+    out, size, dots = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(3))
+    starts, q = rows.query_start.tolist(), q.double().cpu()
+    for b, (slot, n) in enumerate(zip(rows.slots.tolist(), rows.lens.tolist())):
+        lo, hi = starts[b], starts[b + 1]
+        at = table[slot, : -(-n // page)].long().cpu()
+        kk = k[at].transpose(1, 2).reshape(-1, hkv, d)[:n].double()
+        vv = v[at].permute(0, 3, 1, 2).reshape(-1, hkv, d)[:n].double()
+        for i in range(lo, hi):
+            pos = n - (hi - lo) + i - lo
+            first = 0 if window == 0 else max(0, pos - window + 1) if window > 0 else max(0, pos) // -window * -window
+            if pos < first:
+                continue
+            for head in range(q.shape[1]):
+                ks, vs = kk[first: pos + 1, head // group], vv[first: pos + 1, head // group]
+                x = ks @ q[i, head] * scale
+                top = x.max()
+                e = torch.exp(x - top)
+                total = e.sum() + (torch.exp(sink[head].double().cpu() - top) if sink is not None else 0.0)
+                out[i, head] = (e / total) @ vs
+                size[i, head] = (e / total) @ vs.abs()
+                dots[i, head] = (ks.abs() @ q[i, head].abs()).max() * scale
+    return out, size, dots
+
+
+def _bound(want, size, dots, d, keys, dtype):
+    """By what a result may be off. A score is a sum of d products in float32 (exact products: off by at most d 2^-24 of the sum
+    of their sizes), taken times scale log2(e) (2^-23 more) into exp2 (2^-22 of its result, the instruction's own bound beside the
+    rounding of its argument): a weight moves by twice that at most, above and below the fraction's line. Sums over the keys
+    are in float32: keys 2^-24. A weight is rounded once to bfloat16 (2^-8), or split in three (2^-24 is left), the result once to its type."""
+    u = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    score = dots * (d + 4) * 2.0 ** -24
+    return size * (u + 2 * score + 2 * keys * 2.0 ** -24 + 2.0 ** -20) + u * want.abs()
+
+
+def _check(got, q, pages, scales, table, rows, page, scale, window=0, sink=None):
+    want, size, dots = _want(q, pages, scales, table, rows, page, scale, window, sink)
+    keys = int(rows.lens.max())
+    off, most = (got.double().cpu() - want).abs(), _bound(want, size, dots, q.shape[2], keys, q.dtype)
+    assert got.dtype == q.dtype and got.shape == q.shape
+    assert torch.isfinite(got).all() and (off <= most).all(), f"up to {(off / most.clamp(min=1e-300)).max().item()} of the bound"
+
+
+STEPS = [
+    # (rows, heads, kv heads, head size, page, window): one key, one page less and more, a tile of 64 less and more, several rows
+    ([(0, 1)], 4, 1, 64, 16, 0),
+    ([(15, 1), (16, 1), (62, 1), (63, 1), (64, 1), (200, 1)], 8, 2, 128, 16, 0),
+    ([(300, 1), (7, 1), (1000, 1)], 5, 1, 128, 32, 0),                       # five heads on one
+    ([(700, 1), (31, 1)], 16, 1, 256, 48, 0),                                # pages that no power of two is
+    ([(129, 1)] * 3, 20, 1, 64, 64, 0),                                      # more heads a group than a tile has columns
+    ([(500, 1), (40, 1)], 8, 2, 128, 16, 50),                                # a window
+    ([(500, 1), (40, 1), (130, 1)], 8, 2, 128, 16, -64),                     # chunks
+    ([(100, 3), (5, 1), (0, 2), (640, 5)], 8, 2, 128, 16, 0),                # drafted tokens beside decode rows
+    ([(90, 7), (0, 33)], 5, 1, 64, 16, 20),
+    ([(0, 130), (64, 65), (300, 1), (11, 6)], 8, 4, 128, 32, 0),             # prompts, portions
+    ([(100, 70), (0, 40)], 4, 2, 256, 16, 0),
+    ([(70, 90)], 14, 2, 128, 16, -32),
+]
+
+
+def test_plain_forms_agree():
+    """The twin and the 64-bit definition, and the twin's write with the format."""
+    for rows, heads, kv, d, page, window in STEPS[:6]:
+        q, pages, scales, table, attn, _ = _step(rows, heads, kv, d, page)
+        clean = pages.view(torch.uint8).clone()
+        clean[(clean & 0x7f) == 0x7f] = 0
+        got = PLAIN.paged_attention_q8(q, clean.view(E4M3), scales, table, attn, page, d ** -0.5, window)
+        _check(got, q, pages, scales, table, attn, page, d ** -0.5, window)
+
+
+# -- what is refused, without a GPU -----------------------------------------------------------------------------------------
+
+class Refusing(ContinuationOps):
+    """The checks alone: tensors may lie anywhere, nothing is launched."""
+
+    class lib:
+        holon_kv_write_q8 = holon_kv_read_q8 = holon_cache_attention = holon_verify_drafts = None
+        holon_cache_attention_room = staticmethod(lambda *a: 0)
+        holon_verify_drafts_room = staticmethod(lambda *a: 16)
+
+    def __init__(self):
+        self.launched = []
+
+    @staticmethod
+    def _place(what, t):
+        return t.device
+
+    @staticmethod
+    def _stream():
+        return 0
+
+    def _call(self, fn, *args):
+        self.launched.append(args)
+
+
+def test_refused_on_the_cpu():
+    with pytest.raises(KernelError, match="GPU tensor"):
+        ContinuationOps().kv_read_q8(torch.zeros(2, 2, 1, 1024, dtype=torch.uint8), torch.zeros(2, 2, 1, 16, dtype=torch.uint8),
+                                     torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 16)
+
+
+def test_refused_caches_and_rows():
+    ops = Refusing()
+    q, pages, scales, table, rows, _ = _step([(20, 1), (3, 2)], 4, 2, 64, 16)
+    k = torch.randn(5, 2, 64).bfloat16()
+    at = torch.zeros(5, dtype=torch.int32)
+    ops.kv_write_q8(k, k, pages, scales, at, at, 16)
+    ops.kv_write_q8(k.float(), k.float(), pages.view(torch.uint8), scales.view(torch.uint8), at, at, 16)
+    wide = torch.randn(5, 384).bfloat16()
+    ops.kv_write_q8(wide[:, :128].view(5, 2, 64), wide[:, 128:256].view(5, 2, 64), pages, scales, at, at, 16)
+    ops.kv_read_q8(pages, scales, at, at, 16, torch.float32)
+    ops.paged_attention_q8(q, pages, scales, table, rows, 16, 0.1)
+    assert len(ops.launched) == 5
+    for bad in (lambda: ops.kv_write_q8(k, k.float(), pages, scales, at, at, 16),
+                lambda: ops.kv_write_q8(k.half(), k.half(), pages, scales, at, at, 16),
+                lambda: ops.kv_write_q8(k[:, :1], k[:, :1], pages, scales, at, at, 16),
+                lambda: ops.kv_write_q8(k, wide[:, :128].view(5, 2, 64), pages, scales, at, at, 16),
+                lambda: ops.kv_write_q8(k, k, pages, scales, at.long(), at, 16),
+                lambda: ops.kv_write_q8(k, k, pages, scales, at[:4], at, 16),
+                lambda: ops.kv_write_q8(k, k, pages, scales[:, :, :, :8], at, at, 16),
+                lambda: ops.kv_write_q8(k, k, pages.view(torch.int8), scales, at, at, 16),
+                lambda: ops.kv_write_q8(k, k, pages, scales, at, at, 8),
+                lambda: ops.kv_write_q8(k, k, pages[:, :, :, :512], scales, at, at, 16),
+                lambda: ops.kv_read_q8(pages, scales, at, at, 16, torch.float16),
+                lambda: ops.kv_read_q8(pages.transpose(1, 2), scales, at, at, 16),
+                lambda: ops.paged_attention_q8(q.half(), pages, scales, table, rows, 16, 0.1),
+                lambda: ops.paged_attention_q8(q[:, :3], pages, scales, table, rows, 16, 0.1),
+                lambda: ops.paged_attention_q8(q.transpose(0, 1), pages, scales, table, rows, 16, 0.1),
+                lambda: ops.paged_attention_q8(q, pages, scales, table.long(), rows, 16, 0.1),
+                lambda: ops.paged_attention_q8(q, pages, scales, table, rows, 16, 0.0),
+                lambda: ops.paged_attention_q8(q, pages, scales, table, rows, 16, float("nan")),
+                lambda: ops.paged_attention_q8(q, pages, scales, table, rows, 16, 0.1, sink=torch.zeros(3)),
+                lambda: ops.prefix_attention(q, pages, table, rows, None, 16, 0.1)):      # 8-bit pages without scales
+        with pytest.raises(KernelError):
+            bad()
+    small = torch.zeros(2, 2, 1, 16 * 96, dtype=torch.uint8), torch.zeros(2, 2, 1, 16, dtype=torch.uint8)
+    with pytest.raises(KernelError, match="head_dim 96"):
+        ops.kv_read_q8(*small, at, at, 16)
+    odd = torch.zeros(2, 2, 1, 8 * 64, dtype=torch.uint8), torch.zeros(2, 2, 1, 8, dtype=torch.uint8)
+    with pytest.raises(KernelError):
+        ops.kv_read_q8(*odd, at, at, 8)
+    shifted = torch.zeros(4 * 2048 + 8, dtype=torch.uint8)[8:].view(4, 2, 1, 1024)
+    with pytest.raises(KernelError, match="borders of 16"):
+        ops.kv_read_q8(shifted, torch.zeros(4, 2, 1, 16, dtype=torch.uint8), at, at, 16)
+    assert len(ops.launched) == 5
+
+
+def test_refused_prefixes():
+    ops = Refusing()
+    q, pages, _, table, rows, prefix = _step([(40, 1), (41, 1)], 4, 2, 64, 16, shared=[(0, 1, 32)], q8=False)
+    ops.prefix_attention(q, pages, table, rows, prefix, 16, 0.1)
+    with pytest.raises(KernelError):                                    # the float32 path keeps paged_attention
+        ops.prefix_attention(q.float(), pages.float(), table, rows, prefix, 16, 0.1)
+    with pytest.raises(KernelError, match="group_start"):
+        ops.prefix_attention(q, pages, table, rows, SharedPrefix(prefix.group_start[:1], prefix.lens, 1, 2, 32), 16, 0.1)
+    with pytest.raises(KernelError, match="prefix lens"):
+        ops.prefix_attention(q, pages, table, rows, SharedPrefix(prefix.group_start, prefix.lens.float(), 1, 2, 32), 16, 0.1)
+    assert len(ops.launched) == 1
+
+
+def test_refused_drafts():
+    ops = Refusing()
+    n, b = 7, 2
+    good = dict(logits=torch.zeros(n, 50), drafted=torch.zeros(n, dtype=torch.int32), draft_probs=torch.zeros(n, 50), accept=torch.zeros(n),
+                draw=torch.zeros(b), temperature=torch.ones(b), start=torch.tensor([0, 3, 7], dtype=torch.int32), most=4)
+    ops.verify_drafts(**good)
+    for name, bad in (("logits", torch.zeros(n, 50).bfloat16()), ("logits", torch.zeros(50, n).t()), ("drafted", torch.zeros(n).long()),
+                      ("draft_probs", torch.zeros(n, 49)), ("draft_probs", torch.zeros(n, 50).double()), ("accept", torch.zeros(n - 1)),
+                      ("draw", torch.zeros(b + 1)), ("temperature", torch.ones(b).double()), ("start", torch.zeros(b, dtype=torch.int32)),
+                      ("most", 64), ("most", -1)):
+        with pytest.raises(KernelError):
+            ops.verify_drafts(**{**good, name: bad})
+    assert len(ops.launched) == 1
+
+
+# -- the kernels --------------------------------------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def hip():
+    from holon_amd.kernels import load_hip
+    return load_hip()
+
+
+gpu = pytest.mark.gpu
+
+
+def _blank(n, kv, page, d, seed, gap=0):
+    """A pool full of other bytes: whatever a write leaves alone shows."""
+    g = torch.Generator().manual_seed(seed)
+    codes, scales = 2 * kv * page * d, 2 * kv * page
+    both = torch.randint(0, 256, (n, codes + scales + gap), generator=g, dtype=torch.uint8)
+    return both, lambda x: (x[:, :codes].view(n, 2, kv, page * d), x[:, codes: codes + scales].view(n, 2, kv, page))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(("t", "kv", "d", "page", "gap"), [(1, 1, 64, 16, 0), (1, 8, 128, 16, 0), (8, 8, 128, 16, 16), (37, 3, 128, 32, 0),
+                                                           (100, 2, 256, 16, 0), (33, 1, 64, 48, 32), (513, 4, 128, 64, 0), (16, 2, 256, 32, 0)])
+def test_write_and_read_back(hip, t, kv, d, page, gap, dtype):
+    """Bytes equal the format's wherever a token goes, and nothing else of the pool changes; what is read back is what they stand for."""
+    g = torch.Generator().manual_seed(t + d)
+    rows = (torch.randn(t, 3 * kv * d, generator=g) * torch.exp(3 * torch.randn(t, 1, generator=g))).to(dtype)
+    rows[0, 0], rows[-1, -1], rows[t // 2, kv * d] = float("nan"), float("inf"), float("-inf")
+    rows[t // 3, : kv * d] = 0
+    rows[-1, kv * d: 2 * kv * d] = 2.0 ** -133                     # bfloat16's smallest
+    k, v = rows[:, kv * d: 2 * kv * d].view(t, kv, d), rows[:, 2 * kv * d:].view(t, kv, d)       # columns of wider rows
+    n = t // page + 9
+    for run in ("in order", "anywhere", "some nowhere"):
+        rng = np.random.default_rng(t)
+        if run == "in order":                                     # from the middle of a page on
+            order, first = rng.permutation(n), min(5, page - 1)
+            at = np.arange(t) + first
+            wp, wo = order[at // page], at % page
+        else:
+            at = rng.permutation(n * page)[:t]
+            wp, wo = at // page, at % page
+            if run == "some nowhere":
+                wp, wo = wp.copy(), wo.copy()
+                wp[::3], wo[1::5] = np.where(np.arange(t)[::3] % 2, -1, n), np.where(np.arange(t)[1::5] % 2, -7, page)
+        wp, wo = (torch.as_tensor(x.astype(np.int32)) for x in (wp, wo))
+        both, views = _blank(n, kv, page, d, t, gap)
+        want = both.clone()
+        PLAIN.kv_write_q8(k, v, *views(want), wp, wo, page)
+        got = both.cuda()
+        hip.kv_write_q8(rows.cuda()[:, kv * d: 2 * kv * d].view(t, kv, d), rows.cuda()[:, 2 * kv * d:].view(t, kv, d),
+                        *views(got), wp.cuda(), wo.cuda(), page)
+        a, b = views(want), views(got.cpu())
+        nan = (a[0] & 0x7f) == 0x7f
+        assert torch.equal((b[0] & 0x7f) == 0x7f, nan) and torch.equal(a[0][~nan], b[0][~nan]), run
+        assert torch.equal(a[1], b[1]) and torch.equal(got.cpu()[:, want.shape[1] - gap:], both[:, want.shape[1] - gap:]), run
+        pages, scales = views(got)
+        for into in (torch.bfloat16, torch.float32):
+            seen = hip.kv_read_q8(pages, scales, wp.cuda(), wo.cuda(), page, into)
+            true = PLAIN.kv_read_q8(*views(got.cpu()), wp, wo, page, into)
+            for x, y in zip(seen, true):
+                assert x.dtype == into and torch.equal(torch.isnan(x.cpu()), torch.isnan(y))
+                assert torch.equal(torch.nan_to_num(x.cpu(), 0.0), torch.nan_to_num(y, 0.0)), (run, into)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("step", range(len(STEPS)))
+def test_attention_over_the_8_bit_cache(hip, step, dtype):
+    rows, heads, kv, d, page, window = STEPS[step]
+    print(f"step {step} {dtype}", flush=True)
+    args = _step(rows, heads, kv, d, page, seed=step, dtype=dtype, device="cuda", gap=16 * (step % 3))[:5]
+    q, pages, scales, table, attn = args
+    got = hip.paged_attention_q8(q, pages, scales, table, attn, page, d ** -0.5, window)
+    _check(got, q, pages, scales, table, attn, page, d ** -0.5, window)
+    sink = torch.linspace(-2, 3, heads).cuda()
+    got = hip.paged_attention_q8(q, pages, scales, table, attn, page, d ** -0.5, window, sink)
+    _check(got, q, pages, scales, table, attn, page, d ** -0.5, window, sink)
+
+
+@gpu
+def test_long_contexts_are_cut_and_joined(hip):
+    for rows, heads, kv, d, dtype in (([(5000, 1)], 4, 1, 128, torch.bfloat16), ([(9000, 1), (37, 1)], 2, 1, 64, torch.float32),
+                                      ([(6000, 4), (100, 2)], 4, 1, 128, torch.bfloat16), ([(4100, 1)], 2, 1, 256, torch.bfloat16)):
+        q, pages, scales, table, attn, _ = _step(rows, heads, kv, d, 16, seed=3, dtype=dtype, device="cuda")
+        got = hip.paged_attention_q8(q, pages, scales, table, attn, 16, d ** -0.5)
+        _check(got, q, pages, scales, table, attn, 16, d ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("q8", [True, False])
+def test_what_a_query_does_not_see_does_not_reach_it(hip, q8):
+    """A value (and a key) that is no number, or infinite, inside a portion: queries in front of it and behind its window get what
+    they get without it, those that see it get no finite number."""
+    for rows, heads, d, at, window in (([(50, 40)], 4, 128, 70, 0), ([(3, 9)], 5, 64, 6, 0), ([(100, 300)], 2, 128, 250, 0), ([(100, 90)], 4, 128, 130, 24)):
+        if window and not q8:
+            continue
+        for part, value in ((1, float("nan")), (0, float("nan")), (1, float("inf")), (1, float("-inf"))):
+            q, pages, scales, table, attn, _ = _step(rows, heads, 1, d, 16, seed=at, device="cuda", q8=q8)
+            run = (lambda: hip.paged_attention_q8(q, pages, scales, table, attn, 16, d ** -0.5, window)) if q8 else \
+                (lambda: hip.prefix_attention(q, pages, table, attn, None, 16, d ** -0.5))
+            clean = run()
+            page, off = int(table[attn.slots[0], at // 16]), at % 16
+            odd = torch.tensor([0x7f], dtype=torch.uint8, device="cuda").view(E4M3) if q8 else torch.tensor([value], dtype=torch.bfloat16, device="cuda")
+            if part == 0:
+                pages[page, 0, 0, off * d + 5] = odd[0]
+            else:
+                pages[page, 1, 0].view(d, 16)[5, off] = odd[0]
+            got = run()
+            pos = torch.arange(rows[0][0], sum(rows[0]))
+            sees = (pos >= at) & ((pos < at + window) if window else torch.ones_like(pos, dtype=torch.bool))
+            assert torch.equal(got[~sees], clean[~sees])
+            hit = got[sees][:, :, 5] if part == 1 else got[sees]
+            if part == 1 and not q8 and value == value:
+                assert (hit == value).all()
+            else:
+                assert torch.isnan(hit).all()
+            if part == 1:
+                others = [i for i in range(d) if i != 5]
+                assert torch.equal(got[:, :, others], clean[:, :, others])
+
+
+@gpu
+def test_rows_that_see_nothing(hip):
+    """A row of length 0 and queries that lie before the sequence give zeros; their neighbours are as ever."""
+    q, pages, scales, table, attn, _ = _step([(9, 1), (30, 1), (12, 4)], 4, 2, 64, 16, device="cuda")
+    attn.lens[0] = 0
+    attn.lens[2] = 2                                              # four queries of a sequence of two tokens
+    got = hip.paged_attention_q8(q, pages, scales, table, attn, 16, 0.125)
+    assert not got[0].any() and not got[2:4].any() and got[4:].any()
+    _check(got, q, pages, scales, table, attn, 16, 0.125)
+
+
+SHARED = [
+    # (rows, groups, heads, kv heads, head size, page): a prefix of one page, one that ends inside a page, several groups, drafted tokens
+    ([(20, 1), (40, 1)], [(0, 1, 16)], 4, 1, 64, 16),
+    ([(300, 1), (290, 1), (257, 1), (310, 1)], [(0, 3, 250)], 8, 2, 128, 16),
+    ([(100, 1)] * 5 + [(700, 1)] * 3 + [(50, 1)], [(0, 4, 64), (5, 7, 640)], 10, 2, 128, 32),      # and a row in no group
+    ([(130, 5), (128, 5), (150, 5)], [(0, 2, 128)], 5, 1, 128, 16),
+    ([(64, 1)] * 3 + [(200, 3)] * 2, [(0, 2, 64), (3, 4, 192)], 16, 1, 256, 64),
+    ([(129, 70), (128, 2), (500, 1)], [(0, 2, 128)], 4, 2, 64, 16),                                 # a portion in the group
+    ([(1000, 1)] * 40, [(0, 39, 992)], 8, 1, 128, 16),                                              # more columns than a block takes
+    ([(30, 1), (31, 1)], [(0, 0, 0), (1, 1, 16)], 4, 1, 64, 16),                                    # nothing shared, a row by itself
+]
+
+
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("step", range(len(SHARED)))
+def test_attention_over_a_shared_prefix(hip, step, q8):
+    rows, shared, heads, kv, d, page = SHARED[step]
+    print(f"step {step} 8-bit {q8}", flush=True)
+    q, pages, scales, table, attn, prefix = _step(rows, heads, kv, d, page, seed=step, shared=shared, q8=q8, device="cuda")
+    sink = torch.linspace(-2, 3, heads).cuda()
+    for s in (None, sink):
+        got = hip.prefix_attention(q, pages, table, attn, prefix, page, d ** -0.5, scales, s)
+        _check(got, q, pages, scales, table, attn, page, d ** -0.5, 0, s)
+
+
+def _drafts(counts, vocab, seed, *, probs=True, spread=2.5):
+    g = torch.Generator().manual_seed(seed)
+    start = [0] + list(np.cumsum(counts))
+    n, b = start[-1], len(counts)
+    logits = torch.randn(n, vocab, generator=g) * spread
+    q = torch.softmax(logits + 0.7 * torch.randn(n, vocab, generator=g), -1)
+    return dict(logits=logits, drafted=torch.multinomial(q, 1, generator=g)[:, 0].int() if n else torch.zeros(0, dtype=torch.int32),
+                draft_probs=q if probs else None, accept=torch.rand(n, generator=g), draw=torch.rand(b, generator=g),
+                temperature=(0.5 + torch.rand(b, generator=g)) * (torch.arange(b) % 4 != 3), start=torch.tensor(start, dtype=torch.int32),
+                most=max(list(counts) + [1]) - 1)
+
+
+def _verify(hip, case):
+    want = PLAIN.verify_drafts(**case)
+    got = hip.verify_drafts(**{k: x.cuda() if torch.is_tensor(x) else x for k, x in case.items()})
+    for x, y in zip(got, want):
+        assert x.dtype == torch.int32 and torch.equal(x.cpu(), y), (x.cpu().tolist(), y.tolist())
+    return want
+
+
+@gpu
+@pytest.mark.parametrize(("counts", "vocab"), [([1], 7), ([4], 1000), ([5, 3, 1, 5, 2], 4096), ([3] * 9, 4097), ([2, 0, 4], 8190), ([64, 1], 333),
+                                               ([4, 4], 50001), ([6], 151936)])
+@pytest.mark.parametrize("probs", [True, False])
+def test_verify(hip, counts, vocab, probs):
+    taken = []
+    for seed in range(4):
+        taken += _verify(hip, _drafts(counts, vocab, seed, probs=probs))[1].tolist()
+    assert not probs or len(counts) < 3 or max(taken) > 0
+
+
+@gpu
+def test_verify_at_the_borders(hip):
+    """Numbers of 0 and next to 1, drafts that are none, certain rows, rows without mass, infinite logits and ones that are no number."""
+    for seed, probs in ((0, True), (1, False)):
+        case = _drafts([4] * 8, 5000, seed, probs=probs)
+        case["accept"][::3], case["accept"][1::3] = 0.0, 1.0 - 2.0 ** -24
+        case["draw"][::2], case["draw"][1::2] = 0.0, 1.0 - 2.0 ** -24
+        _verify(hip, case)
+        case["drafted"][::5], case["drafted"][2::7] = -1, 5000
+        _verify(hip, case)
+        case["logits"][3] = float("-inf")
+        case["logits"][5, :4000] = float("-inf")
+        case["logits"][9, 17], case["logits"][9, 4900] = float("inf"), float("inf")
+        case["logits"][12, ::2] = float("nan")
+        case["logits"][14] = float("nan")
+        case["logits"][0:4] = 0.0                                  # all alike
+        _verify(hip, case)
+        case["temperature"][:] = 0
+        _verify(hip, case)
+        case["temperature"][:] = torch.tensor([1e-30, 1e-3, 0.05, 3e38, float("inf"), 50.0, 1.0, -1.0])
+        _verify(hip, case)
+    same = _drafts([5] * 4, 3001, 3)
+    same["draft_probs"] = torch.softmax(same["logits"], -1)       # drafts from the target itself
+    same["temperature"][:] = 1
+    assert _verify(hip, same)[1].sum() >= 14
+
+
+@gpu
+def test_verify_keeps_the_targets_law(hip):
+    """Whatever the drafts come from, the first token is distributed as p: frequencies over many numbers within five standard errors."""
+    vocab, n = 11, 30000
+    g = torch.Generator().manual_seed(5)
+    logits, other = torch.randn(vocab, generator=g), torch.randn(vocab, generator=g) * 1.5
+    p, q = torch.softmax(logits.double(), -1), torch.softmax(other, -1)
+    drafted = torch.zeros(2 * n, dtype=torch.int32)
+    drafted[::2] = torch.multinomial(q, n, replacement=True, generator=g).int()
+    tokens, _ = hip.verify_drafts(logits.expand(2 * n, -1).contiguous().cuda(), drafted.cuda(), q.expand(2 * n, -1).contiguous().cuda(),
+                                  torch.rand(2 * n, generator=g).cuda(), torch.rand(n, generator=g).cuda(), torch.ones(n).cuda(),
+                                  torch.arange(0, 2 * n + 1, 2, dtype=torch.int32).cuda(), 1)
+    seen = torch.bincount(tokens[:, 0].cpu().long(), minlength=vocab).double() / n
+    assert ((seen - p).abs() <= 5 * torch.sqrt(p * (1 - p) / n)).all()
