@@ -17,6 +17,7 @@ namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 struct CacheArgs {
@@ -65,6 +66,30 @@ __device__ __forceinline__ int shared_keys(const CacheArgs& a, int row) {
     before += __popcll(__ballot(j <= a.n_groups && a.group_start[min(j, a.n_groups)] <= row));
   }
   return before >= 1 && before <= a.n_groups ? max(a.group_lens[before - 1], 0) : 0;
+}
+
+// Whose queries a block takes, and which keys: queries qs .. qs + nq - 1 against keys from .. n - 1 of a row, the last of them at
+// position n - 1; or all queries of a group's rows against the prefix of n keys, which every one of them sees whole.
+struct Job {
+  int row, qs, nq, n, from;
+};
+__device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) {
+  Job j;
+  if (by_group) {
+    j.row = a.group_start[at];
+    const int end = a.group_start[at + 1];
+    j.qs = a.qstart[j.row];
+    j.n = a.group_lens[at];
+    j.nq = end > j.row && j.n > 0 ? a.qstart[end] - j.qs : 0;
+    j.from = 0;
+  } else {
+    j.row = a.row_ids[at];
+    j.qs = a.qstart[j.row];
+    j.nq = a.qstart[j.row + 1] - j.qs;
+    j.n = a.lens[j.row];
+    j.from = shared_keys(a, j.row);
+  }
+  return j;
 }
 
 // Sixteen codes as 16 bfloat16 values times `power`, in order.
@@ -140,7 +165,7 @@ constexpr int most_waves(int D, bool f32, int NT) { return D == 256 || f32 || NT
 constexpr bool two_tiles(int D, bool f32) { return D <= 128 && !f32; }
 
 template <int D, bool Q8, typename QT, int NT>
-__global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::value, NT)) cache_rows_kernel(CacheArgs a) {
+__global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::value, NT)) cache_rows_kernel(CacheArgs a, int by_group, int max_query) {
   constexpr int PARTS = std::is_same<QT, float>::value ? 3 : 1;
   constexpr int KB = Q8 ? 64 : 32, RUN = KB / 4, SCORES = KB / 16, PV = KB / 32;
   constexpr int KLOADS = Q8 ? D / 64 : D / 32;             // 16-byte loads of a key's share
@@ -148,18 +173,21 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
   extern __shared__ __attribute__((aligned(16))) float red[];   // [waves - 1][NT][16 D values, 16 maxima, 16 sums]
   const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, waves = blockDim.x / WAVE;
   const int g = lane / 16, c = lane % 16;
-  const int ri = blockIdx.z, hk = blockIdx.y, row = a.row_ids[ri];
+  const int ri = blockIdx.z, hk = blockIdx.y;
   const int group = a.heads / a.kv_heads, P = a.page_size;
   const int out_splits = a.splits / waves;
   const int tile0 = blockIdx.x / out_splits * NT, piece = blockIdx.x % out_splits;
-  const int qs = a.qstart[row], nq = a.qstart[row + 1] - qs, n = a.lens[row];
-  if (tile0 * 16 >= nq * group) return;                    // (the same for the whole block: a shorter row's)
+  const Job job = job_of(a, by_group, ri);
+  const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
+  if (tile0 * 16 >= nq * group || (!by_group && nq > max_query)) return;      // (the same for the whole block)
   Column col[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) col[t] = column_of(a, (tile0 + t) * 16 + c, hk, group, qs, nq, n);
-  const int pos_first = n - nq + tile0 * 16 / group;                               // the tiles' first and last positions
-  const int pos_last = n - nq + min((tile0 + NT) * 16 - 1, nq * group - 1) / group;
-  const int from = max(shared_keys(a, row), 0);
+  for (int t = 0; t < NT; ++t) {
+    col[t] = column_of(a, (tile0 + t) * 16 + c, hk, group, qs, nq, n);
+    if (by_group) col[t].pos = n - 1;
+  }
+  const int pos_first = by_group ? n - 1 : n - nq + tile0 * 16 / group;            // the tiles' first and last positions
+  const int pos_last = by_group ? n - 1 : n - nq + min((tile0 + NT) * 16 - 1, nq * group - 1) / group;
   const int first = max(from, first_seen(pos_first, a.window)), whole_from = max(from, first_seen(pos_last, a.window));
   const int base = first / KB * KB;
   const int share = max(KB, ((pos_last - base + a.splits) / a.splits + KB - 1) / KB * KB);
@@ -171,7 +199,7 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
 
   Tiles<D, NT> tl;
   tl.clear();
-  if (n > 0 && nq > 0 && key_lo <= key_hi) {
+  if (key_lo <= key_hi) {
     const int32_t* trow = table_row(a, row);
     const int max_page = a.table_stride - 1;
     bf16x8_t qf[NT][PARTS][D / 32];
@@ -302,7 +330,7 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
       }
       // Where queries of the tiles see different keys, a value that is not finite reaches those alone that see it: it leaves
       // the product (zero times it is no number) and sets their sums by itself.
-      if (!whole && nq > 1) {
+      if (!whole && nq > 1 && !by_group) {
         bool odd = false;
 #pragma unroll
         for (int ds = 0; ds < D / 16; ++ds)
@@ -410,102 +438,501 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
 #pragma unroll
       for (int ds = 0; ds < D / 16; ++ds) *reinterpret_cast<f32x4_t*>(po + 16 * ds) = tl.o[t][ds];
       if (g == 0) { a.part_ml[2 * cell] = tl.m[t]; a.part_ml[2 * cell + 1] = tl.l[t]; }
+      if (a.part_first > 0 && from == 0 && piece == 0) {   // no prefix: its parts are another launch's, which leaves this row out
+        const int64_t none = (place * a.heads + col[t].head) * a.parts;
+        for (int i = g; i < a.part_first; i += 4) { a.part_ml[2 * (none + i)] = -INFINITY; a.part_ml[2 * (none + i) + 1] = 0.f; }
+      }
     }
   }
 }
 
-// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over a cell's parts, in their order: a block of D / 4 threads a
-// (token, head).
-template <int D, typename QT>
-__global__ void __launch_bounds__(D / 4) cache_merge_kernel(CacheArgs a) {
-  const int ri = blockIdx.z, qi = blockIdx.y, head = blockIdx.x, tid = threadIdx.x;
-  const int row = a.row_ids[ri], qs = a.qstart[row], nq = a.qstart[row + 1] - qs, token = qs + qi;
-  if (qi >= nq || (uint32_t)token >= (uint32_t)a.n_tokens) return;
-  const int64_t place = a.cell_queries > 0 ? (int64_t)ri * a.cell_queries + qi : token;
-  const int64_t cell = (place * a.heads + head) * a.parts;
-  float big = -INFINITY;
-  bool odd = false;
-  for (int i = 0; i < a.parts; ++i) {
-    big = fmaxf(big, a.part_ml[2 * (cell + i)]);
-    odd |= !(a.part_ml[2 * (cell + i) + 1] >= 0.f);        // a sum that is no number
+// Many columns over the same keys: a portion's queries, or all queries of a group's rows over their prefix. A block of four waves
+// takes 128 columns, a wave 32 on v_mfma_f32_32x32x16_bf16, and walks the keys in stages of 32, which its threads bring into LDS
+// as bfloat16 (codes are widened once a block, not once a wave): two buffers, and in registers the stage after the next.
+//   S^T (32 keys x 32 columns): A = 32 keys x 16 dims: lane (h, c) reads row c of the stage's keys, dims 8 h .. + 7 of 16. Row
+//     8 i + 4 h + r holds key 16 (i / 2) + 8 h + 4 (i % 2) + r, so that a lane's 16 scores are, in order, those of keys 8 h .. + 7
+//     of the stage's first 16 and of its last: the B operands of
+//   O^T (32 dims x 32 columns) += V^T P^T: A = 32 dims x 16 keys, the values transposed as in the pages.
+// Rows of LDS are swizzled by pieces of 16 bytes, so that 16 lanes that read one piece of 16 rows touch every bank once.
+template <int D, bool Q8>
+struct Stage {
+  static constexpr int K_BYTES = 32 * D * 2, BYTES = 2 * K_BYTES;
+  static constexpr int N = Q8 ? D / 64 : D / 32;           // 16-byte loads a thread, keys first, then values
+  static constexpr int HALF = Q8 ? 2 * D : 4 * D;          // loads of keys in all
+  u32x4_t w[N];
+  uint32_t ks[N];                                          // a key's scale
+  uint32_t vs;                                             // threads 0 .. 31: a value's
+
+  static __device__ __forceinline__ int row_of(int key) { return 8 * (2 * (key / 16) + key % 8 / 4) + 4 * (key % 16 / 8) + key % 4; }
+  static __device__ __forceinline__ int swizzle(int row) { return D == 64 ? row / 2 % 8 : row % 16; }
+
+  // Asks for the stage at kb, whose halves lie in pages e0 and e1.
+  __device__ __forceinline__ void load(const CacheArgs& a, int hk, int kb, int64_t e0, int64_t e1) {
+    constexpr int B = Q8 ? 1 : 2;
+    const int P = a.page_size, tid = threadIdx.x;
+    const int64_t plane = (int64_t)P * D * B;
+    const int off0 = kb % P, off1 = (kb + 16) % P;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + 256 * i;
+      if (idx < HALF) {
+        constexpr int CH = D * B / 16;
+        const int key = idx / CH, second = key / 16;
+        const int64_t page = second ? e1 : e0;
+        const int at = (second ? off1 : off0) + key % 16;
+        w[i] = *reinterpret_cast<const u32x4_t*>(a.pages + page * a.page_stride + hk * plane + (int64_t)at * D * B + idx % CH * 16);
+        if constexpr (Q8) ks[i] = a.scales[page * a.scale_stride + (int64_t)hk * P + at];
+      } else {
+        constexpr int CH = 2 * B;                          // pieces of a dim's 32 keys
+        const int v = idx - HALF, dim = v / CH, piece = v % CH, second = piece / B;
+        const int64_t page = second ? e1 : e0;
+        const int at = (second ? off1 : off0) + piece % B * 8;
+        w[i] = *reinterpret_cast<const u32x4_t*>(a.pages + page * a.page_stride + (a.kv_heads + hk) * plane + ((int64_t)dim * P + at) * B);
+      }
+    }
+    if constexpr (Q8) {
+      if (tid < 32) vs = a.scales[(tid < 16 ? e0 : e1) * a.scale_stride + (int64_t)(a.kv_heads + hk) * P + (tid < 16 ? off0 : off1) + tid % 16];
+    }
   }
+  // Puts it into LDS. Values of keys outside [lo, hi] are cleared (they are not the row's). `watch`: so are values that are not
+  // finite, and `up` and `down` (a word a dim, a bit a key) say where those were that are +inf or NaN, -inf or NaN; the
+  // answer is whether there were any.
+  __device__ __forceinline__ bool store(unsigned char* lds, float* powers, uint8_t* up, uint8_t* down, int kb, int lo, int hi, bool watch) {
+    const int tid = threadIdx.x;
+    const bool edge = kb < lo || kb + 31 > hi;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + 256 * i;
+      if (idx < HALF) {
+        constexpr int CH = D * (Q8 ? 1 : 2) / 16;
+        const int row = row_of(idx / CH), ch = idx % CH;
+        unsigned char* to = lds + row * (2 * D);
+        if constexpr (Q8) {
+          bf16x8_t x, y;
+          widen(w[i], q8_power(ks[i]), x, y);
+          *reinterpret_cast<bf16x8_t*>(to + 16 * ((2 * ch) ^ swizzle(row))) = x;
+          *reinterpret_cast<bf16x8_t*>(to + 16 * ((2 * ch + 1) ^ swizzle(row))) = y;
+        } else {
+          *reinterpret_cast<u32x4_t*>(to + 16 * (ch ^ swizzle(row))) = w[i];
+        }
+      } else {
+        constexpr int CH = Q8 ? 2 : 4;
+        const int v = idx - HALF, dim = v / CH, piece = v % CH;
+        if (edge) {
+          const int key = kb + piece * (Q8 ? 16 : 8);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t keep = 0;
+#pragma unroll
+            for (int e = 0; e < (Q8 ? 4 : 2); ++e) {
+              const int k = key + (Q8 ? 4 : 2) * x + e;
+              keep |= k >= lo && k <= hi ? (Q8 ? 0xffu << (8 * e) : 0xffffu << (16 * e)) : 0u;
+            }
+            w[i][x] &= keep;
+          }
+        }
+        if (watch) {
+          uint32_t ups = 0, downs = 0;
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int e = 0; e < (Q8 ? 4 : 2); ++e) {
+              const int shift = (Q8 ? 8 : 16) * e, k = (Q8 ? 4 : 2) * x + e;
+              const uint32_t v = w[i][x] >> shift & (Q8 ? 0xffu : 0xffffu), size = v & (Q8 ? 0x7fu : 0x7fffu);
+              if (size < (Q8 ? 0x7fu : 0x7f80u)) continue;
+              w[i][x] &= ~((Q8 ? 0xffu : 0xffffu) << shift);
+              if (Q8 || size > 0x7f80u || !(v & 0x8000u)) ups |= 1u << k;
+              if (Q8 || size > 0x7f80u || (v & 0x8000u)) downs |= 1u << k;
+            }
+          odd |= (ups | downs) != 0;
+          if constexpr (Q8) {
+            *reinterpret_cast<uint16_t*>(up + 4 * dim + 2 * piece) = (uint16_t)ups;
+            *reinterpret_cast<uint16_t*>(down + 4 * dim + 2 * piece) = (uint16_t)downs;
+          } else {
+            up[4 * dim + piece] = (uint8_t)ups;
+            down[4 * dim + piece] = (uint8_t)downs;
+          }
+        }
+        const int half = Q8 ? piece : piece / 2;
+        unsigned char* to = lds + K_BYTES + half * (K_BYTES / 2) + dim * 32;
+        const int turn = dim / 8 % 2;
+        if constexpr (Q8) {
+          bf16x8_t x, y;
+          widen(w[i], 1.f, x, y);
+          *reinterpret_cast<bf16x8_t*>(to + 16 * turn) = x;
+          *reinterpret_cast<bf16x8_t*>(to + 16 * (1 ^ turn)) = y;
+        } else {
+          *reinterpret_cast<u32x4_t*>(to + 16 * (piece % 2 ^ turn)) = w[i];
+        }
+      }
+    }
+    if constexpr (Q8) {
+      if (tid < 32) powers[tid] = kb + tid >= lo && kb + tid <= hi ? q8_power(vs) : 0.f;
+    }
+    return odd;
+  }
+  static __device__ __forceinline__ bf16x8_t key(const unsigned char* lds, int ds) {
+    const int lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
+    return *reinterpret_cast<const bf16x8_t*>(lds + c * (2 * D) + 16 * ((2 * ds + h) ^ swizzle(c)));
+  }
+  static __device__ __forceinline__ bf16x8_t value(const unsigned char* lds, int db, int half) {
+    const int lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
+    return *reinterpret_cast<const bf16x8_t*>(lds + K_BYTES + half * (K_BYTES / 2) + (32 * db + c) * 32 + 16 * (h ^ (c / 8 % 2)));
+  }
+};
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(CacheArgs a, int by_group, int less_than) {
+  using S = Stage<D, Q8>;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][S::BYTES];
+  __shared__ __attribute__((aligned(16))) float powers[2][32];
+  __shared__ uint32_t ups[2][D], downs[2][D];
+  __shared__ int odd_stage[2];                             // the key of a stage with values that are not finite
+  const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
+  const int hk = blockIdx.x, piece = blockIdx.y % a.splits, group = a.heads / a.kv_heads;
+  // the last columns first: theirs are the longest walks
+  const int tile = gridDim.y / a.splits - 1 - blockIdx.y / a.splits;
+  const Job job = job_of(a, by_group, blockIdx.z);
+  const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
+  const int columns = nq * group;
+  if (tile * 128 >= columns || (!by_group && nq <= less_than)) return;
+  const int f0 = tile * 128 + 32 * wave, f = f0 + c;
+  Column col = column_of(a, f, hk, group, qs, nq, n);
+  const int behind = n - nq;                               // the first query's position
+  const int pos_first = by_group ? n - 1 : behind + tile * 128 / group;
+  const int pos_last = by_group ? n - 1 : behind + min(tile * 128 + 127, columns - 1) / group;
+  if (by_group) col.pos = n - 1;
+  const int tile_first = by_group ? n - 1 : behind + f0 / group;
+  const int tile_last = f0 >= columns ? -1 : by_group ? n - 1 : behind + min(f0 + 31, columns - 1) / group;
+  const int first = max(from, first_seen(pos_first, a.window)), whole_from = max(from, first_seen(tile_last, a.window));
+  const int from_here = max(from, first_seen(col.pos, a.window));
+  const int base = first / 32 * 32;
+  const int share = max(32, ((pos_last - base + a.splits) / a.splits + 31) / 32 * 32);
+  const int lo = max(base + piece * share, first), hi = min(pos_last, base + piece * share + share - 1);
+
+  f32x16_t o[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (lo <= hi) {
+    bf16x8_t qf[D / 16];
+    const bf16_t* qp = (const bf16_t*)a.q + ((int64_t)col.token * a.heads + col.head) * D + 8 * h;
+#pragma unroll
+    for (int ds = 0; ds < D / 16; ++ds) {
+      u32x4_t x = {0, 0, 0, 0};
+      if (col.valid) x = *reinterpret_cast<const u32x4_t*>(qp + 16 * ds);
+      qf[ds] = __builtin_bit_cast(bf16x8_t, x);
+    }
+    const int32_t* trow = table_row(a, row);
+    const int max_page = a.table_stride - 1, P = a.page_size;
+    const auto look = [&](int kb, int64_t (&e)[2]) {
+      e[0] = page_at(a, trow[min(kb / P, max_page)]);
+      e[1] = page_at(a, trow[min((kb + 16) / P, max_page)]);
+    };
+    // queries of the block see different keys from here on, or up to here
+    const auto differs = [&](int kb) { return kb + 31 > pos_first || kb < first_seen(pos_last, a.window); };
+    const int kb_first = lo / 32 * 32;
+    if (threadIdx.x < 2) odd_stage[threadIdx.x] = -1;
+    S now, next, after;
+    int64_t e[2];
+    look(kb_first, e);
+    now.load(a, hk, kb_first, e[0], e[1]);
+    if (kb_first + 32 <= hi) {
+      look(kb_first + 32, e);
+      next.load(a, hk, kb_first + 32, e[0], e[1]);
+    }
+    if (kb_first + 64 <= hi) look(kb_first + 64, e);
+    lds_barrier();
+    if (now.store(lds[0], powers[0], (uint8_t*)ups[0], (uint8_t*)downs[0], kb_first, lo, hi, differs(kb_first))) odd_stage[0] = kb_first;
+    lds_barrier();
+    int buf = 0;
+    for (int kb = kb_first; kb <= hi; kb += 32) {
+      if (kb + 64 <= hi) {
+        after.load(a, hk, kb + 64, e[0], e[1]);
+        if (kb + 96 <= hi) look(kb + 96, e);
+      }
+      const unsigned char* st = lds[buf];
+      if (kb <= tile_last && kb + 31 >= (a.window ? first_seen(tile_first, a.window) : 0)) {
+        f32x16_t sc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+        constexpr int AT_ONCE = D / 16 < 8 ? D / 16 : 8;
+#pragma unroll
+        for (int d0 = 0; d0 < D / 16; d0 += AT_ONCE) {
+          bf16x8_t kf[AT_ONCE];
+#pragma unroll
+          for (int ds = 0; ds < AT_ONCE; ++ds) kf[ds] = S::key(st, d0 + ds);
+#pragma unroll
+          for (int ds = 0; ds < AT_ONCE; ++ds) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ds], qf[d0 + ds], sc, 0, 0, 0);
+        }
+        // score 8 t + i of this lane: key kb + 16 t + 8 h + i
+        const bool whole = kb >= max(lo, whole_from) && kb + 31 <= min(hi, tile_first);
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = kb + 16 * (i / 8) + 8 * h + i % 8;
+            if (!(key <= col.pos && key >= from_here && key <= hi)) sc[i] = -INFINITY;
+          }
+        }
+        float mx = sc[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+        mx = xor_max<32>(mx);
+        const float m_new = fmaxf(m, mx * a.scale_log2), m_use = m_new == -INFINITY ? 0.f : m_new;
+        bf16x8_t pb[2];
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f32x4_t pw[2];
+          if constexpr (Q8) {
+            pw[0] = *reinterpret_cast<const f32x4_t*>(&powers[buf][16 * t + 8 * h]);
+            pw[1] = *reinterpret_cast<const f32x4_t*>(&powers[buf][16 * t + 8 * h + 4]);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float p = __builtin_amdgcn_exp2f(fmaf(sc[8 * t + i], a.scale_log2, -m_use));
+            sum += p;
+            if constexpr (Q8) p *= pw[i / 4][i % 4];
+            pb[t][i] = (__bf16)p;
+          }
+        }
+        if (__any(m_new != m)) {
+          const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+          l *= alpha;
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db) o[db] *= alpha;
+          m = m_new;
+        }
+        l += sum;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+          const bf16x8_t v0 = S::value(st, db, 0), v1 = S::value(st, db, 1);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pb[0], o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, pb[1], o[db], 0, 0, 0);
+        }
+        if (odd_stage[buf] == kb) {                        // values that are not finite: to the columns that see them alone
+          uint32_t seen = 0;                               // a bit a key
+#pragma unroll
+          for (int i = 0; i < 16; ++i) seen |= (float)pb[i / 8][i % 8] > 0.f ? 1u << (16 * (i / 8) + 8 * h + i % 8) : 0u;
+          seen |= lane_xor<32>(seen);
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int dim = 32 * db + 8 * (i / 4) + 4 * h + i % 4;
+              if (seen & ups[buf][dim]) o[db][i] += INFINITY;
+              if (seen & downs[buf][dim]) o[db][i] -= INFINITY;
+            }
+        }
+      }
+      if (kb + 32 <= hi) {
+        if (next.store(lds[buf ^ 1], powers[buf ^ 1], (uint8_t*)ups[buf ^ 1], (uint8_t*)downs[buf ^ 1], kb + 32, lo, hi, differs(kb + 32))) odd_stage[buf ^ 1] = kb + 32;
+        lds_barrier();
+        buf ^= 1;
+        next = after;
+      }
+    }
+  }
+  l = xor_sum<32>(l);
+  if (!col.valid) return;
+  if (a.parts == 1) {
+    if (a.sink != nullptr && m != -INFINITY) l += exp2f(a.sink[col.head] * 1.4426950408889634f - m);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    bf16_t* op = (bf16_t*)a.out + ((int64_t)col.token * a.heads + col.head) * D + 4 * h;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ushort4 w;
+        w.x = float_to_bf16(o[db][4 * i + 0] * inv);
+        w.y = float_to_bf16(o[db][4 * i + 1] * inv);
+        w.z = float_to_bf16(o[db][4 * i + 2] * inv);
+        w.w = float_to_bf16(o[db][4 * i + 3] * inv);
+        *reinterpret_cast<ushort4*>(op + 32 * db + 8 * i) = w;
+      }
+  } else {
+    const int64_t place = a.cell_queries > 0 ? (int64_t)blockIdx.z * a.cell_queries + (col.token - qs) : col.token;
+    const int64_t cell = (place * a.heads + col.head) * a.parts + a.part_first + piece;
+    float* po = a.part_o + cell * D + 4 * h;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4_t*>(po + 32 * db + 8 * i) = f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+    if (h == 0) { a.part_ml[2 * cell] = m; a.part_ml[2 * cell + 1] = l; }
+    if (a.part_first > 0 && from == 0 && piece == 0) {     // (as in the kernel above)
+      const int64_t none = (place * a.heads + col.head) * a.parts;
+      for (int i = h; i < a.part_first; i += 2) { a.part_ml[2 * (none + i)] = -INFINITY; a.part_ml[2 * (none + i) + 1] = 0.f; }
+    }
+  }
+}
+
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over a cell's parts, in their order: D / 4 threads a (token, head).
+template <int D, typename QT>
+__global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_query, int less_than, int64_t cells) {
+  constexpr int LANES = D / 4;
+  const int64_t at = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int d0 = 4 * (threadIdx.x % LANES);
+  if (at >= cells) return;
+  const int head = (int)(at % a.heads);
+  int64_t token = at / a.heads, place = token;
+  if (a.cell_queries > 0) {                                // cells by row and query
+    const int ri = (int)(token / max_query), qi = (int)(token % max_query), row = a.row_ids[ri];
+    const int qs = a.qstart[row], nq = a.qstart[row + 1] - qs;
+    if (qi >= nq || nq > max_query || nq <= less_than) return;      // (a row of more queries, or of fewer, is another kernel's)
+    token = qs + qi;
+  }
+  if (token < 0 || token >= a.n_tokens) return;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (place * a.heads + head) * a.parts;
+  const float* po = a.part_o + (place * a.heads + head) * a.parts * D + d0;
+  float big = -INFINITY;
+#pragma unroll 8
+  for (int i = 0; i < a.parts; ++i) big = fmaxf(big, ml[i].x);
   float l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int i = 0; i < a.parts; ++i) {
-    const float m = a.part_ml[2 * (cell + i)];
-    if (m == -INFINITY && !odd) continue;                  // it saw no key
-    const float w = __builtin_amdgcn_exp2f(m - big);
-    l += w * a.part_ml[2 * (cell + i) + 1];
-    o += w * *reinterpret_cast<const f32x4_t*>(a.part_o + (cell + i) * D + 4 * tid);
+    const float2 x = ml[i];
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(po + (int64_t)i * D);
+    const float w = x.y != 0.f ? __builtin_amdgcn_exp2f(x.x - big) : 0.f;      // (a sum of 0: it saw no key, and left nothing else)
+    l += x.y != 0.f ? w * x.y : 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] += x.y != 0.f ? w * v[r] : 0.f;
   }
   if (a.sink != nullptr && big != -INFINITY) l += exp2f(a.sink[head] * 1.4426950408889634f - big);
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  QT* op = (QT*)a.out + ((int64_t)token * a.heads + head) * D + 4 * tid;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) op[r] = Elem<QT>::store(o[r] * inv);
+  QT* op = (QT*)a.out + (token * a.heads + head) * D + d0;
+  if constexpr (std::is_same<QT, float>::value) {
+    *reinterpret_cast<f32x4_t*>(op) = o * inv;
+  } else {
+    ushort4 w;
+    w.x = float_to_bf16(o[0] * inv); w.y = float_to_bf16(o[1] * inv); w.z = float_to_bf16(o[2] * inv); w.w = float_to_bf16(o[3] * inv);
+    *reinterpret_cast<ushort4*>(op) = w;
+  }
 }
 
-template <int D, bool Q8, typename QT, int NT>
-void launch_rows(const CacheArgs& a, int n_rows, int max_query, int waves, hipStream_t s) {
-  const int tiles = ((int64_t)max_query * (a.heads / a.kv_heads) + 16 * NT - 1) / (16 * NT);
-  const size_t lds = (size_t)(waves - 1) * NT * (16 * D + 32) * sizeof(float);
-  cache_rows_kernel<D, Q8, QT, NT><<<dim3(tiles * (a.splits / waves), a.kv_heads, n_rows), waves * WAVE, lds, s>>>(a);
-}
+// How the keys of a launch are cut: `splits` shares, `waves` of them a block of the kernel of few columns (their sums meet in
+// LDS), so that parts() partial results a cell are left.
+struct Cut {
+  int splits = 1, waves = 1, two = 0;      // two: two tiles of columns a wave
+  int tiles = 0;                           // > 0: the kernel of many columns, so many blocks of them
+  int parts() const { return tiles ? splits : splits / waves; }
+};
+
+struct Launch {
+  hipStream_t stream;
+  int q8, dtype;
+};
 
 template <int D, bool Q8, typename QT>
-void launch_rows_tiles(const CacheArgs& a, int n_rows, int max_query, int waves, int two, hipStream_t s) {
-  if constexpr (two_tiles(D, std::is_same<QT, float>::value)) {
-    if (two) return launch_rows<D, Q8, QT, 2>(a, n_rows, max_query, waves, s);
+void launch_size(const CacheArgs& a, const Cut& c, int jobs, int by_group, int most, int less_than, hipStream_t s) {
+  constexpr bool F32 = std::is_same<QT, float>::value;
+  if constexpr (!F32) {
+    if (c.tiles) {
+      cache_tiles_kernel<D, Q8><<<dim3(a.kv_heads, c.tiles * c.splits, jobs), 256, 0, s>>>(a, by_group, less_than);
+      return;
+    }
   }
-  launch_rows<D, Q8, QT, 1>(a, n_rows, max_query, waves, s);
+  const int nt = 1 + c.two, tiles = (int)(((int64_t)most * (a.heads / a.kv_heads) + 16 * nt - 1) / (16 * nt));
+  const size_t lds = (size_t)(c.waves - 1) * nt * (16 * D + 32) * sizeof(float);
+  const dim3 grid(tiles * (c.splits / c.waves), a.kv_heads, jobs);
+  if constexpr (two_tiles(D, F32)) {
+    if (c.two) {
+      cache_rows_kernel<D, Q8, QT, 2><<<grid, c.waves * WAVE, lds, s>>>(a, by_group, most);
+      return;
+    }
+  }
+  cache_rows_kernel<D, Q8, QT, 1><<<grid, c.waves * WAVE, lds, s>>>(a, by_group, most);
 }
 template <int D>
-void launch_rows_kind(const CacheArgs& a, int q8, int dtype, int n_rows, int max_query, int waves, int two, hipStream_t s) {
-  if (!q8) launch_rows_tiles<D, false, bf16_t>(a, n_rows, max_query, waves, two, s);
-  else if (dtype == HOLON_BF16) launch_rows_tiles<D, true, bf16_t>(a, n_rows, max_query, waves, two, s);
-  else launch_rows_tiles<D, true, float>(a, n_rows, max_query, waves, two, s);
+void launch_kind(const CacheArgs& a, const Launch& w, const Cut& c, int jobs, int by_group, int most, int less_than) {
+  if (!w.q8) launch_size<D, false, bf16_t>(a, c, jobs, by_group, most, less_than, w.stream);
+  else if (w.dtype == HOLON_BF16) launch_size<D, true, bf16_t>(a, c, jobs, by_group, most, less_than, w.stream);
+  else launch_size<D, true, float>(a, c, jobs, by_group, most, less_than, w.stream);
+}
+template <int D>
+void launch_merge(const CacheArgs& a, const Launch& w, int max_query, int less_than, int64_t cells) {
+  const unsigned blocks = (unsigned)((cells + 256 / (D / 4) - 1) / (256 / (D / 4)));
+  if (w.dtype == HOLON_BF16) cache_merge_kernel<D, bf16_t><<<blocks, 256, 0, w.stream>>>(a, max_query, less_than, cells);
+  else cache_merge_kernel<D, float><<<blocks, 256, 0, w.stream>>>(a, max_query, less_than, cells);
 }
 
-}  // namespace
+// Rows whose columns (queries times the heads of a group) are at most this many take the kernel of few columns, which reads the keys
+// once for every 32 of them.
+constexpr int FEW_COLUMNS = 64;
 
-namespace {
-
-// How the keys of a launch's rows are cut over waves: `splits` shares, `waves` of them a block (their sums meet in LDS), so that
-// splits / waves parts a cell are left for the merge.
-struct Cut {
-  int splits, waves, two;      // two: two tiles of columns a wave
-  int parts() const { return splits / waves; }
-};
-Cut cut_rows(int n_rows, int max_query, int64_t span, int heads, int kv_heads, int head_dim, int window, bool f32) {
+// `jobs` rows (or groups) of up to `columns` columns over up to `span` keys.
+Cut cut_keys(int jobs, int64_t columns, int64_t span, int kv_heads, int head_dim, bool f32) {
   Cut r;
-  const int64_t columns = (int64_t)max_query * (heads / kv_heads);
+  const int64_t units = std::max<int64_t>(1, (int64_t)jobs * kv_heads);
+  span = std::max<int64_t>(span, 1);
+  columns = std::max<int64_t>(columns, 1);
+  if (columns > FEW_COLUMNS && !f32) {
+    r.tiles = (int)((columns + 127) / 128);
+    const int64_t want = std::max<int64_t>(1, 512 / (units * r.tiles));                 // two blocks a compute unit
+    r.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (span + 127) / 128));
+    return r;
+  }
   r.two = columns > 16 && two_tiles(head_dim, f32);
-  const int64_t pairs = std::max<int64_t>(1, n_rows * kv_heads * ((columns + 16 * (1 + r.two) - 1) / (16 * (1 + r.two))));
-  if (window > 0) span = std::min<int64_t>(span, window + max_query + 63);
-  if (window < 0) span = std::min<int64_t>(span, -(int64_t)window + 63);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(64, 2048 / pairs));
+  const int64_t pairs = units * ((columns + 16 * (1 + r.two) - 1) / (16 * (1 + r.two)));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(64, 2048 / std::max<int64_t>(1, pairs)));
   const int64_t per = std::max<int64_t>(64, ((span + want - 1) / want + 63) / 64 * 64);
   const int64_t shares = std::max<int64_t>(1, (span + per - 1) / per);
   const int64_t blocks = pairs <= 16 ? 256 : 512;
-  const int cap = most_waves(head_dim, f32, 1 + r.two);
   const int64_t outer = std::min(shares, std::max<int64_t>(1, (blocks + pairs - 1) / pairs));
-  r.waves = (int)std::min<int64_t>(cap, (shares + outer - 1) / outer);
+  r.waves = (int)std::min<int64_t>(most_waves(head_dim, f32, 1 + r.two), (shares + outer - 1) / outer);
   r.splits = (int)((shares + r.waves - 1) / r.waves) * r.waves;
   return r;
 }
+int64_t seen_span(int64_t len, int64_t queries, int window) {
+  if (window > 0) return std::min<int64_t>(len, window + queries + 63);
+  if (window < 0) return std::min<int64_t>(len, -(int64_t)window + 63);
+  return len;
+}
 
-// What one call runs.
+// What one call runs: the decode rows, the rows of a few queries, those of many, the groups' prefixes.
 struct Plan {
-  Cut decode, chunk;
-  int64_t decode_cells, chunk_cells;      // of partial results
+  Cut decode, few, many, shared;
+  int few_query = 0;                       // rows of up to so many queries are among the few
+  bool any_decode, any_few, any_many, any_shared, by_token;
+  int parts = 1;                           // of a cell, where cells go by token
+  int64_t decode_cells = 0, few_cells = 0, many_cells = 0;
 };
-Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len, int heads, int kv_heads,
-             int head_dim, int window, bool f32) {
+Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len, int n_groups, int max_group_query,
+             int max_group_len, int n_tokens, int heads, int kv_heads, int head_dim, int window, bool f32) {
   Plan p;
-  p.decode = cut_rows(n_decode, 1, max_decode_len, heads, kv_heads, head_dim, window, f32);
-  p.chunk = cut_rows(n_chunk, max_chunk_query, max_chunk_len, heads, kv_heads, head_dim, window, f32);
-  p.decode_cells = p.decode.parts() > 1 ? (int64_t)n_decode * heads * p.decode.parts() : 0;
-  p.chunk_cells = p.chunk.parts() > 1 ? (int64_t)n_chunk * max_chunk_query * heads * p.chunk.parts() : 0;
+  const int group = heads / kv_heads;
+  p.any_shared = n_groups > 0 && max_group_query > 0 && max_group_len > 0;
+  const int own_decode = p.any_shared ? std::max(max_decode_len - max_group_len, 64) : max_decode_len;
+  const int own_chunk = p.any_shared ? std::max(max_chunk_len - max_group_len, 64) : max_chunk_len;
+  const int few = f32 ? max_chunk_query : std::min(max_chunk_query, std::max(1, FEW_COLUMNS / group));
+  p.few_query = few;
+  p.any_decode = n_decode > 0;
+  p.any_few = n_chunk > 0 && few > 1;
+  p.any_many = n_chunk > 0 && max_chunk_query > few;
+  if (p.any_many && n_chunk == 1) p.any_few = false;       // (the one row is as long as the longest)
+  p.decode = cut_keys(n_decode, group, seen_span(own_decode, 1, window), kv_heads, head_dim, f32);
+  p.few = cut_keys(n_chunk, (int64_t)few * group, seen_span(own_chunk, few, window), kv_heads, head_dim, f32);
+  p.many = cut_keys(n_chunk, std::max<int64_t>((int64_t)max_chunk_query * group, FEW_COLUMNS + 1), seen_span(own_chunk, max_chunk_query, window),
+                    kv_heads, head_dim, f32);
+  p.by_token = p.any_shared;
+  if (p.by_token) {
+    p.shared = cut_keys(n_groups, (int64_t)max_group_query * group, max_group_len, kv_heads, head_dim, f32);
+    // every cell has the prefix's parts and then as many of its row's own whichever kernel made them
+    const int own = p.any_decode ? p.decode.parts() : p.any_few ? p.few.parts() : p.many.parts();
+    p.decode.splits = own * p.decode.waves;
+    p.few.splits = own * p.few.waves;
+    p.many.splits = own;
+    p.parts = p.shared.parts() + own;
+    p.decode_cells = (int64_t)n_tokens * heads * p.parts;
+  } else {
+    if (p.any_decode && p.decode.parts() > 1) p.decode_cells = (int64_t)n_decode * heads * p.decode.parts();
+    if (p.any_few && p.few.parts() > 1) p.few_cells = (int64_t)n_chunk * few * heads * p.few.parts();
+    if (p.any_many && p.many.parts() > 1) p.many_cells = (int64_t)n_chunk * max_chunk_query * heads * p.many.parts();
+  }
   return p;
 }
 
@@ -514,9 +941,10 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
 extern "C" int64_t holon_cache_attention_room(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len,
                                               int n_groups, int max_group_query, int max_group_len, int n_tokens, int heads,
                                               int kv_heads, int head_dim, int window, int dtype) {
-  const Plan p = plan_of(n_decode, max_decode_len, n_chunk, max_chunk_query, max_chunk_len, heads, kv_heads, head_dim, window,
-                         dtype == HOLON_F32);
-  return (p.decode_cells + p.chunk_cells) * (head_dim + 2) * (int64_t)sizeof(float);
+  if (kv_heads <= 0 || heads < kv_heads) return 0;         // (refused by the call that follows)
+  const Plan p = plan_of(n_decode, max_decode_len, n_chunk, max_chunk_query, max_chunk_len, n_groups, max_group_query, max_group_len,
+                         n_tokens, heads, kv_heads, head_dim, window, dtype == HOLON_F32);
+  return (p.decode_cells + p.few_cells + p.many_cells) * (head_dim + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int holon_cache_attention(const void* q, void* out, const void* pages, const void* scales, int64_t page_stride,
@@ -542,33 +970,42 @@ extern "C" int holon_cache_attention(const void* q, void* out, const void* pages
   a.slots = slots; a.lens = lens; a.qstart = qstart; a.n_tokens = n_tokens;
   a.heads = heads; a.kv_heads = kv_heads; a.page_size = page_size;
   a.scale_log2 = scale * 1.4426950408889634f; a.window = window; a.sink = sink;
-  const Plan p = plan_of(n_decode, max_decode_len, n_chunk, max_chunk_query, max_chunk_len, heads, kv_heads, head_dim, window,
-                         dtype == HOLON_F32);
+  const Plan p = plan_of(n_decode, max_decode_len, n_chunk, max_chunk_query, max_chunk_len, n_groups, max_group_query, max_group_len,
+                         n_tokens, heads, kv_heads, head_dim, window, dtype == HOLON_F32);
   float* at = (float*)room;
-  hipStream_t s = (hipStream_t)stream;
-  const auto serve = [&](const int32_t* ids, int n_rows, int max_query, const Cut& c, int64_t cells) {
-    if (n_rows == 0 || max_query == 0) return;
-    a.row_ids = ids;
-    a.splits = c.splits; a.parts = c.parts(); a.part_first = 0; a.cell_queries = max_query;
-    a.part_o = at; a.part_ml = at + cells * head_dim;
-    at += cells * (head_dim + 2);
-    if (head_dim == 64) launch_rows_kind<64>(a, q8, dtype, n_rows, max_query, c.waves, c.two, s);
-    else if (head_dim == 128) launch_rows_kind<128>(a, q8, dtype, n_rows, max_query, c.waves, c.two, s);
-    else launch_rows_kind<256>(a, q8, dtype, n_rows, max_query, c.waves, c.two, s);
-    if (a.parts > 1) {
-      const dim3 grid(heads, max_query, n_rows);
-      const auto merge = [&](auto size) {
-        constexpr int D = decltype(size)::value;
-        if (dtype == HOLON_BF16) cache_merge_kernel<D, bf16_t><<<grid, D / 4, 0, s>>>(a);
-        else cache_merge_kernel<D, float><<<grid, D / 4, 0, s>>>(a);
-      };
-      if (head_dim == 64) merge(std::integral_constant<int, 64>{});
-      else if (head_dim == 128) merge(std::integral_constant<int, 128>{});
-      else merge(std::integral_constant<int, 256>{});
-    }
+  const Launch w{(hipStream_t)stream, q8, dtype};
+  const auto launch = [&](const Cut& c, int jobs, int by_group, int most, int less_than) {
+    a.splits = c.splits;
+    if (head_dim == 64) launch_kind<64>(a, w, c, jobs, by_group, most, less_than);
+    else if (head_dim == 128) launch_kind<128>(a, w, c, jobs, by_group, most, less_than);
+    else launch_kind<256>(a, w, c, jobs, by_group, most, less_than);
   };
-  serve(decode_rows, n_decode, 1, p.decode, p.decode_cells);
-  serve(chunk_rows, n_chunk, max_chunk_query, p.chunk, p.chunk_cells);
+  const auto merge = [&](int max_query, int less_than, int64_t cells) {
+    if (head_dim == 64) launch_merge<64>(a, w, max_query, less_than, cells);
+    else if (head_dim == 128) launch_merge<128>(a, w, max_query, less_than, cells);
+    else launch_merge<256>(a, w, max_query, less_than, cells);
+  };
+  if (p.by_token) {
+    a.group_start = group_start; a.group_lens = group_lens; a.n_groups = n_groups;
+    a.parts = p.parts; a.part_o = at; a.part_ml = at + p.decode_cells * head_dim;
+    launch(p.shared, n_groups, 1, max_group_query, 0);
+    a.part_first = p.shared.parts();
+  }
+  const auto serve = [&](bool any, const Cut& c, const int32_t* ids, int n_rows, int most, int less_than, int64_t cells) {
+    if (!any) return;
+    a.row_ids = ids;
+    if (!p.by_token) {
+      a.parts = c.parts(); a.cell_queries = most;
+      a.part_o = at; a.part_ml = at + cells * head_dim;
+      at += cells * (head_dim + 2);
+    }
+    launch(c, n_rows, 0, most, less_than);
+    if (!p.by_token && a.parts > 1) merge(most, less_than, (int64_t)n_rows * most * heads);
+  };
+  serve(p.any_decode, p.decode, decode_rows, n_decode, 1, 0, p.decode_cells);
+  serve(p.any_few, p.few, chunk_rows, n_chunk, p.few_query, 0, p.few_cells);
+  serve(p.any_many, p.many, chunk_rows, n_chunk, max_chunk_query, p.any_few ? p.few_query : 0, p.many_cells);
+  if (p.by_token) merge(1, 0, (int64_t)n_tokens * heads);
   HOLON_LAUNCH_OK();
   return 0;
 }

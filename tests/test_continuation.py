@@ -170,6 +170,10 @@ STEPS = [
     ([(0, 130), (64, 65), (300, 1), (11, 6)], 8, 4, 128, 32, 0),             # prompts, portions
     ([(100, 70), (0, 40)], 4, 2, 256, 16, 0),
     ([(70, 90)], 14, 2, 128, 16, -32),
+    ([(0, 64), (31, 33), (200, 64)], 2, 2, 64, 48, 0),                       # as many columns as the kernel of few takes, and less
+    ([(3, 150), (0, 65)], 1, 1, 64, 16, 40),
+    ([(2000, 66), (70, 2)], 4, 1, 128, 32, 0),                               # a short portion behind a long context
+    ([(40, 1), (33, 2)], 70, 1, 64, 16, 0),                                  # more heads on one than the kernel of few columns takes
 ]
 
 
@@ -420,6 +424,15 @@ def test_rows_that_see_nothing(hip):
     _check(got, q, pages, scales, table, attn, 16, 0.125)
 
 
+@gpu
+@pytest.mark.parametrize("step", range(len(STEPS)))
+def test_a_bfloat16_cache_without_a_prefix(hip, step):
+    rows, heads, kv, d, page, window = STEPS[step]
+    q, pages, _, table, attn, _ = _step(rows, heads, kv, d, page, seed=step, q8=False, device="cuda")
+    got = hip.prefix_attention(q, pages, table, attn, None, page, d ** -0.5)
+    _check(got, q, pages, None, table, attn, page, d ** -0.5)
+
+
 SHARED = [
     # (rows, groups, heads, kv heads, head size, page): a prefix of one page, one that ends inside a page, several groups, drafted tokens
     ([(20, 1), (40, 1)], [(0, 1, 16)], 4, 1, 64, 16),
@@ -429,6 +442,8 @@ SHARED = [
     ([(64, 1)] * 3 + [(200, 3)] * 2, [(0, 2, 64), (3, 4, 192)], 16, 1, 256, 64),
     ([(129, 70), (128, 2), (500, 1)], [(0, 2, 128)], 4, 2, 64, 16),                                 # a portion in the group
     ([(1000, 1)] * 40, [(0, 39, 992)], 8, 1, 128, 16),                                              # more columns than a block takes
+    ([(96, 200), (100, 40)], [(0, 1, 96)], 4, 1, 128, 32),                                          # portions alone
+    ([(520, 4)] * 20 + [(17, 3)], [(0, 19, 512)], 6, 2, 64, 16),                                    # and a row in no group
     ([(30, 1), (31, 1)], [(0, 0, 0), (1, 1, 16)], 4, 1, 64, 16),                                    # nothing shared, a row by itself
 ]
 
