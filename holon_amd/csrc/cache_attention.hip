@@ -32,7 +32,7 @@ struct CacheArgs {
   const int32_t* slots;        // [B]
   const int32_t* lens;         // [B]
   const int32_t* qstart;       // [B + 1]
-  const int32_t* row_ids;      // the rows of this launch
+  const int32_t* row_ids;      // the rows of this launch (null: they are decode rows alone, in order)
   int n_tokens;
   int heads, kv_heads, page_size;
   float scale_log2;            // scale * log2(e)
@@ -83,9 +83,10 @@ __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) 
     j.nq = end > j.row && j.n > 0 ? a.qstart[end] - j.qs : 0;
     j.from = 0;
   } else {
-    j.row = a.row_ids[at];
-    j.qs = a.qstart[j.row];
-    j.nq = a.qstart[j.row + 1] - j.qs;
+    const bool in_order = a.row_ids == nullptr;            // rows of one query, one a token, from the first on
+    j.row = in_order ? at : a.row_ids[at];
+    j.qs = in_order ? at : a.qstart[j.row];
+    j.nq = in_order ? 1 : a.qstart[j.row + 1] - j.qs;
     j.n = a.lens[j.row];
     j.from = shared_keys(a, j.row);
   }
@@ -202,6 +203,32 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
   if (key_lo <= key_hi) {
     const int32_t* trow = table_row(a, row);
     const int max_page = a.table_stride - 1;
+    const int bytes = Q8 ? 1 : 2;
+    const int64_t plane = (int64_t)P * D * bytes;
+    const int krun = RUN * (c / 4);                        // this lane's keys: krun + c % 4 + 4 j; its values: RUN g ..
+    // Everything that a block of keys needs is asked for while the block before it is multiplied, the table's entries a block
+    // earlier still: a wave's loads come back in order, so none may wait for one asked for just now.
+    struct Keys {
+      u32x4_t raw[SCORES][KLOADS], power;
+    };
+    const auto look = [&](int kb, int32_t& ek, int32_t& ev) {
+      ek = trow[min((kb + krun) / P, max_page)];
+      ev = trow[min((kb + RUN * g) / P, max_page)];
+    };
+    const auto load_keys = [&](int kb, int32_t ek, Keys& to) {
+      const int at = (kb + krun) % P;
+      const int64_t page = page_at(a, ek);
+      const uint8_t* p = a.pages + page * a.page_stride + hk * plane + (int64_t)(at + c % 4) * D * bytes + 16 * g;
+#pragma unroll
+      for (int j = 0; j < SCORES; ++j)
+#pragma unroll
+        for (int i = 0; i < KLOADS; ++i) to.raw[j][i] = *reinterpret_cast<const u32x4_t*>(p + 4 * j * D * bytes + 64 * i);
+      if constexpr (Q8) to.power = *reinterpret_cast<const u32x4_t*>(a.scales + page * a.scale_stride + (int64_t)hk * P + at);
+    };
+    int32_t ek, ev, ek_next, ev_next;
+    Keys keys;
+    look(key_lo, ek, ev);
+    look(key_lo + KB, ek_next, ev_next);
     bf16x8_t qf[NT][PARTS][D / 32];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -209,40 +236,44 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
 #pragma unroll
       for (int ks = 0; ks < D / 32; ++ks) {
         const int d0 = Q8 ? 64 * (ks / 2) + 16 * g + 8 * (ks % 2) : 32 * ks + 8 * g;
+        if constexpr (PARTS == 1) {
+          u32x4_t x = {0, 0, 0, 0};
+          if (col[t].valid) x = *reinterpret_cast<const u32x4_t*>(qp + d0);
+          qf[t][0][ks] = __builtin_bit_cast(bf16x8_t, x);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          __bf16 p[PARTS];
-          const float x = col[t].valid ? Elem<QT>::load(qp[d0 + i]) : 0.f;
-          split<PARTS>(x, p);
+          for (int i = 0; i < 8; i += 4) {
+            f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+            if (col[t].valid) x = *reinterpret_cast<const f32x4_t*>(qp + d0 + i);
 #pragma unroll
-          for (int s = 0; s < PARTS; ++s) qf[t][s][ks][i] = p[s];
+            for (int r = 0; r < 4; ++r) {
+              __bf16 p[PARTS];
+              split<PARTS>(x[r], p);
+#pragma unroll
+              for (int s = 0; s < PARTS; ++s) qf[t][s][ks][i + r] = p[s];
+            }
+          }
         }
       }
     }
-    const int bytes = Q8 ? 1 : 2;
-    const int64_t plane = (int64_t)P * D * bytes;
-    const uint8_t* kplane = a.pages + hk * plane;
-    const uint8_t* vplane = a.pages + (a.kv_heads + hk) * plane;
-    const uint8_t* ksplane = Q8 ? a.scales + (int64_t)hk * P : nullptr;
-    const uint8_t* vsplane = Q8 ? a.scales + (int64_t)(a.kv_heads + hk) * P : nullptr;
-    const int krun = RUN * (c / 4);                        // this lane's keys: krun + c % 4 + 4 j; its values: RUN g ..
+    load_keys(key_lo, ek, keys);
     for (int kb = key_lo; kb <= key_hi; kb += KB) {
-      const int kk = kb + krun, vk = kb + RUN * g;
-      const int64_t kpage = page_at(a, trow[min(kk / P, max_page)]), vpage = page_at(a, trow[min(vk / P, max_page)]);
-      u32x4_t kraw[SCORES][KLOADS], vraw[D / 16], ks4 = {}, vs4 = {};
-      if constexpr (Q8) {
-        ks4 = *reinterpret_cast<const u32x4_t*>(ksplane + kpage * a.scale_stride + kk % P);
-        vs4 = *reinterpret_cast<const u32x4_t*>(vsplane + vpage * a.scale_stride + vk % P);
+      const int vk = kb + RUN * g;
+      u32x4_t vraw[D / 16], vs4 = {};
+      {
+        const int at = vk % P;
+        const int64_t page = page_at(a, ev);
+        const uint8_t* p = a.pages + page * a.page_stride + (a.kv_heads + hk) * plane + ((int64_t)c * P + at) * bytes;
+#pragma unroll
+        for (int ds = 0; ds < D / 16; ++ds) vraw[ds] = *reinterpret_cast<const u32x4_t*>(p + (int64_t)ds * 16 * P * bytes);
+        if constexpr (Q8) vs4 = *reinterpret_cast<const u32x4_t*>(a.scales + page * a.scale_stride + (int64_t)(a.kv_heads + hk) * P + at);
       }
-      const uint8_t* kp = kplane + kpage * a.page_stride + (int64_t)(kk % P + c % 4) * D * bytes + 16 * g;
-#pragma unroll
-      for (int j = 0; j < SCORES; ++j)
-#pragma unroll
-        for (int i = 0; i < KLOADS; ++i) kraw[j][i] = *reinterpret_cast<const u32x4_t*>(kp + (int64_t)4 * j * D * bytes + 64 * i);
-      const uint8_t* vp = vplane + vpage * a.page_stride + ((int64_t)c * P + vk % P) * bytes;
-#pragma unroll
-      for (int ds = 0; ds < D / 16; ++ds) vraw[ds] = *reinterpret_cast<const u32x4_t*>(vp + (int64_t)ds * 16 * P * bytes);
-
+      Keys next;
+      if (kb + KB <= key_hi) {
+        load_keys(kb + KB, ek_next, next);
+        ev = ev_next;
+        if (kb + 2 * KB <= key_hi) look(kb + 2 * KB, ek_next, ev_next);
+      }
       const bool whole = kb >= whole_from && kb + KB - 1 <= min(pos_first, key_hi);
       f32x4_t sc[NT][SCORES];
 #pragma unroll
@@ -251,12 +282,12 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
         for (int j = 0; j < SCORES; ++j) sc[t][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < SCORES; ++j) {
-        const float power = Q8 ? q8_power((ks4[j] >> (8 * (c % 4))) & 0xffu) : 1.f;
+        const float power = Q8 ? q8_power((keys.power[j] >> (8 * (c % 4))) & 0xffu) : 1.f;
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {
           bf16x8_t f[Q8 ? 2 : 1];
-          if constexpr (Q8) widen(kraw[j][i], power, f[0], f[1]);
-          else f[0] = __builtin_bit_cast(bf16x8_t, kraw[j][i]);
+          if constexpr (Q8) widen(keys.raw[j][i], power, f[0], f[1]);
+          else f[0] = __builtin_bit_cast(bf16x8_t, keys.raw[j][i]);
 #pragma unroll
           for (int u = 0; u < (Q8 ? 2 : 1); ++u)
 #pragma unroll
@@ -388,6 +419,7 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
             for (int s = 0; s < PARTS; ++s)
               tl.o[t][ds] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[u], pb[t][u][s], tl.o[t][ds], 0, 0, 0);
       }
+      keys = next;
     }
   }
 #pragma unroll
@@ -780,8 +812,10 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
   const int head = (int)(at % a.heads);
   int64_t token = at / a.heads, place = token;
   if (a.cell_queries > 0) {                                // cells by row and query
-    const int ri = (int)(token / max_query), qi = (int)(token % max_query), row = a.row_ids[ri];
-    const int qs = a.qstart[row], nq = a.qstart[row + 1] - qs;
+    const int ri = (int)(token / max_query), qi = (int)(token % max_query);
+    const bool in_order = a.row_ids == nullptr;
+    const int row = in_order ? ri : a.row_ids[ri];
+    const int qs = in_order ? ri : a.qstart[row], nq = in_order ? 1 : a.qstart[row + 1] - qs;
     if (qi >= nq || nq > max_query || nq <= less_than) return;      // (a row of more queries, or of fewer, is another kernel's)
     token = qs + qi;
   }
@@ -882,8 +916,10 @@ Cut cut_keys(int jobs, int64_t columns, int64_t span, int kv_heads, int head_dim
   const int64_t per = std::max<int64_t>(64, ((span + want - 1) / want + 63) / 64 * 64);
   const int64_t shares = std::max<int64_t>(1, (span + per - 1) / per);
   const int64_t blocks = pairs <= 16 ? 256 : 512;
-  const int64_t outer = std::min(shares, std::max<int64_t>(1, (blocks + pairs - 1) / pairs));
-  r.waves = (int)std::min<int64_t>(most_waves(head_dim, f32, 1 + r.two), (shares + outer - 1) / outer);
+  const int cap = most_waves(head_dim, f32, 1 + r.two);
+  // few enough shares meet in one block, and no merge follows
+  const int64_t outer = shares <= cap ? 1 : std::min(shares, std::max<int64_t>(1, (blocks + pairs - 1) / pairs));
+  r.waves = (int)std::min<int64_t>(cap, (shares + outer - 1) / outer);
   r.splits = (int)((shares + r.waves - 1) / r.waves) * r.waves;
   return r;
 }
@@ -902,7 +938,7 @@ struct Plan {
   int64_t decode_cells = 0, few_cells = 0, many_cells = 0;
 };
 Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len, int n_groups, int max_group_query,
-             int max_group_len, int n_tokens, int heads, int kv_heads, int head_dim, int window, bool f32) {
+             int max_group_len, int64_t n_tokens, int heads, int kv_heads, int head_dim, int window, bool f32) {
   Plan p;
   const int group = heads / kv_heads;
   p.any_shared = n_groups > 0 && max_group_query > 0 && max_group_len > 0;
@@ -938,47 +974,48 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
 
 }  // namespace
 
-extern "C" int64_t holon_cache_attention_room(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len,
-                                              int n_groups, int max_group_query, int max_group_len, int n_tokens, int heads,
-                                              int kv_heads, int head_dim, int window, int dtype) {
-  if (kv_heads <= 0 || heads < kv_heads) return 0;         // (refused by the call that follows)
-  const Plan p = plan_of(n_decode, max_decode_len, n_chunk, max_chunk_query, max_chunk_len, n_groups, max_group_query, max_group_len,
-                         n_tokens, heads, kv_heads, head_dim, window, dtype == HOLON_F32);
-  return (p.decode_cells + p.few_cells + p.many_cells) * (head_dim + 2) * (int64_t)sizeof(float);
+static Plan plan_of(const HolonCacheAttention& c) {
+  return plan_of(c.n_decode, c.max_decode_len, c.n_chunk, c.max_chunk_query, c.max_chunk_len, c.n_groups, c.max_group_query, c.max_group_len,
+                 c.tokens, c.heads, c.kv_heads, c.head_dim, c.window, c.dtype == HOLON_F32);
 }
 
-extern "C" int holon_cache_attention(const void* q, void* out, const void* pages, const void* scales, int64_t page_stride,
-                                     int64_t scale_stride, int num_pages, const int32_t* table, int table_stride, int n_slots,
-                                     const int32_t* slots, const int32_t* lens, const int32_t* qstart, const int32_t* decode_rows,
-                                     int n_decode, int max_decode_len, const int32_t* chunk_rows, int n_chunk, int max_chunk_query,
-                                     int max_chunk_len, const int32_t* group_start, const int32_t* group_lens, int n_groups,
-                                     int max_group_query, int max_group_len, int n_tokens, int heads, int kv_heads, int head_dim,
-                                     int page_size, float scale, int window, const float* sink, void* room, int dtype, void* stream) {
-  const bool q8 = scales != nullptr;
+extern "C" int64_t holon_cache_attention_room(const HolonCacheAttention* call) {
+  const HolonCacheAttention& c = *call;
+  if (c.kv_heads <= 0 || c.heads < c.kv_heads) return 0;   // (refused by the call that follows)
+  const Plan p = plan_of(c);
+  return (p.decode_cells + p.few_cells + p.many_cells) * (c.head_dim + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void* q, void* out, void* room, void* stream) {
+  const HolonCacheAttention& c = *call;
+  const int head_dim = c.head_dim, heads = c.heads, dtype = c.dtype;
+  const bool q8 = c.scales != nullptr;
   HOLON_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "attention: heads of %d (64, 128 and 256 are served)", head_dim);
-  HOLON_CHECK(page_size > 0 && page_size % 16 == 0, "attention: pages of %d tokens (multiples of 16 are served)", page_size);
+  HOLON_CHECK(c.page_size > 0 && c.page_size % 16 == 0, "attention: pages of %d tokens (multiples of 16 are served)", c.page_size);
   HOLON_CHECK(dtype == HOLON_BF16 || (q8 && dtype == HOLON_F32), "attention: queries of another type than the cache serves");
-  HOLON_CHECK(heads > 0 && kv_heads > 0 && kv_heads <= 65535 && heads % kv_heads == 0, "attention: %d heads over %d", heads, kv_heads);
-  HOLON_CHECK(n_decode >= 0 && n_chunk >= 0 && n_decode <= 65535 && n_chunk <= 65535 && max_chunk_query <= 65535 && n_tokens >= 0 &&
-                  num_pages > 0 && n_slots > 0 && table_stride > 0 && n_groups >= 0, "attention: bad sizes");
-  HOLON_CHECK(scale > 0.f, "attention: a scale of %g", (double)scale);
-  HOLON_CHECK(page_stride % 16 == 0 && scale_stride % 16 == 0, "attention: pages lie on no borders of 16 bytes");
+  HOLON_CHECK(heads > 0 && c.kv_heads > 0 && c.kv_heads <= 65535 && heads % c.kv_heads == 0, "attention: %d heads over %d", heads, c.kv_heads);
+  HOLON_CHECK(c.n_decode >= 0 && c.n_chunk >= 0 && c.n_decode <= 65535 && c.n_chunk <= 65535 && c.max_chunk_query <= 65535 && c.tokens >= 0 &&
+                  c.tokens <= 0x7fffffff && c.n_groups <= 65535 && c.max_decode_len >= 0 && c.max_chunk_len >= 0 && c.max_group_query >= 0 &&
+                  c.max_group_len >= 0 && c.num_pages > 0 && c.n_slots > 0 && c.table_stride > 0 && c.n_groups >= 0 &&
+                  (c.n_chunk == 0 || c.max_chunk_query > 0), "attention: bad sizes");
+  HOLON_CHECK(c.scale > 0.f, "attention: a scale of %g", (double)c.scale);
+  HOLON_CHECK(c.page_stride % 16 == 0 && c.scale_stride % 16 == 0, "attention: pages lie on no borders of 16 bytes");
+  if (c.tokens == 0) return 0;
   CacheArgs a{};
-  a.q = q; a.out = out; a.pages = (const uint8_t*)pages; a.scales = (const uint8_t*)scales;
-  a.page_stride = page_stride; a.scale_stride = scale_stride; a.num_pages = num_pages;
-  a.table = table; a.table_stride = table_stride; a.n_slots = n_slots;
-  a.slots = slots; a.lens = lens; a.qstart = qstart; a.n_tokens = n_tokens;
-  a.heads = heads; a.kv_heads = kv_heads; a.page_size = page_size;
-  a.scale_log2 = scale * 1.4426950408889634f; a.window = window; a.sink = sink;
-  const Plan p = plan_of(n_decode, max_decode_len, n_chunk, max_chunk_query, max_chunk_len, n_groups, max_group_query, max_group_len,
-                         n_tokens, heads, kv_heads, head_dim, window, dtype == HOLON_F32);
+  a.q = q; a.out = out; a.pages = (const uint8_t*)c.pages; a.scales = (const uint8_t*)c.scales;
+  a.page_stride = c.page_stride; a.scale_stride = c.scale_stride; a.num_pages = c.num_pages;
+  a.table = c.table; a.table_stride = c.table_stride; a.n_slots = c.n_slots;
+  a.slots = c.slots; a.lens = c.lens; a.qstart = c.qstart; a.n_tokens = (int)c.tokens;
+  a.heads = heads; a.kv_heads = c.kv_heads; a.page_size = c.page_size;
+  a.scale_log2 = c.scale * 1.4426950408889634f; a.window = c.window; a.sink = c.sink;
+  const Plan p = plan_of(c);
   float* at = (float*)room;
   const Launch w{(hipStream_t)stream, q8, dtype};
-  const auto launch = [&](const Cut& c, int jobs, int by_group, int most, int less_than) {
-    a.splits = c.splits;
-    if (head_dim == 64) launch_kind<64>(a, w, c, jobs, by_group, most, less_than);
-    else if (head_dim == 128) launch_kind<128>(a, w, c, jobs, by_group, most, less_than);
-    else launch_kind<256>(a, w, c, jobs, by_group, most, less_than);
+  const auto launch = [&](const Cut& cut, int jobs, int by_group, int most, int less_than) {
+    a.splits = cut.splits;
+    if (head_dim == 64) launch_kind<64>(a, w, cut, jobs, by_group, most, less_than);
+    else if (head_dim == 128) launch_kind<128>(a, w, cut, jobs, by_group, most, less_than);
+    else launch_kind<256>(a, w, cut, jobs, by_group, most, less_than);
   };
   const auto merge = [&](int max_query, int less_than, int64_t cells) {
     if (head_dim == 64) launch_merge<64>(a, w, max_query, less_than, cells);
@@ -986,26 +1023,26 @@ extern "C" int holon_cache_attention(const void* q, void* out, const void* pages
     else launch_merge<256>(a, w, max_query, less_than, cells);
   };
   if (p.by_token) {
-    a.group_start = group_start; a.group_lens = group_lens; a.n_groups = n_groups;
+    a.group_start = c.group_start; a.group_lens = c.group_lens; a.n_groups = c.n_groups;
     a.parts = p.parts; a.part_o = at; a.part_ml = at + p.decode_cells * head_dim;
-    launch(p.shared, n_groups, 1, max_group_query, 0);
+    launch(p.shared, c.n_groups, 1, c.max_group_query, 0);
     a.part_first = p.shared.parts();
   }
-  const auto serve = [&](bool any, const Cut& c, const int32_t* ids, int n_rows, int most, int less_than, int64_t cells) {
+  const auto serve = [&](bool any, const Cut& cut, const int32_t* ids, int n_rows, int most, int less_than, int64_t cells) {
     if (!any) return;
     a.row_ids = ids;
     if (!p.by_token) {
-      a.parts = c.parts(); a.cell_queries = most;
+      a.parts = cut.parts(); a.cell_queries = most;
       a.part_o = at; a.part_ml = at + cells * head_dim;
       at += cells * (head_dim + 2);
     }
-    launch(c, n_rows, 0, most, less_than);
+    launch(cut, n_rows, 0, most, less_than);
     if (!p.by_token && a.parts > 1) merge(most, less_than, (int64_t)n_rows * most * heads);
   };
-  serve(p.any_decode, p.decode, decode_rows, n_decode, 1, 0, p.decode_cells);
-  serve(p.any_few, p.few, chunk_rows, n_chunk, p.few_query, 0, p.few_cells);
-  serve(p.any_many, p.many, chunk_rows, n_chunk, max_chunk_query, p.any_few ? p.few_query : 0, p.many_cells);
-  if (p.by_token) merge(1, 0, (int64_t)n_tokens * heads);
+  serve(p.any_decode, p.decode, c.decode_rows, c.n_decode, 1, 0, p.decode_cells);
+  serve(p.any_few, p.few, c.chunk_rows, c.n_chunk, p.few_query, 0, p.few_cells);
+  serve(p.any_many, p.many, c.chunk_rows, c.n_chunk, c.max_chunk_query, p.any_few ? p.few_query : 0, p.many_cells);
+  if (p.by_token) merge(1, 0, c.tokens * heads);
   HOLON_LAUNCH_OK();
   return 0;
 }

@@ -556,16 +556,25 @@ int holon_kv_read_q8(void* k, void* v, const void* pages, const void* scales, in
                      int num_pages, int dtype, void* stream);
 // Paged attention over it (scales given; dtype of q and out), or over bfloat16 pages (scales NULL), rows sharing their first tokens
 // by groups (n_groups 0: none). `room`: holon_cache_attention_room bytes of scratch, on a border of 16.
-int64_t holon_cache_attention_room(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len, int n_groups,
-                                   int max_group_query, int max_group_len, int n_tokens, int heads, int kv_heads, int head_dim,
-                                   int window, int dtype);
-int holon_cache_attention(const void* q, void* out, const void* pages, const void* scales, int64_t page_stride, int64_t scale_stride,
-                          int num_pages, const int32_t* table, int table_stride, int n_slots, const int32_t* slots,
-                          const int32_t* lens, const int32_t* qstart, const int32_t* decode_rows, int n_decode, int max_decode_len,
-                          const int32_t* chunk_rows, int n_chunk, int max_chunk_query, int max_chunk_len,
-                          const int32_t* group_start, const int32_t* group_lens, int n_groups, int max_group_query,
-                          int max_group_len, int n_tokens, int heads, int kv_heads, int head_dim, int page_size, float scale,
-                          int window, const float* sink, void* room, int dtype, void* stream);
+struct HolonCacheAttention {
+  const void* pages;
+  const void* scales;
+  const int32_t* table;        // [n_slots, table_stride]
+  const int32_t* slots;        // [rows]
+  const int32_t* lens;         // [rows]
+  const int32_t* qstart;       // [rows + 1]
+  const int32_t* decode_rows;  // NULL: the step is decode rows alone, row i token i
+  const int32_t* chunk_rows;
+  const int32_t* group_start;  // [n_groups + 1]
+  const int32_t* group_lens;   // [n_groups]
+  const float* sink;           // [heads], nullable
+  int64_t page_stride, scale_stride, tokens;
+  int num_pages, table_stride, n_slots, rows, n_decode, max_decode_len, n_chunk, max_chunk_query, max_chunk_len, n_groups, max_group_query,
+      max_group_len, heads, kv_heads, head_dim, page_size, window, dtype;
+  float scale;
+};
+int64_t holon_cache_attention_room(const struct HolonCacheAttention* call);
+int holon_cache_attention(const struct HolonCacheAttention* call, const void* q, void* out, void* room, void* stream);
 // Drafted tokens against softmax(logits / temperature): see verify_drafts.hip. `room`: holon_verify_drafts_room bytes.
 int64_t holon_verify_drafts_room(int rows, int requests, int vocab);
 int holon_verify_drafts(const float* logits, const int32_t* drafted, const float* draft_probs, const float* accept,

@@ -35,30 +35,23 @@ struct Masses {
   double left, all;     // of max(p - q, 0), of p
 };
 
-// 2^z for z <= 0: a whole power, and on [-1/2, 1/2] the sum of (r ln 2)^k / k! up to k = 12, whose next term is below 2e-16.
+// 2^z for z <= 0, 0 for what is no number: a whole power, and on [-1/2, 1/2] the sum of (r ln 2)^k / k! up to k = 11, whose next
+// term is at most 7e-15.
 __device__ __forceinline__ double exp2_of(double z) {
   const double n = rint(z), r = z - n;
-  constexpr double C = 0.69314718055994530942;
-  const double x = r * C;
-  double p = 1.0 / 479001600.0;
-  p = fma(p, x, 1.0 / 39916800.0);
-  p = fma(p, x, 1.0 / 3628800.0);
-  p = fma(p, x, 1.0 / 362880.0);
-  p = fma(p, x, 1.0 / 40320.0);
-  p = fma(p, x, 1.0 / 5040.0);
-  p = fma(p, x, 1.0 / 720.0);
-  p = fma(p, x, 1.0 / 120.0);
-  p = fma(p, x, 1.0 / 24.0);
-  p = fma(p, x, 1.0 / 6.0);
-  p = fma(p, x, 0.5);
-  p = fma(p, x, 1.0);
-  p = fma(p, x, 1.0);
-  return z < -1000.0 ? 0.0 : ldexp(p, (int)fmax(n, -1100.0));
+  constexpr double L = 0.69314718055994530942;
+  constexpr double C[12] = {1.0, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, L * L * L * L * L / 120, L * L * L * L * L * L / 720,
+                            L * L * L * L * L * L * L / 5040, L * L * L * L * L * L * L * L / 40320, L * L * L * L * L * L * L * L * L / 362880,
+                            L * L * L * L * L * L * L * L * L * L / 3628800, L * L * L * L * L * L * L * L * L * L * L / 39916800};
+  double p = C[11];
+#pragma unroll
+  for (int k = 10; k >= 0; --k) p = fma(p, r, C[k]);
+  return z >= -1000.0 ? ldexp(p, (int)n) : 0.0;
 }
 // exp((l - max) / T): 1 at the largest value, also where that is infinite; nothing for what is no number.
 __device__ __forceinline__ double weight_of(float l, float max, double c) {
-  if (l == max) return l == -INFINITY ? 0.0 : 1.0;
-  return l < max && max < INFINITY ? exp2_of(((double)l - (double)max) * c) : 0.0;
+  if (fabsf(max) == INFINITY) return l == max && max > 0.f ? 1.0 : 0.0;      // (the same for all of a row)
+  return exp2_of(((double)l - (double)max) * c);
 }
 
 // The values of piece `lo` that a thread takes: 4 * (tid + 256 j) .. + 3, j < 4, in 16-byte loads where rows allow it.
@@ -114,11 +107,11 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const float* __res
   __shared__ float tops[THREADS / WAVE];
   __shared__ int ats[THREADS / WAVE];
   const int piece = blockIdx.x, row = blockIdx.y, lo = piece * PIECE;
+  float x[EACH];
+  load_piece(logits + (int64_t)row * vocab, lo, vocab, wide, -INFINITY, x);
   const int b = owner_of(start, requests, row);
   if (b < 0) return;                                          // a row behind the last request's (the same for the whole block)
   const double c = heat_of(temperature[b]);
-  float x[EACH];
-  load_piece(logits + (int64_t)row * vocab, lo, vocab, wide, -INFINITY, x);
   float top = -INFINITY;
   int at = 0x7fffffff;
 #pragma unroll
@@ -227,73 +220,94 @@ __global__ void __launch_bounds__(THREADS) verify_masses_kernel(const float* __r
   if (threadIdx.x == 0) masses[(int64_t)b * gridDim.x + piece] = Masses{left, all};
 }
 
+// Running sums over a block's threads, each thread's own among them; in an order that is the same for every call.
+__device__ __forceinline__ double block_upto64(double v, double* part) {
+  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+#pragma unroll
+  for (int o = 1; o < WAVE; o *= 2) {
+    const double before = __shfl_up(v, o, WAVE);
+    if (lane >= o) v += before;
+  }
+  if (lane == WAVE - 1) part[wave] = v;
+  __syncthreads();
+  double base = 0.0;
+  for (int w = 0; w < wave; ++w) base += part[w];
+  __syncthreads();
+  return base + v;
+}
+__device__ __forceinline__ int block_min(int v, int* part) {
+#pragma unroll
+  for (int o = WAVE / 2; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, WAVE));
+  if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = v;
+  __syncthreads();
+  v = min(min(part[0], part[1]), min(part[2], part[3]));
+  __syncthreads();
+  return v;
+}
+
 __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
                                                               const float* __restrict__ draft_probs, const float* __restrict__ draw,
                                                               const Judged* __restrict__ judged, const Masses* __restrict__ masses,
                                                               int32_t* __restrict__ tokens, int32_t* __restrict__ accepted,
                                                               int pieces, int vocab, int most) {
-  __shared__ double upto[THREADS];
-  __shared__ int found, last, chosen;
-  __shared__ double target, base;
+  __shared__ double part[THREADS / WAVE], total;
+  __shared__ int ints[THREADS / WAVE];
+  constexpr int NONE = 0x7fffffff;
   const int b = blockIdx.x, tid = threadIdx.x;
   const Judged j = judged[b];
   int token = j.token;
   if (j.row >= 0 && j.heat > 0.0) {
     const Masses* mine = masses + (int64_t)b * pieces;
-    if (tid == 0) {
-      double left = 0.0, all = 0.0;
-      for (int i = 0; i < pieces; ++i) { left += mine[i].left; all += mine[i].all; }
-      const bool use = left > 0.0;                            // (q = p everywhere leaves nothing: then from p)
-      const double want = (double)draw[b] * (use ? left : all);
-      double sum = 0.0, before = 0.0;
-      int pick = -1, heavy = -1;
-      for (int i = 0; i < pieces && pick < 0; ++i) {
-        const double m = use ? mine[i].left : mine[i].all;
-        if (m > 0.0) { heavy = i; before = sum; }
-        sum += m;
-        if (sum > want) pick = i;
-      }
-      chosen = pick >= 0 ? pick : heavy;                      // (a number so near one that rounding passed the last border)
-      base = before;
-      target = want;
-      found = 0x7fffffff;
-      last = use ? -1 : -2;
+    double left = 0.0, all = 0.0;
+    for (int i = tid; i < pieces; i += THREADS) { left += mine[i].left; all += mine[i].all; }
+    left = block_sum64(left, part);
+    all = block_sum64(all, part);
+    const bool use = left > 0.0;                              // (q = p everywhere leaves nothing: then from p)
+    const double target = (double)draw[b] * (use ? left : all);
+    // the piece in which the running sum passes the target, or (a number so near one that rounding passed the last border) the
+    // last one with any mass
+    int chosen = NONE, heavy = NONE;
+    double base = 0.0, carry = 0.0;
+    for (int at = 0; at < pieces; at += THREADS) {
+      const int i = at + tid;
+      const double m = i < pieces ? (use ? mine[i].left : mine[i].all) : 0.0, upto = carry + block_upto64(m, part);
+      if (tid == THREADS - 1) total = upto;
+      chosen = block_min(m > 0.0 && upto > target ? i : NONE, ints);
+      const int last = -block_min(m > 0.0 ? -i : NONE, ints);
+      const int pick = chosen != NONE ? chosen : last;        // (the last one with mass so far, -NONE: none here)
+      if (i == pick) part[0] = upto - m;
+      __syncthreads();
+      if (pick != -NONE) { heavy = pick; base = part[0]; }
+      carry = total;
+      __syncthreads();
+      if (chosen != NONE) break;
     }
-    __syncthreads();
-    const bool use = last == -1;
-    if (chosen >= 0) {
-      const int lo = chosen * PIECE + tid * EACH;
+    token = 0;                                                // no token has any mass
+    if (heavy != NONE) {
+      const int lo = heavy * PIECE + tid * EACH;
       const float* row = logits + (int64_t)j.row * vocab;
       const float* qrow = draft_probs != nullptr && j.draft >= 0 ? draft_probs + (int64_t)j.row * vocab : nullptr;
       double m[EACH], s = 0.0;
-      int heavy = -1;
+      int last = -1;
+#pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int x = lo + i;
         double p = x < vocab ? weight_of(row[x], j.max, j.heat) * j.inv_z : 0.0;
         if (use && x < vocab) p = qrow != nullptr ? fmax(p - (double)qrow[x], 0.0) : (x == j.draft ? 0.0 : p);
         m[i] = p;
         s += p;
-        if (p > 0.0) heavy = x;
+        if (p > 0.0) last = x;
       }
-      upto[tid] = s;
-      __syncthreads();
-      if (tid == 0) {                                         // running sums in order
-        double sum = base;
-        for (int i = 0; i < THREADS; ++i) { const double v = upto[i]; upto[i] = sum; sum += v; }
-      }
-      __syncthreads();
-      double sum = upto[tid];
-      int first = 0x7fffffff;
-      for (int i = 0; i < EACH && first == 0x7fffffff; ++i) {
+      double sum = base + (block_upto64(s, part) - s);
+      int first = NONE;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
         sum += m[i];
-        if (m[i] > 0.0 && sum > target) first = lo + i;
+        if (m[i] > 0.0 && sum > target) first = min(first, lo + i);
       }
-      if (first != 0x7fffffff) atomicMin(&found, first);      // (whole numbers: in any order the same)
-      if (heavy >= 0) atomicMax(&last, heavy);
-      __syncthreads();
-      token = found != 0x7fffffff ? found : max(last, 0);
-    } else {
-      token = 0;                                              // no token has any mass
+      first = block_min(first, ints);
+      last = -block_min(-last, ints);
+      token = first != NONE ? first : max(last, 0);
     }
   }
   for (int i = tid; i <= most; i += THREADS)

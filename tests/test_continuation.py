@@ -77,7 +77,7 @@ def _step(rows, heads, kv, d, page, *, seed=0, shared=(), dtype=torch.bfloat16, 
     dec, chk = np.flatnonzero(counts == 1), np.flatnonzero(counts > 1)
     attn = AttnRows(slots=i32(slots), lens=i32(lens), query_start=i32(np.concatenate([[0], np.cumsum(counts)])), decode_rows=i32(dec),
                     chunk_rows=i32(chk), n_decode=len(dec), n_chunk=len(chk), max_decode_len=int(lens[dec].max()) if len(dec) else 0,
-                    max_chunk_query=int(counts[chk].max()) if len(chk) else 0, max_chunk_len=int(lens[chk].max()) if len(chk) else 0)
+                    max_chunk_query=int(counts[chk].max()) if len(chk) else 0, max_chunk_len=int(lens[chk].max()) if len(chk) else 0, in_order=len(chk) == 0)
     q = (torch.randn(int(counts.sum()), heads, d, generator=g) * 1.5).to(dtype).to(device)
     if q8:
         kc, ke = quantise_q8(k)
@@ -200,12 +200,11 @@ class Refusing(ContinuationOps):
     def __init__(self):
         self.launched = []
 
-    @staticmethod
-    def _place(what, t):
-        return t.device
+    def _place(self, what, t):
+        return -1
 
     @staticmethod
-    def _stream():
+    def _stream_of(device):
         return 0
 
     def _call(self, fn, *args):
@@ -253,7 +252,7 @@ def test_refused_caches_and_rows():
         with pytest.raises(KernelError):
             bad()
     small = torch.zeros(2, 2, 1, 16 * 96, dtype=torch.uint8), torch.zeros(2, 2, 1, 16, dtype=torch.uint8)
-    with pytest.raises(KernelError, match="head_dim 96"):
+    with pytest.raises(KernelError, match="heads of 64"):
         ops.kv_read_q8(*small, at, at, 16)
     odd = torch.zeros(2, 2, 1, 8 * 64, dtype=torch.uint8), torch.zeros(2, 2, 1, 8, dtype=torch.uint8)
     with pytest.raises(KernelError):
