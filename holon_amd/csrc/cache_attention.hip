@@ -35,6 +35,7 @@ struct CacheArgs {
   const int32_t* row_ids;      // the rows of this launch (null: they are decode rows alone, in order)
   int n_tokens;
   int heads, kv_heads, page_size;
+  uint32_t page_magic;         // see page_index
   float scale_log2;            // scale * log2(e)
   int window;                  // see first_seen
   const float* sink;           // [Hq], nullable
@@ -48,6 +49,14 @@ struct CacheArgs {
   const int32_t* group_lens;
   int n_groups;
 };
+
+// The page that a position lies in: position / page_size, by a product (a division is forty vector instructions, also where every
+// lane asks the same, and a stage of 32 keys asks four times). With n = position / 16 and d = page_size / 16, the high half of n
+// ceil(2^32 / d) is n / d for n d < 2^32, which the host checks of a whole table row; magic 0: d = 1.
+__device__ __forceinline__ int page_index(const CacheArgs& a, int pos) {
+  const uint32_t n = (uint32_t)pos >> 4;
+  return (int)(a.page_magic ? __umulhi(n, a.page_magic) : n);
+}
 
 // What is out of range is not followed: the pool's last page, the table's last row.
 __device__ __forceinline__ int64_t page_at(const CacheArgs& a, int32_t page) {
@@ -121,6 +130,8 @@ template <bool Q8> __device__ __forceinline__ bool not_finite(uint32_t w) {
   if constexpr (Q8) return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
   else return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
+
+constexpr float SLACK = 8.f;   // see where it is used
 
 // A wave's tiles of 16 columns and where their sums stand.
 template <int D, int NT>
@@ -212,11 +223,11 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
       u32x4_t raw[SCORES][KLOADS], power;
     };
     const auto look = [&](int kb, int32_t& ek, int32_t& ev) {
-      ek = trow[min((kb + krun) / P, max_page)];
-      ev = trow[min((kb + RUN * g) / P, max_page)];
+      ek = trow[min(page_index(a, kb + krun), max_page)];
+      ev = trow[min(page_index(a, kb + RUN * g), max_page)];
     };
     const auto load_keys = [&](int kb, int32_t ek, Keys& to) {
-      const int at = (kb + krun) % P;
+      const int at = kb + krun - page_index(a, kb + krun) * P;
       const int64_t page = page_at(a, ek);
       const uint8_t* p = a.pages + page * a.page_stride + hk * plane + (int64_t)(at + c % 4) * D * bytes + 16 * g;
 #pragma unroll
@@ -261,7 +272,7 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
       const int vk = kb + RUN * g;
       u32x4_t vraw[D / 16], vs4 = {};
       {
-        const int at = vk % P;
+        const int at = vk - page_index(a, vk) * P;
         const int64_t page = page_at(a, ev);
         const uint8_t* p = a.pages + page * a.page_stride + (a.kv_heads + hk) * plane + ((int64_t)c * P + at) * bytes;
 #pragma unroll
@@ -335,8 +346,11 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
         for (int i = 1; i < RUN; ++i) mx = fmaxf(mx, sv[i]);
         mx = xor_max<16>(mx);
         mx = xor_max<32>(mx);
-        const float m_new = fmaxf(tl.m[t], mx * a.scale_log2);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        // The sums stand under a maximum that may lag behind: weights up to 2^SLACK lose nothing in float32 or in a rounding, and
+        // what was summed is rescaled in a few blocks, not in every one where one of 16 columns meets a new largest score.
+        const float top = mx * a.scale_log2;
+        const bool move = __any(top > tl.m[t] + SLACK);
+        const float m_new = move ? fmaxf(tl.m[t], top) : tl.m[t], m_use = m_new == -INFINITY ? 0.f : m_new;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < RUN; ++i) {
@@ -348,12 +362,12 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
 #pragma unroll
           for (int s = 0; s < PARTS; ++s) pb[t][i / 8][s][i % 8] = pp[s];
         }
-        alpha[t] = __builtin_amdgcn_exp2f(tl.m[t] - m_use);
-        moved |= m_new != tl.m[t];
+        alpha[t] = move ? __builtin_amdgcn_exp2f(tl.m[t] - m_use) : 1.f;
+        moved |= move;
         tl.m[t] = m_new;
         tl.l[t] = tl.l[t] * alpha[t] + sum;
       }
-      if (__any(moved)) {
+      if (moved) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -498,32 +512,39 @@ struct Stage {
   static __device__ __forceinline__ int row_of(int key) { return 8 * (2 * (key / 16) + key % 8 / 4) + 4 * (key % 16 / 8) + key % 4; }
   static __device__ __forceinline__ int swizzle(int row) { return D == 64 ? row / 2 % 8 : row % 16; }
 
-  // Asks for the stage at kb, whose halves lie in pages e0 and e1.
-  __device__ __forceinline__ void load(const CacheArgs& a, int hk, int kb, int64_t e0, int64_t e1) {
+  // Asks for the stage at kb, whose halves lie in pages e[0] and e[1]. Every load of a wave reads one half: its base is the same for
+  // all lanes, and what a lane adds to it is the same for every stage.
+  __device__ __forceinline__ void load(const CacheArgs& a, int hk, int kb, const int32_t (&e)[2]) {
     constexpr int B = Q8 ? 1 : 2;
     const int P = a.page_size, tid = threadIdx.x;
     const int64_t plane = (int64_t)P * D * B;
-    const int off0 = kb % P, off1 = (kb + 16) % P;
+    const uint8_t* base[2];
+    const uint8_t* power[2];
+    int off[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int64_t page = page_at(a, __builtin_amdgcn_readfirstlane(e[half]));
+      off[half] = kb + 16 * half - page_index(a, kb + 16 * half) * P;
+      base[half] = a.pages + page * a.page_stride + hk * plane;
+      power[half] = Q8 ? a.scales + page * a.scale_stride + (int64_t)hk * P + off[half] : nullptr;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int idx = tid + 256 * i;
       if (idx < HALF) {
         constexpr int CH = D * B / 16;
-        const int key = idx / CH, second = key / 16;
-        const int64_t page = second ? e1 : e0;
-        const int at = (second ? off1 : off0) + key % 16;
-        w[i] = *reinterpret_cast<const u32x4_t*>(a.pages + page * a.page_stride + hk * plane + (int64_t)at * D * B + idx % CH * 16);
-        if constexpr (Q8) ks[i] = a.scales[page * a.scale_stride + (int64_t)hk * P + at];
+        const int key = idx / CH, second = __builtin_amdgcn_readfirstlane(key / 16);
+        const uint8_t* from = (second ? base[1] : base[0]) + (int64_t)(second ? off[1] : off[0]) * (D * B);
+        w[i] = *reinterpret_cast<const u32x4_t*>(from + (uint32_t)(key % 16 * (D * B) + idx % CH * 16));
+        if constexpr (Q8) ks[i] = (second ? power[1] : power[0])[(uint32_t)(key % 16)];
       } else {
-        constexpr int CH = 2 * B;                          // pieces of a dim's 32 keys
-        const int v = idx - HALF, dim = v / CH, piece = v % CH, second = piece / B;
-        const int64_t page = second ? e1 : e0;
-        const int at = (second ? off1 : off0) + piece % B * 8;
-        w[i] = *reinterpret_cast<const u32x4_t*>(a.pages + page * a.page_stride + (a.kv_heads + hk) * plane + ((int64_t)dim * P + at) * B);
+        const int v = idx - HALF, dim = v % D, piece = v / D, second = __builtin_amdgcn_readfirstlane(piece / B);
+        const uint8_t* from = (second ? base[1] : base[0]) + a.kv_heads * plane + (second ? off[1] : off[0]) * B;
+        w[i] = *reinterpret_cast<const u32x4_t*>(from + (uint32_t)(dim * (P * B) + piece % B * 16));
       }
     }
     if constexpr (Q8) {
-      if (tid < 32) vs = a.scales[(tid < 16 ? e0 : e1) * a.scale_stride + (int64_t)(a.kv_heads + hk) * P + (tid < 16 ? off0 : off1) + tid % 16];
+      if (tid < 32) vs = (tid < 16 ? power[0] : power[1])[(int64_t)a.kv_heads * P + tid % 16];
     }
   }
   // Puts it into LDS. Values of keys outside [lo, hi] are cleared (they are not the row's). `watch`: so are values that are not
@@ -549,8 +570,7 @@ struct Stage {
           *reinterpret_cast<u32x4_t*>(to + 16 * (ch ^ swizzle(row))) = w[i];
         }
       } else {
-        constexpr int CH = Q8 ? 2 : 4;
-        const int v = idx - HALF, dim = v / CH, piece = v % CH;
+        const int v = idx - HALF, dim = v % D, piece = v / D;
         if (edge) {
           const int key = kb + piece * (Q8 ? 16 : 8);
 #pragma unroll
@@ -659,22 +679,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
       qf[ds] = __builtin_bit_cast(bf16x8_t, x);
     }
     const int32_t* trow = table_row(a, row);
-    const int max_page = a.table_stride - 1, P = a.page_size;
-    const auto look = [&](int kb, int64_t (&e)[2]) {
-      e[0] = page_at(a, trow[min(kb / P, max_page)]);
-      e[1] = page_at(a, trow[min((kb + 16) / P, max_page)]);
+    const int max_page = a.table_stride - 1;
+    const auto look = [&](int kb, int32_t (&e)[2]) {
+      e[0] = trow[min(page_index(a, kb), max_page)];
+      e[1] = trow[min(page_index(a, kb + 16), max_page)];
     };
     // queries of the block see different keys from here on, or up to here
     const auto differs = [&](int kb) { return kb + 31 > pos_first || kb < first_seen(pos_last, a.window); };
     const int kb_first = lo / 32 * 32;
     if (threadIdx.x < 2) odd_stage[threadIdx.x] = -1;
     S now, next, after;
-    int64_t e[2];
+    int32_t e[2];
     look(kb_first, e);
-    now.load(a, hk, kb_first, e[0], e[1]);
+    now.load(a, hk, kb_first, e);
     if (kb_first + 32 <= hi) {
       look(kb_first + 32, e);
-      next.load(a, hk, kb_first + 32, e[0], e[1]);
+      next.load(a, hk, kb_first + 32, e);
     }
     if (kb_first + 64 <= hi) look(kb_first + 64, e);
     lds_barrier();
@@ -683,7 +703,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
     int buf = 0;
     for (int kb = kb_first; kb <= hi; kb += 32) {
       if (kb + 64 <= hi) {
-        after.load(a, hk, kb + 64, e[0], e[1]);
+        after.load(a, hk, kb + 64, e);
         if (kb + 96 <= hi) look(kb + 96, e);
       }
       const unsigned char* st = lds[buf];
@@ -713,7 +733,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
         mx = xor_max<32>(mx);
-        const float m_new = fmaxf(m, mx * a.scale_log2), m_use = m_new == -INFINITY ? 0.f : m_new;
+        // (the maximum lags behind as above: 64 products a lane in a few stages, not where any of 32 columns meets a new one)
+        const float top = mx * a.scale_log2;
+        const bool move = __any(top > m + SLACK);
+        const float m_new = move ? fmaxf(m, top) : m, m_use = m_new == -INFINITY ? 0.f : m_new;
         bf16x8_t pb[2];
         float sum = 0.f;
 #pragma unroll
@@ -731,7 +754,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
             pb[t][i] = (__bf16)p;
           }
         }
-        if (__any(m_new != m)) {
+        if (move) {
           const float alpha = __builtin_amdgcn_exp2f(m - m_use);
           l *= alpha;
 #pragma unroll
@@ -1000,6 +1023,9 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
                   (c.n_chunk == 0 || c.max_chunk_query > 0), "attention: bad sizes");
   HOLON_CHECK(c.scale > 0.f, "attention: a scale of %g", (double)c.scale);
   HOLON_CHECK(c.page_stride % 16 == 0 && c.scale_stride % 16 == 0, "attention: pages lie on no borders of 16 bytes");
+  // (positions are 32-bit numbers; and see page_index)
+  HOLON_CHECK((int64_t)c.table_stride * c.page_size < (1ll << 31) && (int64_t)c.table_stride * c.page_size <= (1ll << 40) / c.page_size,
+              "attention: a table row of %d pages of %d tokens is too long", c.table_stride, c.page_size);
   if (c.tokens == 0) return 0;
   CacheArgs a{};
   a.q = q; a.out = out; a.pages = (const uint8_t*)c.pages; a.scales = (const uint8_t*)c.scales;
@@ -1007,6 +1033,7 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   a.table = c.table; a.table_stride = c.table_stride; a.n_slots = c.n_slots;
   a.slots = c.slots; a.lens = c.lens; a.qstart = c.qstart; a.n_tokens = (int)c.tokens;
   a.heads = heads; a.kv_heads = c.kv_heads; a.page_size = c.page_size;
+  a.page_magic = c.page_size > 16 ? (uint32_t)(((1ull << 32) + c.page_size / 16 - 1) / (c.page_size / 16)) : 0u;
   a.scale_log2 = c.scale * 1.4426950408889634f; a.window = c.window; a.sink = c.sink;
   const Plan p = plan_of(c);
   float* at = (float*)room;
