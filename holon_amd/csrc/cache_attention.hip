@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
 
 // Many columns over the same keys: a portion's queries, or all queries of a group's rows over their prefix. A block of four waves
 // takes 128 columns, a wave 32 on v_mfma_f32_32x32x16_bf16, and walks the keys in stages of 32, which its threads bring into LDS
-// as bfloat16 (codes are widened once a block, not once a wave): two buffers, and in registers the stage after the next.
+// as bfloat16 (codes are widened once a block, not once a wave): three buffers, the stage after the next on its way in registers.
 //   S^T (32 keys x 32 columns): A = 32 keys x 16 dims: lane (h, c) reads row c of the stage's keys, dims 8 h .. + 7 of 16. Row
 //     8 i + 4 h + r holds key 16 (i / 2) + 8 h + 4 (i % 2) + r, so that a lane's 16 scores are, in order, those of keys 8 h .. + 7
 //     of the stage's first 16 and of its last: the B operands of
@@ -637,10 +637,10 @@ struct Stage {
 template <int D, bool Q8>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(CacheArgs a, int by_group, int less_than) {
   using S = Stage<D, Q8>;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][S::BYTES];
-  __shared__ __attribute__((aligned(16))) float powers[2][32];
-  __shared__ uint32_t ups[2][D], downs[2][D];
-  __shared__ int odd_stage[2];                             // the key of a stage with values that are not finite
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[3][S::BYTES];
+  __shared__ __attribute__((aligned(16))) float powers[3][32];
+  __shared__ uint32_t ups[3][D], downs[3][D];
+  __shared__ int odd_stage[3];                             // the key of a stage with values that are not finite
   const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
   const int hk = blockIdx.x, piece = blockIdx.y % a.splits, group = a.heads / a.kv_heads;
   // the last columns first: theirs are the longest walks
@@ -687,23 +687,30 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
     // queries of the block see different keys from here on, or up to here
     const auto differs = [&](int kb) { return kb + 31 > pos_first || kb < first_seen(pos_last, a.window); };
     const int kb_first = lo / 32 * 32;
-    if (threadIdx.x < 2) odd_stage[threadIdx.x] = -1;
-    S now, next, after;
+    const auto store = [&](S& s, int kb, int buf) {
+      if (s.store(lds[buf], powers[buf], (uint8_t*)ups[buf], (uint8_t*)downs[buf], kb, lo, hi, differs(kb))) odd_stage[buf] = kb;
+    };
+    if (threadIdx.x < 3) odd_stage[threadIdx.x] = -1;
+    S coming;
     int32_t e[2];
-    look(kb_first, e);
-    now.load(a, hk, kb_first, e);
-    if (kb_first + 32 <= hi) {
-      look(kb_first + 32, e);
-      next.load(a, hk, kb_first + 32, e);
+    {
+      S first_stage;
+      look(kb_first, e);
+      first_stage.load(a, hk, kb_first, e);
+      if (kb_first + 32 <= hi) {
+        look(kb_first + 32, e);
+        coming.load(a, hk, kb_first + 32, e);
+      }
+      if (kb_first + 64 <= hi) look(kb_first + 64, e);
+      lds_barrier();
+      store(first_stage, kb_first, 0);
+      if (kb_first + 32 <= hi) store(coming, kb_first + 32, 1);
     }
-    if (kb_first + 64 <= hi) look(kb_first + 64, e);
-    lds_barrier();
-    if (now.store(lds[0], powers[0], (uint8_t*)ups[0], (uint8_t*)downs[0], kb_first, lo, hi, differs(kb_first))) odd_stage[0] = kb_first;
     lds_barrier();
     int buf = 0;
     for (int kb = kb_first; kb <= hi; kb += 32) {
       if (kb + 64 <= hi) {
-        after.load(a, hk, kb + 64, e);
+        coming.load(a, hk, kb + 64, e);
         if (kb + 96 <= hi) look(kb + 96, e);
       }
       const unsigned char* st = lds[buf];
@@ -719,6 +726,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
           for (int ds = 0; ds < AT_ONCE; ++ds) kf[ds] = S::key(st, d0 + ds);
 #pragma unroll
           for (int ds = 0; ds < AT_ONCE; ++ds) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ds], qf[d0 + ds], sc, 0, 0, 0);
+        }
+        // the values are asked for before the softmax that their products wait for
+        bf16x8_t vf[D / 32][2];
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+          vf[db][0] = S::value(st, db, 0);
+          vf[db][1] = S::value(st, db, 1);
         }
         // score 8 t + i of this lane: key kb + 16 t + 8 h + i
         const bool whole = kb >= max(lo, whole_from) && kb + 31 <= min(hi, tile_first);
@@ -764,9 +778,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
         l += sum;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) {
-          const bf16x8_t v0 = S::value(st, db, 0), v1 = S::value(st, db, 1);
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pb[0], o[db], 0, 0, 0);
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, pb[1], o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db][0], pb[0], o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db][1], pb[1], o[db], 0, 0, 0);
         }
         if (odd_stage[buf] == kb) {                        // values that are not finite: to the columns that see them alone
           uint32_t seen = 0;                               // a bit a key
@@ -783,12 +796,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
             }
         }
       }
-      if (kb + 32 <= hi) {
-        if (next.store(lds[buf ^ 1], powers[buf ^ 1], (uint8_t*)ups[buf ^ 1], (uint8_t*)downs[buf ^ 1], kb + 32, lo, hi, differs(kb + 32))) odd_stage[buf ^ 1] = kb + 32;
-        lds_barrier();
-        buf ^= 1;
-        next = after;
-      }
+      if (kb + 64 <= hi) store(coming, kb + 64, buf == 0 ? 2 : buf - 1);      // the buffer that was read a stage ago
+      lds_barrier();
+      buf = buf == 2 ? 0 : buf + 1;
     }
   }
   l = xor_sum<32>(l);
