@@ -51,12 +51,9 @@ struct CacheArgs {
 };
 
 // The page that a position lies in: position / page_size, by a product (a division is forty vector instructions, also where every
-// lane asks the same, and a stage of 32 keys asks four times). With n = position / 16 and d = page_size / 16, the high half of n
-// ceil(2^32 / d) is n / d for n d < 2^32, which the host checks of a whole table row; magic 0: d = 1.
-__device__ __forceinline__ int page_index(const CacheArgs& a, int pos) {
-  const uint32_t n = (uint32_t)pos >> 4;
-  return (int)(a.page_magic ? __umulhi(n, a.page_magic) : n);
-}
+// lane asks the same, and a stage of 32 keys asks four times). With magic = ceil(2^32 / P), the high half of position * magic is the
+// quotient while position * (magic P - 2^32) < 2^32, which the host checks of a whole table row (a P that is a power of two: always).
+__device__ __forceinline__ int page_index(const CacheArgs& a, int pos) { return (int)__umulhi((uint32_t)pos, a.page_magic); }
 
 // What is out of range is not followed: the pool's last page, the table's last row.
 __device__ __forceinline__ int64_t page_at(const CacheArgs& a, int32_t page) {
@@ -500,51 +497,66 @@ __global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::
 //     of the stage's first 16 and of its last: the B operands of
 //   O^T (32 dims x 32 columns) += V^T P^T: A = 32 dims x 16 keys, the values transposed as in the pages.
 // Rows of LDS are swizzled by pieces of 16 bytes, so that 16 lanes that read one piece of 16 rows touch every bank once.
-template <int D, bool Q8>
+template <int D, bool Q8, int WAVES>
 struct Stage {
-  static constexpr int K_BYTES = 32 * D * 2, BYTES = 2 * K_BYTES;
-  static constexpr int N = Q8 ? D / 64 : D / 32;           // 16-byte loads a thread, keys first, then values
-  static constexpr int HALF = Q8 ? 2 * D : 4 * D;          // loads of keys in all
+  static constexpr int K_BYTES = 32 * D * 2, BYTES = 2 * K_BYTES, THREADS = WAVES * WAVE;
+  static constexpr int HALF = Q8 ? 2 * D : 4 * D;          // 16-byte loads of keys in all, and as many of values behind them
+  static constexpr int N = (2 * HALF + THREADS - 1) / THREADS;      // of a thread
+  // A load reads one half of the stage, 16 keys of one page, the same one for all lanes of its wave; where a thread has four loads and
+  // more, which half is known here, else a wave's loads share theirs.
+  static constexpr bool ONE_HALF = HALF / 2 % THREADS != 0;
   u32x4_t w[N];
-  uint32_t ks[N];                                          // a key's scale
-  uint32_t vs;                                             // threads 0 .. 31: a value's
+  uint32_t ks[N];                                          // a key's scale; in 16 threads of each half's, a value's
 
   static __device__ __forceinline__ int row_of(int key) { return 8 * (2 * (key / 16) + key % 8 / 4) + 4 * (key % 16 / 8) + key % 4; }
   static __device__ __forceinline__ int swizzle(int row) { return D == 64 ? row / 2 % 8 : row % 16; }
+  static __device__ __forceinline__ int half_of(int i) {
+    return ONE_HALF ? __builtin_amdgcn_readfirstlane((threadIdx.x + THREADS * i) % HALF / (HALF / 2)) : THREADS * i % HALF / (HALF / 2);
+  }
 
-  // Asks for the stage at kb, whose halves lie in pages e[0] and e[1]. Every load of a wave reads one half: its base is the same for
-  // all lanes, and what a lane adds to it is the same for every stage.
+  // The table's entries of the stage at kb that a wave needs.
+  static __device__ __forceinline__ void look(const CacheArgs& a, const int32_t* trow, int kb, int32_t (&e)[2]) {
+    const int last = a.table_stride - 1;
+    if constexpr (ONE_HALF) {
+      e[0] = trow[min(page_index(a, kb + 16 * half_of(0)), last)];
+    } else {
+      e[0] = trow[min(page_index(a, kb), last)];
+      e[1] = trow[min(page_index(a, kb + 16), last)];
+    }
+  }
+  // Asks for it: what a lane adds to its load's base is the same for every stage.
   __device__ __forceinline__ void load(const CacheArgs& a, int hk, int kb, const int32_t (&e)[2]) {
     constexpr int B = Q8 ? 1 : 2;
-    const int P = a.page_size, tid = threadIdx.x;
-    const int64_t plane = (int64_t)P * D * B;
-    const uint8_t* base[2];
-    const uint8_t* power[2];
-    int off[2];
+    const uint32_t P = a.page_size, plane = P * D * B;
+    const uint8_t* keys[2];
+    const uint8_t* values[2];
+    const uint8_t* powers[2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int64_t page = page_at(a, __builtin_amdgcn_readfirstlane(e[half]));
-      off[half] = kb + 16 * half - page_index(a, kb + 16 * half) * P;
-      base[half] = a.pages + page * a.page_stride + hk * plane;
-      power[half] = Q8 ? a.scales + page * a.scale_stride + (int64_t)hk * P + off[half] : nullptr;
+    for (int x = 0; x < (ONE_HALF ? 1 : 2); ++x) {
+      const int from = kb + 16 * (ONE_HALF ? half_of(0) : x);
+      const uint32_t off = from - page_index(a, from) * P;
+      const uint64_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(e[x]), (uint32_t)(a.num_pages - 1));
+      const uint8_t* base = a.pages + page * (uint32_t)a.page_stride;
+      keys[x] = base + (hk * plane + off * (D * B));
+      values[x] = base + ((a.kv_heads + hk) * plane + off * B);
+      if constexpr (Q8) powers[x] = a.scales + page * (uint32_t)a.scale_stride + (hk * P + off);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + 256 * i;
+      const int idx = threadIdx.x + THREADS * i, x = ONE_HALF ? 0 : half_of(i);
+      if (2 * HALF % THREADS != 0 && idx >= 2 * HALF) break;
       if (idx < HALF) {
         constexpr int CH = D * B / 16;
-        const int key = idx / CH, second = __builtin_amdgcn_readfirstlane(key / 16);
-        const uint8_t* from = (second ? base[1] : base[0]) + (int64_t)(second ? off[1] : off[0]) * (D * B);
-        w[i] = *reinterpret_cast<const u32x4_t*>(from + (uint32_t)(key % 16 * (D * B) + idx % CH * 16));
-        if constexpr (Q8) ks[i] = (second ? power[1] : power[0])[(uint32_t)(key % 16)];
+        const uint32_t key = idx / CH % 16;
+        w[i] = *reinterpret_cast<const u32x4_t*>(keys[x] + (key * (D * B) + idx % CH * 16));
+        if constexpr (Q8) ks[i] = powers[x][key];
       } else {
-        const int v = idx - HALF, dim = v % D, piece = v / D, second = __builtin_amdgcn_readfirstlane(piece / B);
-        const uint8_t* from = (second ? base[1] : base[0]) + a.kv_heads * plane + (second ? off[1] : off[0]) * B;
-        w[i] = *reinterpret_cast<const u32x4_t*>(from + (uint32_t)(dim * (P * B) + piece % B * 16));
+        const uint32_t v = idx - HALF, dim = v % D, piece = v / D;
+        w[i] = *reinterpret_cast<const u32x4_t*>(values[x] + (dim * (P * B) + piece % B * 16));
+        if constexpr (Q8) {
+          if (dim < 16) ks[i] = powers[x][a.kv_heads * P + dim];
+        }
       }
-    }
-    if constexpr (Q8) {
-      if (tid < 32) vs = (tid < 16 ? power[0] : power[1])[(int64_t)a.kv_heads * P + tid % 16];
     }
   }
   // Puts it into LDS. Values of keys outside [lo, hi] are cleared (they are not the row's). `watch`: so are values that are not
@@ -556,7 +568,8 @@ struct Stage {
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + 256 * i;
+      const int idx = tid + THREADS * i;
+      if (2 * HALF % THREADS != 0 && idx >= 2 * HALF) break;
       if (idx < HALF) {
         constexpr int CH = D * (Q8 ? 1 : 2) / 16;
         const int row = row_of(idx / CH), ch = idx % CH;
@@ -611,6 +624,10 @@ struct Stage {
         const int turn = dim / 8 % 2;
         if constexpr (Q8) {
           bf16x8_t x, y;
+          if (dim < 16) {                                  // (key `dim` of the half: its power)
+            const int key = kb + 16 * piece + dim;
+            powers[16 * piece + dim] = key >= lo && key <= hi ? q8_power(ks[i]) : 0.f;
+          }
           widen(w[i], 1.f, x, y);
           *reinterpret_cast<bf16x8_t*>(to + 16 * turn) = x;
           *reinterpret_cast<bf16x8_t*>(to + 16 * (1 ^ turn)) = y;
@@ -618,9 +635,6 @@ struct Stage {
           *reinterpret_cast<u32x4_t*>(to + 16 * (piece % 2 ^ turn)) = w[i];
         }
       }
-    }
-    if constexpr (Q8) {
-      if (tid < 32) powers[tid] = kb + tid >= lo && kb + tid <= hi ? q8_power(vs) : 0.f;
     }
     return odd;
   }
@@ -634,26 +648,29 @@ struct Stage {
   }
 };
 
-template <int D, bool Q8>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(CacheArgs a, int by_group, int less_than) {
-  using S = Stage<D, Q8>;
+template <int D, bool Q8, int WAVES>
+__global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) cache_tiles_kernel(CacheArgs a, int by_group, int less_than, int folded) {
+  using S = Stage<D, Q8, WAVES>;
+  constexpr int COLUMNS = 32 * WAVES;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[3][S::BYTES];
   __shared__ __attribute__((aligned(16))) float powers[3][32];
   __shared__ uint32_t ups[3][D], downs[3][D];
   __shared__ int odd_stage[3];                             // the key of a stage with values that are not finite
   const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
   const int hk = blockIdx.x, piece = blockIdx.y % a.splits, group = a.heads / a.kv_heads;
-  // the last columns first: theirs are the longest walks
-  const int tile = gridDim.y / a.splits - 1 - blockIdx.y / a.splits;
+  // The last columns' walks are the longest: they begin. Where all blocks run at once, two a compute unit, the second half begins
+  // with the shortest, so that the two that share a unit have about the same to do together.
+  const int tiles = gridDim.y / a.splits, nth = blockIdx.y / a.splits;
+  const int tile = folded && nth >= (tiles + 1) / 2 ? nth - (tiles + 1) / 2 : tiles - 1 - nth;
   const Job job = job_of(a, by_group, blockIdx.z);
   const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
   const int columns = nq * group;
-  if (tile * 128 >= columns || (!by_group && nq <= less_than)) return;
-  const int f0 = tile * 128 + 32 * wave, f = f0 + c;
+  if (tile * COLUMNS >= columns || (!by_group && nq <= less_than)) return;
+  const int f0 = tile * COLUMNS + 32 * wave, f = f0 + c;
   Column col = column_of(a, f, hk, group, qs, nq, n);
   const int behind = n - nq;                               // the first query's position
-  const int pos_first = by_group ? n - 1 : behind + tile * 128 / group;
-  const int pos_last = by_group ? n - 1 : behind + min(tile * 128 + 127, columns - 1) / group;
+  const int pos_first = by_group ? n - 1 : behind + tile * COLUMNS / group;
+  const int pos_last = by_group ? n - 1 : behind + min(tile * COLUMNS + COLUMNS - 1, columns - 1) / group;
   if (by_group) col.pos = n - 1;
   const int tile_first = by_group ? n - 1 : behind + f0 / group;
   const int tile_last = f0 >= columns ? -1 : by_group ? n - 1 : behind + min(f0 + 31, columns - 1) / group;
@@ -679,13 +696,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
       qf[ds] = __builtin_bit_cast(bf16x8_t, x);
     }
     const int32_t* trow = table_row(a, row);
-    const int max_page = a.table_stride - 1;
-    const auto look = [&](int kb, int32_t (&e)[2]) {
-      e[0] = trow[min(page_index(a, kb), max_page)];
-      e[1] = trow[min(page_index(a, kb + 16), max_page)];
-    };
     // queries of the block see different keys from here on, or up to here
-    const auto differs = [&](int kb) { return kb + 31 > pos_first || kb < first_seen(pos_last, a.window); };
+    const int seen_last = first_seen(pos_last, a.window), seen_tile = a.window ? first_seen(tile_first, a.window) : 0;
+    const auto differs = [&](int kb) { return kb + 31 > pos_first || kb < seen_last; };
     const int kb_first = lo / 32 * 32;
     const auto store = [&](S& s, int kb, int buf) {
       if (s.store(lds[buf], powers[buf], (uint8_t*)ups[buf], (uint8_t*)downs[buf], kb, lo, hi, differs(kb))) odd_stage[buf] = kb;
@@ -695,13 +708,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
     int32_t e[2];
     {
       S first_stage;
-      look(kb_first, e);
+      S::look(a, trow, kb_first, e);
       first_stage.load(a, hk, kb_first, e);
       if (kb_first + 32 <= hi) {
-        look(kb_first + 32, e);
+        S::look(a, trow, kb_first + 32, e);
         coming.load(a, hk, kb_first + 32, e);
       }
-      if (kb_first + 64 <= hi) look(kb_first + 64, e);
+      if (kb_first + 64 <= hi) S::look(a, trow, kb_first + 64, e);
       lds_barrier();
       store(first_stage, kb_first, 0);
       if (kb_first + 32 <= hi) store(coming, kb_first + 32, 1);
@@ -711,10 +724,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
     for (int kb = kb_first; kb <= hi; kb += 32) {
       if (kb + 64 <= hi) {
         coming.load(a, hk, kb + 64, e);
-        if (kb + 96 <= hi) look(kb + 96, e);
+        if (kb + 96 <= hi) S::look(a, trow, kb + 96, e);
       }
       const unsigned char* st = lds[buf];
-      if (kb <= tile_last && kb + 31 >= (a.window ? first_seen(tile_first, a.window) : 0)) {
+      if (kb <= tile_last && kb + 31 >= seen_tile) {
         f32x16_t sc;
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = 0.f;
@@ -724,9 +737,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) cache_tiles_kernel(Cach
           bf16x8_t kf[AT_ONCE];
 #pragma unroll
           for (int ds = 0; ds < AT_ONCE; ++ds) kf[ds] = S::key(st, d0 + ds);
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int ds = 0; ds < AT_ONCE; ++ds) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ds], qf[d0 + ds], sc, 0, 0, 0);
         }
+        __builtin_amdgcn_s_setprio(0);
         // the values are asked for before the softmax that their products wait for
         bf16x8_t vf[D / 32][2];
 #pragma unroll
@@ -899,7 +914,14 @@ void launch_size(const CacheArgs& a, const Cut& c, int jobs, int by_group, int m
   constexpr bool F32 = std::is_same<QT, float>::value;
   if constexpr (!F32) {
     if (c.tiles) {
-      cache_tiles_kernel<D, Q8><<<dim3(a.kv_heads, c.tiles * c.splits, jobs), 256, 0, s>>>(a, by_group, less_than);
+      const dim3 grid(a.kv_heads, c.tiles * c.splits, jobs);
+      if constexpr (D <= 128) {
+        if (c.waves == 8) {
+          cache_tiles_kernel<D, Q8, 8><<<grid, 512, 0, s>>>(a, by_group, less_than, 0);
+          return;
+        }
+      }
+      cache_tiles_kernel<D, Q8, 4><<<grid, 256, 0, s>>>(a, by_group, less_than, (int64_t)grid.x * grid.y * grid.z <= 512);
       return;
     }
   }
@@ -938,8 +960,10 @@ Cut cut_keys(int jobs, int64_t columns, int64_t span, int kv_heads, int head_dim
   span = std::max<int64_t>(span, 1);
   columns = std::max<int64_t>(columns, 1);
   if (columns > FEW_COLUMNS && !f32) {
-    r.tiles = (int)((columns + 127) / 128);
-    const int64_t want = std::max<int64_t>(1, 512 / (units * r.tiles));                 // two blocks a compute unit
+    const int64_t wide = (columns + 255) / 256;            // blocks of 256 columns, where there are more than run at once
+    r.waves = head_dim <= 128 && units * wide >= 512 ? 8 : 4;
+    r.tiles = (int)((columns + 32 * r.waves - 1) / (32 * r.waves));
+    const int64_t want = std::max<int64_t>(1, 2048 / r.waves / (units * r.tiles));      // two waves a SIMD
     r.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (span + 127) / 128));
     return r;
   }
@@ -992,9 +1016,7 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
     p.shared = cut_keys(n_groups, (int64_t)max_group_query * group, max_group_len, kv_heads, head_dim, f32);
     // every cell has the prefix's parts and then as many of its row's own whichever kernel made them
     const int own = p.any_decode ? p.decode.parts() : p.any_few ? p.few.parts() : p.many.parts();
-    p.decode.splits = own * p.decode.waves;
-    p.few.splits = own * p.few.waves;
-    p.many.splits = own;
+    for (Cut* cut : {&p.decode, &p.few, &p.many}) cut->splits = cut->tiles ? own : own * cut->waves;
     p.parts = p.shared.parts() + own;
     p.decode_cells = (int64_t)n_tokens * heads * p.parts;
   } else {
@@ -1034,8 +1056,10 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   HOLON_CHECK(c.scale > 0.f, "attention: a scale of %g", (double)c.scale);
   HOLON_CHECK(c.page_stride % 16 == 0 && c.scale_stride % 16 == 0, "attention: pages lie on no borders of 16 bytes");
   // (positions are 32-bit numbers; and see page_index)
-  HOLON_CHECK((int64_t)c.table_stride * c.page_size < (1ll << 31) && (int64_t)c.table_stride * c.page_size <= (1ll << 40) / c.page_size,
+  const uint64_t magic = ((1ull << 32) + c.page_size - 1) / c.page_size, excess = magic * c.page_size - (1ull << 32);
+  HOLON_CHECK((int64_t)c.table_stride * c.page_size < (1ll << 31) - 256 && ((uint64_t)c.table_stride * c.page_size + 256) * excess < (1ull << 32),
               "attention: a table row of %d pages of %d tokens is too long", c.table_stride, c.page_size);
+  HOLON_CHECK(c.page_stride < (1ll << 32) && c.scale_stride < (1ll << 32), "attention: pages lie too far apart");
   if (c.tokens == 0) return 0;
   CacheArgs a{};
   a.q = q; a.out = out; a.pages = (const uint8_t*)c.pages; a.scales = (const uint8_t*)c.scales;
@@ -1043,7 +1067,7 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   a.table = c.table; a.table_stride = c.table_stride; a.n_slots = c.n_slots;
   a.slots = c.slots; a.lens = c.lens; a.qstart = c.qstart; a.n_tokens = (int)c.tokens;
   a.heads = heads; a.kv_heads = c.kv_heads; a.page_size = c.page_size;
-  a.page_magic = c.page_size > 16 ? (uint32_t)(((1ull << 32) + c.page_size / 16 - 1) / (c.page_size / 16)) : 0u;
+  a.page_magic = (uint32_t)magic;
   a.scale_log2 = c.scale * 1.4426950408889634f; a.window = c.window; a.sink = c.sink;
   const Plan p = plan_of(c);
   float* at = (float*)room;
