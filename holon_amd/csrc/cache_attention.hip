@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) 
   __shared__ __attribute__((aligned(16))) float powers[3][32];
   __shared__ uint32_t ups[3][D], downs[3][D];
   __shared__ int odd_stage[3];                             // the key of a stage with values that are not finite
-  const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
   const int hk = blockIdx.x, piece = blockIdx.y % a.splits, group = a.heads / a.kv_heads;
   // The last columns' walks are the longest: they begin. Where all blocks run at once, two a compute unit, the second half begins
   // with the shortest, so that the two that share a unit have about the same to do together.
@@ -953,15 +953,18 @@ void launch_merge(const CacheArgs& a, const Launch& w, int max_query, int less_t
 // once for every 32 of them.
 constexpr int FEW_COLUMNS = 64;
 
-// `jobs` rows (or groups) of up to `columns` columns over up to `span` keys.
-Cut cut_keys(int jobs, int64_t columns, int64_t span, int kv_heads, int head_dim, bool f32) {
+// `jobs` rows of up to `queries` queries, or groups (0: all see all keys), up to `columns` columns in all over up to `span` keys.
+Cut cut_keys(int jobs, int64_t columns, int64_t span, int64_t queries, int kv_heads, int head_dim, bool f32) {
   Cut r;
   const int64_t units = std::max<int64_t>(1, (int64_t)jobs * kv_heads);
   span = std::max<int64_t>(span, 1);
   columns = std::max<int64_t>(columns, 1);
   if (columns > FEW_COLUMNS && !f32) {
-    const int64_t wide = (columns + 255) / 256;            // blocks of 256 columns, where there are more than run at once
-    r.waves = head_dim <= 128 && units * wide >= 512 ? 8 : 4;
+    // Blocks of 256 columns (a stage is brought in once for twice the columns; one block a compute unit) where there is one for every
+    // unit and the first ones' walks are not much shorter than the last ones', or two. Heads 32 over 8 of 128, us, 128 columns | 256:
+    // 4,096 tokens behind 28,672 3,000 | 2,783, 2,048 behind 6,144 359 | 347, a whole prompt of 2,048 81 | 91.
+    const int64_t wide = units * ((columns + 255) / 256);
+    r.waves = head_dim <= 128 && (wide >= 512 || (wide >= 256 && 2 * queries <= span)) ? 8 : 4;
     r.tiles = (int)((columns + 32 * r.waves - 1) / (32 * r.waves));
     const int64_t want = std::max<int64_t>(1, 2048 / r.waves / (units * r.tiles));      // two waves a SIMD
     r.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (span + 127) / 128));
@@ -1007,13 +1010,13 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
   p.any_few = n_chunk > 0 && few > 1;
   p.any_many = n_chunk > 0 && max_chunk_query > few;
   if (p.any_many && n_chunk == 1) p.any_few = false;       // (the one row is as long as the longest)
-  p.decode = cut_keys(n_decode, group, seen_span(own_decode, 1, window), kv_heads, head_dim, f32);
-  p.few = cut_keys(n_chunk, (int64_t)few * group, seen_span(own_chunk, few, window), kv_heads, head_dim, f32);
+  p.decode = cut_keys(n_decode, group, seen_span(own_decode, 1, window), 1, kv_heads, head_dim, f32);
+  p.few = cut_keys(n_chunk, (int64_t)few * group, seen_span(own_chunk, few, window), few, kv_heads, head_dim, f32);
   p.many = cut_keys(n_chunk, std::max<int64_t>((int64_t)max_chunk_query * group, FEW_COLUMNS + 1), seen_span(own_chunk, max_chunk_query, window),
-                    kv_heads, head_dim, f32);
+                    max_chunk_query, kv_heads, head_dim, f32);
   p.by_token = p.any_shared;
   if (p.by_token) {
-    p.shared = cut_keys(n_groups, (int64_t)max_group_query * group, max_group_len, kv_heads, head_dim, f32);
+    p.shared = cut_keys(n_groups, (int64_t)max_group_query * group, max_group_len, 0, kv_heads, head_dim, f32);
     // every cell has the prefix's parts and then as many of its row's own whichever kernel made them
     const int own = p.any_decode ? p.decode.parts() : p.any_few ? p.few.parts() : p.many.parts();
     for (Cut* cut : {&p.decode, &p.few, &p.many}) cut->splits = cut->tiles ? own : own * cut->waves;
