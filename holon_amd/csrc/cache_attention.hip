@@ -173,19 +173,18 @@ constexpr int most_waves(int D, bool f32, int NT) { return D == 256 || f32 || NT
 // Whether a wave may take two tiles of columns: what they hold then fits its registers.
 constexpr bool two_tiles(int D, bool f32) { return D <= 128 && !f32; }
 
+// `at`: which tiles of columns and which share of the keys; `red`: (waves - 1) * NT * (16 D + 32) numbers of LDS.
 template <int D, bool Q8, typename QT, int NT>
-__global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::value, NT)) cache_rows_kernel(CacheArgs a, int by_group, int max_query) {
+__device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int max_query, int at, int hk, int ri, float* red) {
   constexpr int PARTS = std::is_same<QT, float>::value ? 3 : 1;
   constexpr int KB = Q8 ? 64 : 32, RUN = KB / 4, SCORES = KB / 16, PV = KB / 32;
   constexpr int KLOADS = Q8 ? D / 64 : D / 32;             // 16-byte loads of a key's share
-  constexpr int PART = 16 * D + 32;
-  extern __shared__ __attribute__((aligned(16))) float red[];   // [waves - 1][NT][16 D values, 16 maxima, 16 sums]
+  constexpr int PART = 16 * D + 32;                        // [waves - 1][NT][16 D values, 16 maxima, 16 sums]
   const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, waves = blockDim.x / WAVE;
   const int g = lane / 16, c = lane % 16;
-  const int ri = blockIdx.z, hk = blockIdx.y;
   const int group = a.heads / a.kv_heads, P = a.page_size;
   const int out_splits = a.splits / waves;
-  const int tile0 = blockIdx.x / out_splits * NT, piece = blockIdx.x % out_splits;
+  const int tile0 = at / out_splits * NT, piece = at % out_splits;
   const Job job = job_of(a, by_group, ri);
   const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
   if (tile0 * 16 >= nq * group || (!by_group && nq > max_query)) return;      // (the same for the whole block)
@@ -649,20 +648,31 @@ struct Stage {
 };
 
 template <int D, bool Q8, int WAVES>
-__global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) cache_tiles_kernel(CacheArgs a, int by_group, int less_than, int folded) {
+struct TilesLds {
+  __attribute__((aligned(1024))) unsigned char stage[3][Stage<D, Q8, WAVES>::BYTES];
+  __attribute__((aligned(16))) float powers[3][32];
+  uint32_t ups[3][D], downs[3][D];
+  int odd_stage[3];                                        // the key of a stage with values that are not finite
+};
+
+// `at`: which columns (of `blocks` / a.splits tiles of them) and which share of the keys.
+template <int D, bool Q8, int WAVES>
+__device__ __forceinline__ void tiles_block(const CacheArgs& a, int by_group, int less_than, int folded, int at, int blocks, int hk, int ri,
+                                            TilesLds<D, Q8, WAVES>& sh) {
   using S = Stage<D, Q8, WAVES>;
   constexpr int COLUMNS = 32 * WAVES;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[3][S::BYTES];
-  __shared__ __attribute__((aligned(16))) float powers[3][32];
-  __shared__ uint32_t ups[3][D], downs[3][D];
-  __shared__ int odd_stage[3];                             // the key of a stage with values that are not finite
+  auto& lds = sh.stage;
+  auto& powers = sh.powers;
+  auto& ups = sh.ups;
+  auto& downs = sh.downs;
+  auto& odd_stage = sh.odd_stage;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE, h = lane / 32, c = lane % 32;
-  const int hk = blockIdx.x, piece = blockIdx.y % a.splits, group = a.heads / a.kv_heads;
+  const int piece = at % a.splits, group = a.heads / a.kv_heads;
   // The last columns' walks are the longest: they begin. Where all blocks run at once, two a compute unit, the second half begins
   // with the shortest, so that the two that share a unit have about the same to do together.
-  const int tiles = gridDim.y / a.splits, nth = blockIdx.y / a.splits;
+  const int tiles = blocks / a.splits, nth = at / a.splits;
   const int tile = folded && nth >= (tiles + 1) / 2 ? nth - (tiles + 1) / 2 : tiles - 1 - nth;
-  const Job job = job_of(a, by_group, blockIdx.z);
+  const Job job = job_of(a, by_group, ri);
   const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
   const int columns = nq * group;
   if (tile * COLUMNS >= columns || (!by_group && nq <= less_than)) return;
@@ -834,7 +844,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) 
         *reinterpret_cast<ushort4*>(op + 32 * db + 8 * i) = w;
       }
   } else {
-    const int64_t place = a.cell_queries > 0 ? (int64_t)blockIdx.z * a.cell_queries + (col.token - qs) : col.token;
+    const int64_t place = a.cell_queries > 0 ? (int64_t)ri * a.cell_queries + (col.token - qs) : col.token;
     const int64_t cell = (place * a.heads + col.head) * a.parts + a.part_first + piece;
     float* po = a.part_o + cell * D + 4 * h;
 #pragma unroll
@@ -847,6 +857,38 @@ __global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) 
       const int64_t none = (place * a.heads + col.head) * a.parts;
       for (int i = h; i < a.part_first; i += 2) { a.part_ml[2 * (none + i)] = -INFINITY; a.part_ml[2 * (none + i) + 1] = 0.f; }
     }
+  }
+}
+
+template <int D, bool Q8, typename QT, int NT>
+__global__ void __launch_bounds__(WAVE * most_waves(D, std::is_same<QT, float>::value, NT)) cache_rows_kernel(CacheArgs a, int by_group,
+                                                                                                             int max_query) {
+  extern __shared__ __attribute__((aligned(16))) float red[];
+  rows_block<D, Q8, QT, NT>(a, by_group, max_query, blockIdx.x, blockIdx.y, blockIdx.z, red);
+}
+
+template <int D, bool Q8, int WAVES>
+__global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) cache_tiles_kernel(CacheArgs a, int by_group, int less_than,
+                                                                                                   int folded) {
+  __shared__ TilesLds<D, Q8, WAVES> sh;
+  tiles_block<D, Q8, WAVES>(a, by_group, less_than, folded, blockIdx.y, gridDim.y, blockIdx.x, blockIdx.z, sh);
+}
+
+// The groups' prefixes and the rows' own keys in one launch: neither fills the GPU by itself for long (the first are few long
+// walks, the second many short ones), and a block of one kind waits beside a block of the other. Blocks of the first kind come first.
+template <int D, bool Q8, bool TILES>
+__global__ void __launch_bounds__(256, 2) cache_prefix_kernel(CacheArgs p, CacheArgs r, int prefix_blocks, int groups, int row_blocks,
+                                                              int max_query) {
+  using Tiles = TilesLds<D, Q8, 4>;
+  __shared__ __attribute__((aligned(1024))) unsigned char mem[TILES ? sizeof(Tiles) : 3 * (16 * D + 32) * sizeof(float)];
+  static_assert(sizeof(Tiles) >= 3 * (16 * D + 32) * sizeof(float), "the rows' sums fit where the stages lie");
+  const int hk = blockIdx.x % p.kv_heads, at = blockIdx.x / p.kv_heads;
+  if (at < prefix_blocks * groups) {
+    if constexpr (TILES) tiles_block<D, Q8, 4>(p, 1, 0, 0, at % prefix_blocks, prefix_blocks, hk, at / prefix_blocks, *reinterpret_cast<Tiles*>(mem));
+    else rows_block<D, Q8, bf16_t, 1>(p, 1, 0, at % prefix_blocks, hk, at / prefix_blocks, reinterpret_cast<float*>(mem));
+  } else {
+    const int x = at - prefix_blocks * groups;
+    rows_block<D, Q8, bf16_t, 1>(r, 0, max_query, x % row_blocks, hk, x / row_blocks, reinterpret_cast<float*>(mem));
   }
 }
 
@@ -942,6 +984,21 @@ void launch_kind(const CacheArgs& a, const Launch& w, const Cut& c, int jobs, in
   else if (w.dtype == HOLON_BF16) launch_size<D, true, bf16_t>(a, c, jobs, by_group, most, less_than, w.stream);
   else launch_size<D, true, float>(a, c, jobs, by_group, most, less_than, w.stream);
 }
+// The prefix kernel: groups cut by `shared`, `n_rows` rows of up to `most` queries that leave `own` parts each.
+template <int D>
+void launch_prefix(const CacheArgs& p, const CacheArgs& r, const Launch& w, const Cut& shared, int groups, int64_t group_columns, int n_rows, int most,
+                   int own) {
+  const int prefix_blocks = (shared.tiles ? shared.tiles : (int)((group_columns + 15) / 16)) * shared.parts();
+  const int row_blocks = (int)(((int64_t)most * (r.heads / r.kv_heads) + 15) / 16) * own;
+  const dim3 grid((unsigned)(p.kv_heads * ((int64_t)prefix_blocks * groups + (int64_t)row_blocks * n_rows)));
+  const auto go = [&](auto q8) {
+    constexpr bool Q8 = decltype(q8)::value;
+    if (shared.tiles) cache_prefix_kernel<D, Q8, true><<<grid, 256, 0, w.stream>>>(p, r, prefix_blocks, groups, row_blocks, most);
+    else cache_prefix_kernel<D, Q8, false><<<grid, 256, 0, w.stream>>>(p, r, prefix_blocks, groups, row_blocks, most);
+  };
+  if (w.q8) go(std::true_type{});
+  else go(std::false_type{});
+}
 template <int D>
 void launch_merge(const CacheArgs& a, const Launch& w, int max_query, int less_than, int64_t cells) {
   const unsigned blocks = (unsigned)((cells + 256 / (D / 4) - 1) / (256 / (D / 4)));
@@ -993,7 +1050,7 @@ int64_t seen_span(int64_t len, int64_t queries, int window) {
 struct Plan {
   Cut decode, few, many, shared;
   int few_query = 0;                       // rows of up to so many queries are among the few
-  bool any_decode, any_few, any_many, any_shared, by_token;
+  bool any_decode, any_few, any_many, any_shared, by_token, together = false;
   int parts = 1;                           // of a cell, where cells go by token
   int64_t decode_cells = 0, few_cells = 0, many_cells = 0;
 };
@@ -1018,7 +1075,28 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
   if (p.by_token) {
     p.shared = cut_keys(n_groups, (int64_t)max_group_query * group, max_group_len, 0, kv_heads, head_dim, f32);
     // every cell has the prefix's parts and then as many of its row's own whichever kernel made them
-    const int own = p.any_decode ? p.decode.parts() : p.any_few ? p.few.parts() : p.many.parts();
+    int own = p.any_decode ? p.decode.parts() : p.any_few ? p.few.parts() : p.many.parts();
+    // one launch for both where there is one kind of rows, of few columns
+    const Cut& rows = p.any_decode ? p.decode : p.few;
+    p.together = p.any_decode != p.any_few && !p.any_many && head_dim <= 128 && !f32 && !rows.tiles;
+    if (p.together) {
+      const int64_t units = (int64_t)n_groups * kv_heads;
+      if (p.shared.tiles) {                                // one block a compute unit, the rows' blocks beside them
+        p.shared.waves = 4;
+        p.shared.tiles = (int)(((int64_t)max_group_query * group + 127) / 128);
+        const int64_t want = std::max<int64_t>(1, 256 / (units * p.shared.tiles));
+        p.shared.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (max_group_len + 127) / 128));
+      } else {
+        const int64_t tiles = ((int64_t)max_group_query * group + 15) / 16;
+        const int64_t want = std::max<int64_t>(1, 256 / (units * tiles)), shares = std::max(1, (max_group_len + 63) / 64);
+        p.shared.two = 0;
+        p.shared.waves = 4;
+        p.shared.splits = 4 * (int)std::min<int64_t>(std::min<int64_t>(want, 32), (shares + 3) / 4);
+      }
+      const int64_t jobs = (p.any_decode ? n_decode : n_chunk) * (int64_t)kv_heads;
+      const int64_t span = p.any_decode ? own_decode : own_chunk;
+      own = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, 512 / jobs), (span + 255) / 256));
+    }
     for (Cut* cut : {&p.decode, &p.few, &p.many}) cut->splits = cut->tiles ? own : own * cut->waves;
     p.parts = p.shared.parts() + own;
     p.decode_cells = (int64_t)n_tokens * heads * p.parts;
@@ -1089,6 +1167,20 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   if (p.by_token) {
     a.group_start = c.group_start; a.group_lens = c.group_lens; a.n_groups = c.n_groups;
     a.parts = p.parts; a.part_o = at; a.part_ml = at + p.decode_cells * head_dim;
+    if (p.together) {
+      CacheArgs r = a;
+      const int own = p.parts - p.shared.parts(), n_rows = p.any_decode ? c.n_decode : c.n_chunk, most = p.any_decode ? 1 : p.few_query;
+      a.splits = p.shared.splits;
+      r.row_ids = p.any_decode ? c.decode_rows : c.chunk_rows;
+      r.splits = own * 4;
+      r.part_first = p.shared.parts();
+      const int64_t columns = (int64_t)c.max_group_query * (heads / c.kv_heads);
+      if (head_dim == 64) launch_prefix<64>(a, r, w, p.shared, c.n_groups, columns, n_rows, most, own);
+      else launch_prefix<128>(a, r, w, p.shared, c.n_groups, columns, n_rows, most, own);
+      merge(1, 0, c.tokens * heads);
+      HOLON_LAUNCH_OK();
+      return 0;
+    }
     launch(p.shared, c.n_groups, 1, c.max_group_query, 0);
     a.part_first = p.shared.parts();
   }
