@@ -1011,7 +1011,7 @@ void launch_merge(const CacheArgs& a, const Launch& w, int max_query, int less_t
 constexpr int FEW_COLUMNS = 64;
 
 // `jobs` rows of up to `queries` queries, or groups (0: all see all keys), up to `columns` columns in all over up to `span` keys.
-Cut cut_keys(int jobs, int64_t columns, int64_t span, int64_t queries, int kv_heads, int head_dim, bool f32) {
+Cut cut_keys(int jobs, int64_t columns, int64_t span, int64_t queries, int kv_heads, int head_dim, int value_bytes, bool f32) {
   Cut r;
   const int64_t units = std::max<int64_t>(1, (int64_t)jobs * kv_heads);
   span = std::max<int64_t>(span, 1);
@@ -1034,10 +1034,14 @@ Cut cut_keys(int jobs, int64_t columns, int64_t span, int64_t queries, int kv_he
   const int64_t shares = std::max<int64_t>(1, (span + per - 1) / per);
   const int64_t blocks = pairs <= 16 ? 256 : 512;
   const int cap = most_waves(head_dim, f32, 1 + r.two);
-  // few enough shares meet in one block, and no merge follows
-  const int64_t outer = shares <= cap ? 1 : std::min(shares, std::max<int64_t>(1, (blocks + pairs - 1) / pairs));
+  // A block's waves take all of a row's keys, and no merge follows, where a wave has 16 KB of keys at most. One block | several and
+  // the merge, us in a graph, where the merge's own launch costs least: 32 heads over 8 of 128, 8 bits, 4 rows of 600 / 1,000 / 1,500 keys
+  // 10.6 / 11.6 / 15.2 | 8.8 / 9.2 / 11.1, 16 rows 10.8 / 12.8 / 17.4 | 11.3 / 13.1 / 17.0; 16 over 8 of 64, 4 rows of 1,000 / 2,000 / 3,000 7.4 /
+  // 10.7 / 13.4 | 8.3 / 8.9 / 9.1. A call that is not recorded spends 4 us on the second launch.
+  const bool one = span * head_dim * value_bytes <= (int64_t)16384 * cap;
+  const int64_t outer = one ? 1 : std::min(shares, std::max<int64_t>(1, (blocks + pairs - 1) / pairs));
   r.waves = (int)std::min<int64_t>(cap, (shares + outer - 1) / outer);
-  r.splits = (int)((shares + r.waves - 1) / r.waves) * r.waves;
+  r.splits = one ? r.waves : (int)((shares + r.waves - 1) / r.waves) * r.waves;
   return r;
 }
 int64_t seen_span(int64_t len, int64_t queries, int window) {
@@ -1055,10 +1059,16 @@ struct Plan {
   int64_t decode_cells = 0, few_cells = 0, many_cells = 0;
 };
 Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query, int max_chunk_len, int n_groups, int max_group_query,
-             int max_group_len, int64_t n_tokens, int heads, int kv_heads, int head_dim, int window, bool f32) {
+             int max_group_len, int64_t n_tokens, int heads, int kv_heads, int head_dim, int window, int value_bytes, bool f32) {
   Plan p;
   const int group = heads / kv_heads;
   p.any_shared = n_groups > 0 && max_group_query > 0 && max_group_len > 0;
+  // Decode rows that one block each serves read their prefix themselves, from L2, while the GPU has room for all blocks: one launch
+  // for two. (A wave has half as much more than above: the other side has a merge in any case.)
+  const int64_t alone = (int64_t)16384 * most_waves(head_dim, f32, 1) * 3 / 2;
+  const bool one_each = p.any_shared && n_chunk == 0 && group <= 16 && (int64_t)n_decode * kv_heads <= 256 &&
+                        (int64_t)max_decode_len * head_dim * value_bytes <= alone;
+  if (one_each) p.any_shared = false;
   const int own_decode = p.any_shared ? std::max(max_decode_len - max_group_len, 64) : max_decode_len;
   const int own_chunk = p.any_shared ? std::max(max_chunk_len - max_group_len, 64) : max_chunk_len;
   const int few = f32 ? max_chunk_query : std::min(max_chunk_query, std::max(1, FEW_COLUMNS / group));
@@ -1067,13 +1077,14 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
   p.any_few = n_chunk > 0 && few > 1;
   p.any_many = n_chunk > 0 && max_chunk_query > few;
   if (p.any_many && n_chunk == 1) p.any_few = false;       // (the one row is as long as the longest)
-  p.decode = cut_keys(n_decode, group, seen_span(own_decode, 1, window), 1, kv_heads, head_dim, f32);
-  p.few = cut_keys(n_chunk, (int64_t)few * group, seen_span(own_chunk, few, window), few, kv_heads, head_dim, f32);
+  p.decode = cut_keys(n_decode, group, seen_span(own_decode, 1, window), 1, kv_heads, head_dim, value_bytes, f32);
+  if (one_each) p.decode.splits = p.decode.waves = (int)std::min<int64_t>(most_waves(head_dim, f32, 1), (max_decode_len + 63) / 64);
+  p.few = cut_keys(n_chunk, (int64_t)few * group, seen_span(own_chunk, few, window), few, kv_heads, head_dim, value_bytes, f32);
   p.many = cut_keys(n_chunk, std::max<int64_t>((int64_t)max_chunk_query * group, FEW_COLUMNS + 1), seen_span(own_chunk, max_chunk_query, window),
-                    max_chunk_query, kv_heads, head_dim, f32);
+                    max_chunk_query, kv_heads, head_dim, value_bytes, f32);
   p.by_token = p.any_shared;
   if (p.by_token) {
-    p.shared = cut_keys(n_groups, (int64_t)max_group_query * group, max_group_len, 0, kv_heads, head_dim, f32);
+    p.shared = cut_keys(n_groups, (int64_t)max_group_query * group, max_group_len, 0, kv_heads, head_dim, value_bytes, f32);
     // every cell has the prefix's parts and then as many of its row's own whichever kernel made them
     int own = p.any_decode ? p.decode.parts() : p.any_few ? p.few.parts() : p.many.parts();
     // one launch for both where there is one kind of rows, of few columns
@@ -1084,7 +1095,7 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
       if (p.shared.tiles) {                                // one block a compute unit, the rows' blocks beside them
         p.shared.waves = 4;
         p.shared.tiles = (int)(((int64_t)max_group_query * group + 127) / 128);
-        const int64_t want = std::max<int64_t>(1, 256 / (units * p.shared.tiles));
+        const int64_t want = std::max<int64_t>(1, 384 / (units * p.shared.tiles));
         p.shared.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (max_group_len + 127) / 128));
       } else {
         const int64_t tiles = ((int64_t)max_group_query * group + 15) / 16;
@@ -1112,7 +1123,7 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
 
 static Plan plan_of(const HolonCacheAttention& c) {
   return plan_of(c.n_decode, c.max_decode_len, c.n_chunk, c.max_chunk_query, c.max_chunk_len, c.n_groups, c.max_group_query, c.max_group_len,
-                 c.tokens, c.heads, c.kv_heads, c.head_dim, c.window, c.dtype == HOLON_F32);
+                 c.tokens, c.heads, c.kv_heads, c.head_dim, c.window, c.scales != nullptr ? 1 : 2, c.dtype == HOLON_F32);
 }
 
 extern "C" int64_t holon_cache_attention_room(const HolonCacheAttention* call) {

@@ -12,12 +12,15 @@
 //
 // Three launches over pieces of 4,096 values: every row's largest value and sum of exponentials; the judgement (each block of a
 // request works it out for itself from those) and its masses; the walk through the one piece that the drawn number falls into.
+// (The walk by the last block to leave its masses, which saves a launch, took the judgement's launch over 64 requests from 28 to 111 us:
+// to see the others' masses across the XCDs each block writes back and drops what its L2 holds of the logits.)
 #include "common.h"
 #include "holon_hip.h"
 
 namespace {
 
 constexpr int PIECE = 4096, THREADS = 256, EACH = PIECE / THREADS, MOST = 64;   // MOST: rows a request may have
+constexpr int NONE = 0x7fffffff;
 
 struct RowPart {        // of one piece of one row
   double sum;           // of 2^((l - max) c), c = log2(e) / T
@@ -26,33 +29,39 @@ struct RowPart {        // of one piece of one row
 };
 struct Judged {         // of one request
   double inv_z;         // 1 / sum of the end row
-  double heat;          // log2(e) / T; 0: T = 0
+  double heat;          // log2(e) / T; 0: T = 0, the token is known
   float max;            // of the end row
-  int row, accepted, draft;   // the end row, how many drafts were taken, the one that was not (-1: none was judged)
-  int token;            // T = 0: the token itself
+  int row, accepted, draft;   // the end row (-1: no rows), how many drafts were taken, the one that was not (-1: none was judged)
+  int token;
 };
 struct Masses {
   double left, all;     // of max(p - q, 0), of p
 };
 
-// 2^z for z <= 0, 0 for what is no number: a whole power, and on [-1/2, 1/2] the sum of (r ln 2)^k / k! up to k = 11, whose next
-// term is at most 7e-15.
-__device__ __forceinline__ double exp2_of(double z) {
-  const double n = rint(z), r = z - n;
-  constexpr double L = 0.69314718055994530942;
-  constexpr double C[12] = {1.0, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, L * L * L * L * L / 120, L * L * L * L * L * L / 720,
-                            L * L * L * L * L * L * L / 5040, L * L * L * L * L * L * L * L / 40320, L * L * L * L * L * L * L * L * L / 362880,
-                            L * L * L * L * L * L * L * L * L * L / 3628800, L * L * L * L * L * L * L * L * L * L * L / 39916800};
-  double p = C[11];
+// exp((l - max) / T) as 2^z, z = (l - max) c with c = log2(e) / T: 2^n times, on [-1/2, 1/2], the sum of (r ln 2)^k / k! up to
+// k = 11, whose next term is at most 7e-15. Adding 1.5 2^52 rounds z to a whole number and leaves it in the low bits, from where it
+// goes into the exponent: three additions where rounding, converting and scaling each take four times an addition's cycles.
+// 1 at the largest value, also where that is infinite; nothing below 2^-1000 of it, and nothing for what is no number.
+struct Weight {
+  double c, max64;
+  float max;
+  bool infinite;
+  __device__ __forceinline__ Weight(float max_, double c_) : c(c_), max64(max_), max(max_), infinite(fabsf(max_) == INFINITY) {}
+  __device__ __forceinline__ double operator()(float l) const {
+    constexpr double L = 0.69314718055994530942, MAGIC = 6755399441055744.0;
+    constexpr double C[12] = {1.0, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, L * L * L * L * L / 120, L * L * L * L * L * L / 720,
+                              L * L * L * L * L * L * L / 5040, L * L * L * L * L * L * L * L / 40320, L * L * L * L * L * L * L * L * L / 362880,
+                              L * L * L * L * L * L * L * L * L * L / 3628800, L * L * L * L * L * L * L * L * L * L * L / 39916800};
+    if (infinite) return l == max && max > 0.f ? 1.0 : 0.0;          // (the same for all of a row)
+    const double z = ((double)l - max64) * c, t = z + MAGIC, r = z - (t - MAGIC);      // (exactly 0 at the largest, however small T is)
+    double p = C[11];
 #pragma unroll
-  for (int k = 10; k >= 0; --k) p = fma(p, r, C[k]);
-  return z >= -1000.0 ? ldexp(p, (int)n) : 0.0;
-}
-// exp((l - max) / T): 1 at the largest value, also where that is infinite; nothing for what is no number.
-__device__ __forceinline__ double weight_of(float l, float max, double c) {
-  if (fabsf(max) == INFINITY) return l == max && max > 0.f ? 1.0 : 0.0;      // (the same for all of a row)
-  return exp2_of(((double)l - (double)max) * c);
-}
+    for (int k = 10; k >= 0; --k) p = fma(p, r, C[k]);
+    const uint64_t bits = __builtin_bit_cast(uint64_t, p);
+    const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, t) << 20);
+    return z >= -1000.0 ? __builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)bits) : 0.0;
+  }
+};
 
 // The values of piece `lo` that a thread takes: 4 * (tid + 256 j) .. + 3, j < 4, in 16-byte loads where rows allow it.
 __device__ __forceinline__ void load_piece(const float* __restrict__ row, int lo, int vocab, bool wide, float fill, float (&x)[EACH]) {
@@ -113,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const float* __res
   if (b < 0) return;                                          // a row behind the last request's (the same for the whole block)
   const double c = heat_of(temperature[b]);
   float top = -INFINITY;
-  int at = 0x7fffffff;
+  int at = NONE;
 #pragma unroll
   for (int i = 0; i < EACH; ++i)                              // (a thread's places grow with i; what is no number is never larger)
     if (x[i] > top) { top = x[i]; at = place_of(lo, i); }
@@ -130,8 +139,9 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const float* __res
     if (tops[w] > top || (tops[w] == top && ats[w] < at)) { top = tops[w]; at = ats[w]; }
   double s = 0.0;
   if (c > 0.0) {
+    const Weight weight(top, c);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) s += weight_of(x[i], top, c);
+    for (int i = 0; i < EACH; ++i) s += weight(x[i]);
     s = block_sum64(s, sums);
   }
   if (threadIdx.x == 0) parts[(int64_t)row * gridDim.x + piece] = RowPart{s, top, at};
@@ -142,7 +152,7 @@ __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const float* __res
 __device__ __forceinline__ RowPart whole_row(const RowPart* __restrict__ parts, int pieces, double c) {
   const int lane = threadIdx.x % WAVE;
   float top = -INFINITY;
-  int at = 0x7fffffff;
+  int at = NONE;
   for (int i = lane; i < pieces; i += WAVE) {
     const RowPart p = parts[i];
     if (p.max > top || (p.max == top && p.at < at)) { top = p.max; at = p.at; }
@@ -154,80 +164,26 @@ __device__ __forceinline__ RowPart whole_row(const RowPart* __restrict__ parts, 
     if (t2 > top || (t2 == top && a2 < at)) { top = t2; at = a2; }
   }
   double s = 0.0;
-  if (c > 0.0)
-    for (int i = lane; i < pieces; i += WAVE) s += parts[i].sum * weight_of(parts[i].max, top, c);
+  if (c > 0.0) {
+    const Weight weight(top, c);
+    for (int i = lane; i < pieces; i += WAVE) s += parts[i].sum * weight(parts[i].max);
+  }
   return RowPart{wave_sum64(s), top, at};
 }
 
-__global__ void __launch_bounds__(THREADS) verify_masses_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
-                                                                const float* __restrict__ draft_probs, const float* __restrict__ accept,
-                                                                const float* __restrict__ temperature,
-                                                                const int32_t* __restrict__ start, const RowPart* __restrict__ parts,
-                                                                Judged* __restrict__ judged, Masses* __restrict__ masses, int rows,
-                                                                int vocab, int most, int wide) {
-  __shared__ RowPart whole[MOST];
-  __shared__ int verdict[MOST];                               // 1: taken, 0: turned down, -1: nothing to judge
-  __shared__ double sums[THREADS / WAVE];
-  const int piece = blockIdx.x, b = blockIdx.y, wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
-  const int first = max(start[b], 0), n = min(min(start[b + 1], rows) - first, most + 1);
-  if (n <= 0) {
-    if (piece == 0 && threadIdx.x == 0) judged[b] = Judged{0.0, 0.0, 0.f, -1, 0, -1, -1};
-    return;
-  }
-  const double c = heat_of(temperature[b]);
-  for (int i = wave; i < n; i += THREADS / WAVE) {
-    const RowPart w = whole_row(parts + (int64_t)(first + i) * gridDim.x, gridDim.x, c);
-    if (lane == 0) {
-      whole[i] = w;
-      int v = -1;
-      const int x = drafted[first + i];
-      if (i + 1 < n && x >= 0 && x < vocab) {
-        const int64_t at = (int64_t)(first + i) * vocab + x;
-        if (c > 0.0) {
-          const double q = draft_probs != nullptr ? (double)draft_probs[at] : 1.0;
-          v = (double)accept[first + i] * q * w.sum <= weight_of(logits[at], w.max, c) ? 1 : 0;
-        } else {
-          v = x == (w.at == 0x7fffffff ? 0 : w.at) ? 1 : 0;
-        }
-      }
-      verdict[i] = v;
-    }
-  }
-  __syncthreads();
-  int end = 0;
-  while (end < n - 1 && verdict[end] == 1) ++end;
-  const bool turned_down = verdict[end] == 0;
-  const RowPart w = whole[end];
-  const int row = first + end, draft = turned_down ? drafted[row] : -1;
-  const double inv_z = w.sum > 0.0 ? 1.0 / w.sum : 0.0;
-  if (piece == 0 && threadIdx.x == 0)
-    judged[b] = Judged{inv_z, c, w.max, row, end, draft, w.at == 0x7fffffff ? 0 : w.at};
-  if (c == 0.0) return;
-  float x[EACH], q[EACH];
-  const int lo = piece * PIECE;
-  load_piece(logits + (int64_t)row * vocab, lo, vocab, wide, -INFINITY, x);
-  const bool by_probs = turned_down && draft_probs != nullptr;
-  if (by_probs) load_piece(draft_probs + (int64_t)row * vocab, lo, vocab, wide, 0.f, q);
-  double left = 0.0, all = 0.0;
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const double p = weight_of(x[i], w.max, c) * inv_z;
-    all += p;
-    left += by_probs ? fmax(p - (double)q[i], 0.0) : (place_of(lo, i) == draft ? 0.0 : p);
-  }
-  all = block_sum64(all, sums);
-  left = block_sum64(left, sums);
-  if (threadIdx.x == 0) masses[(int64_t)b * gridDim.x + piece] = Masses{left, all};
-}
-
-// Running sums over a block's threads, each thread's own among them; in an order that is the same for every call.
-__device__ __forceinline__ double block_upto64(double v, double* part) {
-  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+// Running sums over a wave's lanes and a block's threads, each one's own among them; in an order that is the same for every call.
+__device__ __forceinline__ double wave_upto64(double v) {
+  const int lane = threadIdx.x % WAVE;
 #pragma unroll
   for (int o = 1; o < WAVE; o *= 2) {
     const double before = __shfl_up(v, o, WAVE);
     if (lane >= o) v += before;
   }
+  return v;
+}
+__device__ __forceinline__ double block_upto64(double v, double* part) {
+  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+  v = wave_upto64(v);
   if (lane == WAVE - 1) part[wave] = v;
   __syncthreads();
   double base = 0.0;
@@ -245,45 +201,102 @@ __device__ __forceinline__ int block_min(int v, int* part) {
   return v;
 }
 
+__global__ void __launch_bounds__(THREADS) verify_masses_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
+                                                                const float* __restrict__ draft_probs, const float* __restrict__ accept,
+                                                                const float* __restrict__ temperature,
+                                                                const int32_t* __restrict__ start, const RowPart* __restrict__ parts,
+                                                                Judged* __restrict__ judged, Masses* __restrict__ masses, int rows,
+                                                                int vocab, int most, int wide) {
+  __shared__ RowPart whole[MOST];
+  __shared__ int verdict[MOST];                               // 1: taken, 0: turned down, -1: nothing to judge
+  __shared__ double part[THREADS / WAVE];
+  const int piece = blockIdx.x, pieces = gridDim.x, b = blockIdx.y, tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+  const int first = max(start[b], 0), n = min(min(start[b + 1], rows) - first, most + 1);
+  if (n <= 0) {
+    if (piece == 0 && tid == 0) judged[b] = Judged{0.0, 0.0, 0.f, -1, 0, -1, -1};
+    return;
+  }
+  const double c = heat_of(temperature[b]);
+  for (int i = wave; i < n; i += THREADS / WAVE) {
+    const int row = first + i, x = drafted[row];              // (what the judgement needs is asked for before the sums are added)
+    const bool may = i + 1 < n && x >= 0 && x < vocab;
+    const int64_t at = (int64_t)row * vocab + (may ? x : 0);
+    const float lx = logits[at], qx = draft_probs != nullptr ? draft_probs[at] : 1.f, u = accept[row];
+    const RowPart w = whole_row(parts + (int64_t)row * pieces, pieces, c);
+    const bool good = c > 0.0 ? (double)u * (double)qx * w.sum <= Weight(w.max, c)(lx) : x == (w.at == NONE ? 0 : w.at);
+    if (lane == 0) {
+      whole[i] = w;
+      verdict[i] = may ? (good ? 1 : 0) : -1;
+    }
+  }
+  __syncthreads();
+  int end = 0;
+  while (end < n - 1 && verdict[end] == 1) ++end;
+  const bool turned_down = verdict[end] == 0, by_probs = turned_down && draft_probs != nullptr;
+  const RowPart w = whole[end];
+  const int row = first + end, draft = turned_down ? drafted[row] : -1;
+  const double inv_z = w.sum > 0.0 ? 1.0 / w.sum : 0.0;
+  if (piece == 0 && tid == 0) judged[b] = Judged{inv_z, c, w.max, row, end, draft, w.at == NONE ? 0 : w.at};
+  if (c == 0.0) return;
+  const Weight weight(w.max, c);
+  float x[EACH], q[EACH];
+  load_piece(logits + (int64_t)row * vocab, piece * PIECE, vocab, wide, -INFINITY, x);
+  if (by_probs) load_piece(draft_probs + (int64_t)row * vocab, piece * PIECE, vocab, wide, 0.f, q);
+  double left = 0.0, all = 0.0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const double p = weight(x[i]) * inv_z;
+    all += p;
+    left += by_probs ? fmax(p - (double)q[i], 0.0) : (place_of(piece * PIECE, i) == draft ? 0.0 : p);
+  }
+  all = block_sum64(all, part);
+  left = block_sum64(left, part);
+  if (tid == 0) masses[(int64_t)b * pieces + piece] = Masses{left, all};
+}
+
 __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
                                                               const float* __restrict__ draft_probs, const float* __restrict__ draw,
                                                               const Judged* __restrict__ judged, const Masses* __restrict__ masses,
                                                               int32_t* __restrict__ tokens, int32_t* __restrict__ accepted,
                                                               int pieces, int vocab, int most) {
-  __shared__ double part[THREADS / WAVE], total;
+  __shared__ double part[THREADS / WAVE];
   __shared__ int ints[THREADS / WAVE];
-  constexpr int NONE = 0x7fffffff;
-  const int b = blockIdx.x, tid = threadIdx.x;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % WAVE;
   const Judged j = judged[b];
+  const Masses* mine = masses + (int64_t)b * pieces;
+  const Masses early = mine[min(lane, pieces - 1)];           // (asked for with the judgement)
+  const float u = draw[b];
   int token = j.token;
   if (j.row >= 0 && j.heat > 0.0) {
-    const Masses* mine = masses + (int64_t)b * pieces;
+    // Every wave finds the piece for itself, 64 pieces at a time: the one in which the running sum passes the target, or (a number
+    // so near one that rounding passed the last border) the last one with any mass.
     double left = 0.0, all = 0.0;
-    for (int i = tid; i < pieces; i += THREADS) { left += mine[i].left; all += mine[i].all; }
-    left = block_sum64(left, part);
-    all = block_sum64(all, part);
+    for (int at = 0; at < pieces; at += WAVE) {
+      const Masses m = at == 0 ? early : mine[min(at + lane, pieces - 1)];
+      left += at + lane < pieces ? m.left : 0.0;
+      all += at + lane < pieces ? m.all : 0.0;
+    }
+    left = wave_sum64(left);
+    all = wave_sum64(all);
     const bool use = left > 0.0;                              // (q = p everywhere leaves nothing: then from p)
-    const double target = (double)draw[b] * (use ? left : all);
-    // the piece in which the running sum passes the target, or (a number so near one that rounding passed the last border) the
-    // last one with any mass
-    int chosen = NONE, heavy = NONE;
+    const double target = (double)u * (use ? left : all);
+    int heavy = NONE;
     double base = 0.0, carry = 0.0;
-    for (int at = 0; at < pieces; at += THREADS) {
-      const int i = at + tid;
-      const double m = i < pieces ? (use ? mine[i].left : mine[i].all) : 0.0, upto = carry + block_upto64(m, part);
-      if (tid == THREADS - 1) total = upto;
-      chosen = block_min(m > 0.0 && upto > target ? i : NONE, ints);
-      const int last = -block_min(m > 0.0 ? -i : NONE, ints);
-      const int pick = chosen != NONE ? chosen : last;        // (the last one with mass so far, -NONE: none here)
-      if (i == pick) part[0] = upto - m;
-      __syncthreads();
-      if (pick != -NONE) { heavy = pick; base = part[0]; }
-      carry = total;
-      __syncthreads();
-      if (chosen != NONE) break;
+    for (int at = 0; at < pieces; at += WAVE) {
+      const Masses x = at == 0 ? early : mine[min(at + lane, pieces - 1)];
+      const double m = at + lane < pieces ? (use ? x.left : x.all) : 0.0, upto = carry + wave_upto64(m);
+      const uint64_t over = __ballot(m > 0.0 && upto > target), some = __ballot(m > 0.0);
+      if (over | some) {
+        const int pick = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+        heavy = at + pick;
+        base = __shfl(upto - m, pick, WAVE);
+      }
+      carry = __shfl(upto, WAVE - 1, WAVE);
+      if (over) break;
     }
     token = 0;                                                // no token has any mass
     if (heavy != NONE) {
+      const Weight weight(j.max, j.heat);
       const int lo = heavy * PIECE + tid * EACH;
       const float* row = logits + (int64_t)j.row * vocab;
       const float* qrow = draft_probs != nullptr && j.draft >= 0 ? draft_probs + (int64_t)j.row * vocab : nullptr;
@@ -292,22 +305,22 @@ __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __res
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int x = lo + i;
-        double p = x < vocab ? weight_of(row[x], j.max, j.heat) * j.inv_z : 0.0;
+        double p = x < vocab ? weight(row[x]) * j.inv_z : 0.0;
         if (use && x < vocab) p = qrow != nullptr ? fmax(p - (double)qrow[x], 0.0) : (x == j.draft ? 0.0 : p);
         m[i] = p;
         s += p;
         if (p > 0.0) last = x;
       }
       double sum = base + (block_upto64(s, part) - s);
-      int first = NONE;
+      int found = NONE;
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         sum += m[i];
-        if (m[i] > 0.0 && sum > target) first = min(first, lo + i);
+        if (m[i] > 0.0 && sum > target) found = min(found, lo + i);
       }
-      first = block_min(first, ints);
-      last = -block_min(-last, ints);
-      token = first != NONE ? first : max(last, 0);
+      found = block_min(found, ints);
+      if (found == NONE) last = -block_min(-last, ints);
+      token = found != NONE ? found : max(last, 0);
     }
   }
   for (int i = tid; i <= most; i += THREADS)
@@ -319,7 +332,7 @@ __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __res
 
 extern "C" int64_t holon_verify_drafts_room(int rows, int requests, int vocab) {
   const int64_t pieces = ((int64_t)vocab + PIECE - 1) / PIECE;
-  return rows * pieces * (int64_t)sizeof(RowPart) + requests * (int64_t)sizeof(Judged) + requests * pieces * (int64_t)sizeof(Masses);
+  return (rows * (int64_t)sizeof(RowPart) + requests * (int64_t)sizeof(Masses)) * pieces + requests * (int64_t)sizeof(Judged);
 }
 
 extern "C" int holon_verify_drafts(const float* logits, const int32_t* drafted, const float* draft_probs, const float* accept,

@@ -298,7 +298,7 @@ class TorchKernels:
                 x = torch.where(torch.isnan(x), -torch.inf, x)
                 if heat > 0:
                     z = torch.where(x == x.max(), 0.0, (x - x.max()) / heat)
-                    e = torch.where(x == -torch.inf, 0.0, z.exp())
+                    e = torch.where((x == -torch.inf) | (z * 1.4426950408889634 < -1000), 0.0, z.exp())
                     p = e / e.sum() if e.sum() > 0 else e
                 else:
                     p = torch.nn.functional.one_hot(x.argmax(), vocab).double()
