@@ -43,28 +43,53 @@ struct Masses {
 // goes into the exponent: three additions where rounding, converting and scaling each take four times an addition's cycles.
 // 1 at the largest value, also where that is infinite; nothing below 2^-1000 of it, and nothing for what is no number.
 struct Weight {
-  double c, max64;
-  float max;
+  double c, max64, k[12];
   bool infinite;
-  __device__ __forceinline__ Weight(float max_, double c_) : c(c_), max64(max_), max(max_), infinite(fabsf(max_) == INFINITY) {}
-  __device__ __forceinline__ double operator()(float l) const {
-    constexpr double L = 0.69314718055994530942, MAGIC = 6755399441055744.0;
-    constexpr double C[12] = {1.0, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, L * L * L * L * L / 120, L * L * L * L * L * L / 720,
-                              L * L * L * L * L * L * L / 5040, L * L * L * L * L * L * L * L / 40320, L * L * L * L * L * L * L * L * L / 362880,
-                              L * L * L * L * L * L * L * L * L * L / 3628800, L * L * L * L * L * L * L * L * L * L * L / 39916800};
-    if (infinite) return l == max && max > 0.f ? 1.0 : 0.0;          // (the same for all of a row)
-    const double z = ((double)l - max64) * c, t = z + MAGIC, r = z - (t - MAGIC);      // (exactly 0 at the largest, however small T is)
-    double p = C[11];
+  float max;
+  // (The coefficients come from scalar registers: known to the compiler, each would be moved into the vector register that its
+  // product adds to, two moves a product.)
+  __device__ __forceinline__ Weight(float max_, double c_) : c(c_), max64(max_), infinite(fabsf(max_) == INFINITY), max(max_) {
+    constexpr double L = 0.69314718055994530942;
+    double term = 1.0;
 #pragma unroll
-    for (int k = 10; k >= 0; --k) p = fma(p, r, C[k]);
+    for (int i = 0; i < 12; ++i) {
+      k[i] = term;
+      term *= L / (i + 1);
+      asm("" : "+s"(k[i]));
+    }
+    if (infinite) max64 = 0.0;
+  }
+  // What a row's value counts as: where the largest is infinite, 0 for those that are, and nothing for the others.
+  __device__ __forceinline__ float value(float l) const { return !infinite ? l : l == max && max > 0.f ? 0.f : -INFINITY; }
+  __device__ __forceinline__ double of_value(float l) const {
+    constexpr double MAGIC = 6755399441055744.0;
+    const double z = ((double)l - max64) * c, t = z + MAGIC, r = z - (t - MAGIC);      // (exactly 0 at the largest, however small T is)
+    double p = k[11];
+#pragma unroll
+    for (int i = 10; i >= 0; --i) p = fma(p, r, k[i]);
     const uint64_t bits = __builtin_bit_cast(uint64_t, p);
     const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, t) << 20);
     return z >= -1000.0 ? __builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)bits) : 0.0;
+  }
+  __device__ __forceinline__ double operator()(float l) const { return of_value(value(l)); }
+  template <int N> __device__ __forceinline__ void prepare(float (&x)[N]) const {      // `value` of all, where it changes any
+    if (__any(infinite)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = value(x[i]);
+    }
   }
 };
 
 // The values of piece `lo` that a thread takes: 4 * (tid + 256 j) .. + 3, j < 4, in 16-byte loads where rows allow it.
 __device__ __forceinline__ void load_piece(const float* __restrict__ row, int lo, int vocab, bool wide, float fill, float (&x)[EACH]) {
+  if (wide && lo + PIECE <= vocab) {
+    float4 v[EACH / 4];
+#pragma unroll
+    for (int j = 0; j < EACH / 4; ++j) v[j] = *reinterpret_cast<const float4*>(row + lo + 4 * ((int)threadIdx.x + THREADS * j));
+#pragma unroll
+    for (int j = 0; j < EACH / 4; ++j) { x[4 * j] = v[j].x; x[4 * j + 1] = v[j].y; x[4 * j + 2] = v[j].z; x[4 * j + 3] = v[j].w; }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < EACH / 4; ++j) {
     const int at = lo + 4 * ((int)threadIdx.x + THREADS * j);
@@ -112,39 +137,46 @@ __device__ __forceinline__ double heat_of(float t) { return t > 0.f ? fmax(1.442
 __global__ void __launch_bounds__(THREADS) verify_rows_kernel(const float* __restrict__ logits, const int32_t* __restrict__ start,
                                                               const float* __restrict__ temperature, RowPart* __restrict__ parts,
                                                               int requests, int vocab, int wide) {
-  __shared__ double sums[THREADS / WAVE];
-  __shared__ float tops[THREADS / WAVE];
-  __shared__ int ats[THREADS / WAVE];
+  __shared__ RowPart of_wave[THREADS / WAVE];
   const int piece = blockIdx.x, row = blockIdx.y, lo = piece * PIECE;
   float x[EACH];
   load_piece(logits + (int64_t)row * vocab, lo, vocab, wide, -INFINITY, x);
   const int b = owner_of(start, requests, row);
   if (b < 0) return;                                          // a row behind the last request's (the same for the whole block)
   const double c = heat_of(temperature[b]);
-  float top = -INFINITY;
+  // each wave by itself, under its own largest value: one barrier a block
+  float top = x[0] > -INFINITY ? x[0] : -INFINITY;            // (what is no number is never larger)
+#pragma unroll
+  for (int i = 1; i < EACH; ++i) top = fmaxf(top, x[i]);
+  top = wave_max(top);
   int at = NONE;
-#pragma unroll
-  for (int i = 0; i < EACH; ++i)                              // (a thread's places grow with i; what is no number is never larger)
-    if (x[i] > top) { top = x[i]; at = place_of(lo, i); }
-#pragma unroll
-  for (int o = WAVE / 2; o > 0; o >>= 1) {
-    const float t2 = __shfl_xor(top, o, WAVE);
-    const int a2 = __shfl_xor(at, o, WAVE);
-    if (t2 > top || (t2 == top && a2 < at)) { top = t2; at = a2; }
-  }
-  if (threadIdx.x % WAVE == 0) { tops[threadIdx.x / WAVE] = top; ats[threadIdx.x / WAVE] = at; }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / WAVE; ++w)
-    if (tops[w] > top || (tops[w] == top && ats[w] < at)) { top = tops[w]; at = ats[w]; }
   double s = 0.0;
   if (c > 0.0) {
     const Weight weight(top, c);
+    weight.prepare(x);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) s += weight(x[i]);
-    s = block_sum64(s, sums);
+    for (int i = 0; i < EACH; ++i) s += weight.of_value(x[i]);
+    s = wave_sum64(s);
+  } else {                                                    // T = 0: where the largest stands first
+#pragma unroll
+    for (int i = EACH - 1; i >= 0; --i)
+      if (x[i] == top && top > -INFINITY) at = place_of(lo, i);
+#pragma unroll
+    for (int o = WAVE / 2; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, WAVE));
   }
-  if (threadIdx.x == 0) parts[(int64_t)row * gridDim.x + piece] = RowPart{s, top, at};
+  if (threadIdx.x % WAVE == 0) of_wave[threadIdx.x / WAVE] = RowPart{s, top, at};
+  __syncthreads();
+  if (threadIdx.x < WAVE) {                                   // the four waves' by lanes 0 .. 3, added in that order
+    const RowPart mine = of_wave[threadIdx.x % (THREADS / WAVE)];
+    const float most = lanes_max<THREADS / WAVE>(mine.max);
+    double sum = c > 0.0 ? mine.sum * Weight(most, c)(mine.max) : 0.0;
+    int first = mine.max == most ? mine.at : NONE;
+    sum += lane_xor<1>(sum);
+    sum += lane_xor<2>(sum);
+    first = min(first, lane_xor<1>(first));
+    first = min(first, lane_xor<2>(first));
+    if (threadIdx.x == 0) parts[(int64_t)row * gridDim.x + piece] = RowPart{sum, most, first};
+  }
 }
 
 // One wave: a row's largest value, its first place and its sum of weights from its pieces, added in piece order by lanes and
@@ -243,9 +275,10 @@ __global__ void __launch_bounds__(THREADS) verify_masses_kernel(const float* __r
   load_piece(logits + (int64_t)row * vocab, piece * PIECE, vocab, wide, -INFINITY, x);
   if (by_probs) load_piece(draft_probs + (int64_t)row * vocab, piece * PIECE, vocab, wide, 0.f, q);
   double left = 0.0, all = 0.0;
+  weight.prepare(x);
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const double p = weight(x[i]) * inv_z;
+    const double p = weight.of_value(x[i]) * inv_z;
     all += p;
     left += by_probs ? fmax(p - (double)q[i], 0.0) : (place_of(piece * PIECE, i) == draft ? 0.0 : p);
   }
@@ -300,13 +333,19 @@ __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __res
       const int lo = heavy * PIECE + tid * EACH;
       const float* row = logits + (int64_t)j.row * vocab;
       const float* qrow = draft_probs != nullptr && j.draft >= 0 ? draft_probs + (int64_t)j.row * vocab : nullptr;
+      float v[EACH], q[EACH];
       double m[EACH], s = 0.0;
       int last = -1;
 #pragma unroll
+      for (int i = 0; i < EACH; ++i) v[i] = lo + i < vocab ? row[lo + i] : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) q[i] = qrow != nullptr && lo + i < vocab ? qrow[lo + i] : 0.f;
+      weight.prepare(v);
+#pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int x = lo + i;
-        double p = x < vocab ? weight(row[x]) * j.inv_z : 0.0;
-        if (use && x < vocab) p = qrow != nullptr ? fmax(p - (double)qrow[x], 0.0) : (x == j.draft ? 0.0 : p);
+        double p = weight.of_value(v[i]) * j.inv_z;
+        if (use) p = qrow != nullptr ? fmax(p - (double)q[i], 0.0) : (x == j.draft ? 0.0 : p);
         m[i] = p;
         s += p;
         if (p > 0.0) last = x;
