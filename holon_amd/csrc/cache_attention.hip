@@ -44,6 +44,8 @@ struct CacheArgs {
   int parts, part_first;       // this launch's come from `part_first` on
   int cell_queries;            // > 0: cell (row in row_ids) * cell_queries + query; 0: the token
   int splits;                  // over which waves a row's keys are cut
+  int budget, n_rows;          // budget > 0: blocks a kv head has for its n_rows <= 64 decode rows together, see RowShares;
+  int2* row_parts;             // then [n_rows]: the first of a row's parts, and how many it has
   // rows that share their first tokens: group g is rows group_start[g] .. group_start[g + 1] - 1 and shares group_lens[g] of them
   const int32_t* group_start;
   const int32_t* group_lens;
@@ -59,8 +61,8 @@ __device__ __forceinline__ int page_index(const CacheArgs& a, int pos) { return 
 __device__ __forceinline__ int64_t page_at(const CacheArgs& a, int32_t page) {
   return (int64_t)min((uint32_t)page, (uint32_t)(a.num_pages - 1));
 }
-__device__ __forceinline__ const int32_t* table_row(const CacheArgs& a, int row) {
-  return a.table + (int64_t)min((uint32_t)a.slots[row], (uint32_t)(a.n_slots - 1)) * a.table_stride;
+__device__ __forceinline__ const int32_t* table_at(const CacheArgs& a, int32_t slot) {
+  return a.table + (int64_t)min((uint32_t)slot, (uint32_t)(a.n_slots - 1)) * a.table_stride;
 }
 
 // The keys a row shares with its group (0: it is in none), by the lanes of a wave side by side.
@@ -98,6 +100,35 @@ __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) 
   }
   return j;
 }
+
+// Decode rows of different lengths: as many blocks for each as its keys are of all rows' keys, so that blocks have about the same to
+// do whatever the lengths are. With `units` the blocks of 64 keys that a row sees, a block takes `per` of them and a row
+// ceil(units / per) blocks (one at least), per the least, as far as eight steps find it, for which all rows' blocks are within the
+// budget. Every wave works it out for itself, lane r row r, and has what it needs of the row then.
+struct RowShares {
+  int row, n, slot;            // lane r: row r of the launch
+  int per, blocks, upto;       // a block's units; lane r: row r's blocks, and those of all rows up to it
+  __device__ __forceinline__ explicit RowShares(const CacheArgs& a) {
+    const int r = threadIdx.x % WAVE, here = min(r, a.n_rows - 1);
+    row = a.row_ids == nullptr ? here : a.row_ids[here];
+    n = a.lens[row];
+    slot = a.slots[row];
+    const int units = r < a.n_rows && n > 0 ? (n - 1) / 64 - max(0, first_seen(n - 1, a.window)) / 64 + 1 : 0;
+    const float sum = wave_sum((float)units);              // (whole numbers below 2^24)
+    per = max(1, ((int)sum + a.budget - 1) / a.budget);
+    for (int step = 0; step < 8; ++step) {
+      blocks = r < a.n_rows ? max(1, (units + per - 1) / per) : 0;
+      if (wave_sum((float)blocks) <= (float)a.budget) break;
+      per += 1 + per / 16;
+    }
+    upto = blocks;
+#pragma unroll
+    for (int o = 1; o < WAVE; o *= 2) {
+      const int before = __shfl_up(upto, o, WAVE);
+      if (r >= o) upto += before;
+    }
+  }
+};
 
 // Sixteen codes as 16 bfloat16 values times `power`, in order.
 __device__ __forceinline__ void widen(const u32x4_t& w, float power, bf16x8_t& lo, bf16x8_t& hi) {
@@ -181,9 +212,30 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
   const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, waves = blockDim.x / WAVE;
   const int g = lane / 16, c = lane % 16;
   const int group = a.heads / a.kv_heads, P = a.page_size;
-  const int out_splits = a.splits / waves;
-  const int tile0 = at / out_splits * NT, piece = at % out_splits;
-  const Job job = job_of(a, by_group, ri);
+  const int out_splits = a.budget ? a.budget + a.n_rows : a.splits / waves;
+  const int tile0 = at / out_splits * NT;
+  int piece = at % out_splits, pieces = a.parts, per = 0;
+  const int nth = piece;
+  Job job;
+  int slot = -1;
+  if (a.budget) {
+    const RowShares shares(a);
+    const uint64_t rows_to_go = __ballot(shares.upto > nth);
+    if (rows_to_go == 0) return;                           // (the same for the whole block)
+    ri = __ffsll((unsigned long long)rows_to_go) - 1;
+    pieces = __builtin_amdgcn_readlane(shares.blocks, ri);
+    piece = nth - (__builtin_amdgcn_readlane(shares.upto, ri) - pieces);
+    per = shares.per;
+    job.row = __builtin_amdgcn_readlane(shares.row, ri);
+    job.n = __builtin_amdgcn_readlane(shares.n, ri);
+    slot = __builtin_amdgcn_readlane(shares.slot, ri);
+    job.qs = a.row_ids == nullptr ? job.row : a.qstart[job.row];
+    job.nq = a.row_ids == nullptr ? 1 : a.qstart[job.row + 1] - job.qs;
+    job.from = 0;
+    if (piece == 0 && tile0 == 0 && hk == 0 && threadIdx.x == 0) a.row_parts[ri] = int2{nth, pieces};      // (for the merge)
+  } else {
+    job = job_of(a, by_group, ri);
+  }
   const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
   if (tile0 * 16 >= nq * group || (!by_group && nq > max_query)) return;      // (the same for the whole block)
   Column col[NT];
@@ -195,10 +247,12 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
   const int pos_first = by_group ? n - 1 : n - nq + tile0 * 16 / group;            // the tiles' first and last positions
   const int pos_last = by_group ? n - 1 : n - nq + min((tile0 + NT) * 16 - 1, nq * group - 1) / group;
   const int first = max(from, first_seen(pos_first, a.window)), whole_from = max(from, first_seen(pos_last, a.window));
-  const int base = first / KB * KB;
-  const int share = max(KB, ((pos_last - base + a.splits) / a.splits + KB - 1) / KB * KB);
-  const int key_lo = base + (piece * waves + wave) * share;
-  const int key_hi = min(pos_last, key_lo + share - 1);
+  // a wave's keys: an equal share of the row's, or of its block's
+  const int base = a.budget ? first / 64 * 64 : first / KB * KB;
+  const int share = a.budget ? (per * 64 + waves * KB - 1) / (waves * KB) * KB
+                             : max(KB, ((pos_last - base + a.splits) / a.splits + KB - 1) / KB * KB);
+  const int key_lo = base + (a.budget ? piece * per * 64 + wave * share : (piece * waves + wave) * share);
+  const int key_hi = min(min(pos_last, key_lo + share - 1), a.budget ? base + (piece + 1) * per * 64 - 1 : 0x7fffffff);
   int from_here[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) from_here[t] = max(from, first_seen(col[t].pos, a.window));
@@ -206,7 +260,7 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
   Tiles<D, NT> tl;
   tl.clear();
   if (key_lo <= key_hi) {
-    const int32_t* trow = table_row(a, row);
+    const int32_t* trow = table_at(a, a.budget ? slot : a.slots[row]);
     const int max_page = a.table_stride - 1;
     const int bytes = Q8 ? 1 : 2;
     const int64_t plane = (int64_t)P * D * bytes;
@@ -460,7 +514,7 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (!col[t].valid) continue;
-    if (a.parts == 1) {
+    if (pieces == 1) {
       float l = tl.l[t];
       if (a.sink != nullptr && tl.m[t] != -INFINITY) l += exp2f(a.sink[col[t].head] * 1.4426950408889634f - tl.m[t]);
       const float inv = l == 0.f ? 0.f : 1.0f / l;         // (a NaN stays one)
@@ -471,7 +525,7 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
         for (int r = 0; r < 4; ++r) op[16 * ds + r] = Elem<QT>::store(tl.o[t][ds][r] * inv);
     } else {
       const int64_t place = a.cell_queries > 0 ? (int64_t)ri * a.cell_queries + (col[t].token - qs) : col[t].token;
-      const int64_t cell = (place * a.heads + col[t].head) * a.parts + a.part_first + piece;
+      const int64_t cell = a.budget ? (int64_t)nth * a.heads + col[t].head : (place * a.heads + col[t].head) * a.parts + a.part_first + piece;
       float* po = a.part_o + cell * D + 4 * g;
 #pragma unroll
       for (int ds = 0; ds < D / 16; ++ds) *reinterpret_cast<f32x4_t*>(po + 16 * ds) = tl.o[t][ds];
@@ -703,7 +757,7 @@ __device__ __forceinline__ void tiles_block(const CacheArgs& a, int by_group, in
       if (col.valid) x = *reinterpret_cast<const u32x4_t*>(qp + 16 * ds);
       qf[ds] = __builtin_bit_cast(bf16x8_t, x);
     }
-    const int32_t* trow = table_row(a, row);
+    const int32_t* trow = table_at(a, a.slots[row]);
     // queries of the block see different keys from here on, or up to here
     const int seen_last = first_seen(pos_last, a.window), seen_tile = a.window ? first_seen(tile_first, a.window) : 0;
     const auto differs = [&](int kb) { return kb + 31 > pos_first || kb < seen_last; };
@@ -900,9 +954,17 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
   constexpr int LANES = D / 4;
   const int64_t at = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int d0 = 4 * (threadIdx.x % LANES);
-  if (at >= cells) return;
   const int head = (int)(at % a.heads);
-  int64_t token = at / a.heads, place = token;
+  int64_t token = at / a.heads, place = token, apart = 1;  // its parts lie `apart` cells from one another
+  int parts = a.parts;
+  if (at >= cells) return;
+  if (a.budget) {
+    const int2 mine = a.row_parts[token];
+    parts = mine.y;
+    place = mine.x;
+    apart = a.heads;
+    if (parts <= 1) return;                                // (one block: it has written the result)
+  }
   if (a.cell_queries > 0) {                                // cells by row and query
     const int ri = (int)(token / max_query), qi = (int)(token % max_query);
     const bool in_order = a.row_ids == nullptr;
@@ -912,17 +974,18 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
     token = qs + qi;
   }
   if (token < 0 || token >= a.n_tokens) return;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (place * a.heads + head) * a.parts;
-  const float* po = a.part_o + (place * a.heads + head) * a.parts * D + d0;
+  const int64_t first = a.budget ? place * a.heads + head : (place * a.heads + head) * a.parts;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first;
+  const float* po = a.part_o + first * D + d0;
   float big = -INFINITY;
 #pragma unroll 8
-  for (int i = 0; i < a.parts; ++i) big = fmaxf(big, ml[i].x);
+  for (int i = 0; i < parts; ++i) big = fmaxf(big, ml[i * apart].x);
   float l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int i = 0; i < a.parts; ++i) {
-    const float2 x = ml[i];
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(po + (int64_t)i * D);
+  for (int i = 0; i < parts; ++i) {
+    const float2 x = ml[i * apart];
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(po + i * apart * D);
     const float w = x.y != 0.f ? __builtin_amdgcn_exp2f(x.x - big) : 0.f;      // (a sum of 0: it saw no key, and left nothing else)
     l += x.y != 0.f ? w * x.y : 0.f;
 #pragma unroll
@@ -945,6 +1008,7 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
 struct Cut {
   int splits = 1, waves = 1, two = 0;      // two: two tiles of columns a wave
   int tiles = 0;                           // > 0: the kernel of many columns, so many blocks of them
+  int budget = 0;                          // > 0: blocks a kv head for decode rows by their lengths
   int parts() const { return tiles ? splits : splits / waves; }
 };
 
@@ -971,7 +1035,8 @@ void launch_size(const CacheArgs& a, const Cut& c, int jobs, int by_group, int m
   }
   const int nt = 1 + c.two, tiles = (int)(((int64_t)most * (a.heads / a.kv_heads) + 16 * nt - 1) / (16 * nt));
   const size_t lds = (size_t)(c.waves - 1) * nt * (16 * D + 32) * sizeof(float);
-  const dim3 grid(tiles * (c.splits / c.waves), a.kv_heads, jobs);
+  dim3 grid(tiles * (c.splits / c.waves), a.kv_heads, jobs);
+  if (c.budget) grid = dim3(tiles * (c.budget + jobs), a.kv_heads, 1);
   if constexpr (two_tiles(D, F32)) {
     if (c.two) {
       cache_rows_kernel<D, Q8, QT, 2><<<grid, c.waves * WAVE, lds, s>>>(a, by_group, most);
@@ -1114,7 +1179,13 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
     p.parts = p.shared.parts() + own;
     p.decode_cells = (int64_t)n_tokens * heads * p.parts;
   } else {
-    if (p.any_decode && p.decode.parts() > 1) p.decode_cells = (int64_t)n_decode * heads * p.decode.parts();
+    // Rows of long contexts are cut by their lengths. In equal numbers of shares | by lengths, us in a graph, 32 heads over 8 of 128, 8
+    // bits: 32,768 and seven of 500 keys 40 | 29, 32,768 and fifteen of 500 67 | 31, 16,384 and 47 of 700 83 | 33, eight of 11,000 to 32,768 80 |
+    // 79; all alike, eight of 32,768 109 | 112, 32 of 4,096 51 | 51; where rows are short, 900 to 4,096, 12 | 16.
+    if (p.any_decode && p.decode.parts() > 1 && n_decode > 1 && n_decode <= 64 && seen_span(max_decode_len, 1, window) > 4096)
+      p.decode.budget = p.decode.parts() * n_decode;
+    if (p.any_decode && p.decode.parts() > 1)
+      p.decode_cells = p.decode.budget ? (int64_t)(p.decode.budget + n_decode) * heads : (int64_t)n_decode * heads * p.decode.parts();
     if (p.any_few && p.few.parts() > 1) p.few_cells = (int64_t)n_chunk * few * heads * p.few.parts();
     if (p.any_many && p.many.parts() > 1) p.many_cells = (int64_t)n_chunk * max_chunk_query * heads * p.many.parts();
   }
@@ -1132,7 +1203,7 @@ extern "C" int64_t holon_cache_attention_room(const HolonCacheAttention* call) {
   const HolonCacheAttention& c = *call;
   if (c.kv_heads <= 0 || c.heads < c.kv_heads) return 0;   // (refused by the call that follows)
   const Plan p = plan_of(c);
-  return (p.decode_cells + p.few_cells + p.many_cells) * (c.head_dim + 2) * (int64_t)sizeof(float);
+  return ((p.decode_cells + p.few_cells + p.many_cells) * (c.head_dim + 2) + (p.decode.budget ? 2 * (int64_t)c.n_decode : 0)) * (int64_t)sizeof(float);
 }
 
 extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void* q, void* out, void* room, void* stream) {
@@ -1200,10 +1271,14 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   const auto serve = [&](bool any, const Cut& cut, const int32_t* ids, int n_rows, int most, int less_than, int64_t cells) {
     if (!any) return;
     a.row_ids = ids;
+    a.budget = cut.budget;
+    a.n_rows = n_rows;
     if (!p.by_token) {
       a.parts = cut.parts(); a.cell_queries = most;
       a.part_o = at; a.part_ml = at + cells * head_dim;
       at += cells * (head_dim + 2);
+      a.row_parts = (int2*)at;
+      if (cut.budget) at += 2 * n_rows;
     }
     launch(cut, n_rows, 0, most, less_than);
     if (!p.by_token && a.parts > 1) merge(most, less_than, (int64_t)n_rows * most * heads);

@@ -373,10 +373,95 @@ def test_attention_over_the_8_bit_cache(hip, step, dtype):
 @gpu
 def test_long_contexts_are_cut_and_joined(hip):
     for rows, heads, kv, d, dtype in (([(5000, 1)], 4, 1, 128, torch.bfloat16), ([(9000, 1), (37, 1)], 2, 1, 64, torch.float32),
-                                      ([(6000, 4), (100, 2)], 4, 1, 128, torch.bfloat16), ([(4100, 1)], 2, 1, 256, torch.bfloat16)):
+                                      ([(6000, 4), (100, 2)], 4, 1, 128, torch.bfloat16), ([(4100, 1)], 2, 1, 256, torch.bfloat16),
+                                      # by lengths: one long row among short ones, and rows of no key beside it
+                                      ([(9000, 1)] + [(n, 1) for n in (0, 63, 64, 300, 5000, 7, 1200)], 8, 2, 128, torch.bfloat16),
+                                      ([(4200, 1), (4500, 1), (1, 1)] * 11, 20, 1, 64, torch.bfloat16), ([(4300, 1), (40, 1), (90, 3)], 2, 1, 256, torch.float32)):
         q, pages, scales, table, attn, _ = _step(rows, heads, kv, d, 16, seed=3, dtype=dtype, device="cuda")
         got = hip.paged_attention_q8(q, pages, scales, table, attn, 16, d ** -0.5)
         _check(got, q, pages, scales, table, attn, 16, d ** -0.5)
+        got = hip.paged_attention_q8(q, pages, scales, table, attn, 16, d ** -0.5, 4150)
+        _check(got, q, pages, scales, table, attn, 16, d ** -0.5, 4150)
+
+
+@gpu
+def test_a_call_gives_the_same_bits_again(hip):
+    """Sums have an order that the step's shapes and lengths decide: with other work between, and from another stream."""
+    other = torch.cuda.Stream()
+    for rows, shared, heads, kv, d, q8 in (([(9000, 1), (30, 1), (700, 1)], (), 8, 2, 128, True), ([(300, 1)] * 20, [(0, 19, 288)], 8, 2, 128, False),
+                                           ([(2000, 300), (40, 5)], (), 4, 1, 128, True)):
+        q, pages, scales, table, attn, prefix = _step(rows, heads, kv, d, 16, seed=2, shared=shared, q8=q8, device="cuda")
+        run = lambda: hip.prefix_attention(q, pages, table, attn, prefix, 16, d ** -0.5, scales)             # noqa: E731
+        first = run()
+        torch.randn(1 << 22, device="cuda").sort()
+        assert torch.equal(run(), first)
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            again = run()
+        torch.cuda.current_stream().wait_stream(other)
+        assert torch.equal(again, first)
+
+
+@gpu
+def test_recorded_and_replayed(hip):
+    """Each operation in a graph, replayed on other inputs of the same shapes, with the program's own work between; two graphs do not
+    share what they write."""
+    from holon_amd.kernels.hip import capture
+    steps = [_step([(9000, 1), (30, 1), (700, 1)], 8, 2, 128, 16, seed=s, device="cuda") for s in (1, 2)]
+    groups = [_step([(300, 1)] * 6, 8, 2, 128, 16, seed=s, shared=[(0, 5, 288)], q8=False, device="cuda") for s in (1, 2)]
+    judged = [{k: x.cuda() if torch.is_tensor(x) else x for k, x in _drafts([4, 4, 4], 9000, s).items()} for s in (1, 2)]
+    k, v = torch.randn(40, 2, 128, device="cuda").bfloat16(), torch.randn(40, 2, 128, device="cuda").bfloat16()
+    at = torch.randperm(48)[:40]
+    wp, wo = (at // 16).int().cuda(), (at % 16).int().cuda()
+    pool = lambda: (torch.zeros(4, 2, 2, 2048, dtype=torch.uint8, device="cuda"), torch.ones(4, 2, 2, 16, dtype=torch.uint8, device="cuda"))   # noqa: E731
+
+    def attend(s):
+        q, pages, scales, table, attn, _ = s
+        return hip.paged_attention_q8(q, pages, scales, table, attn, 16, 128 ** -0.5)
+
+    def prefixed(s):
+        q, pages, _, table, attn, prefix = s
+        return hip.prefix_attention(q, pages, table, attn, prefix, 16, 128 ** -0.5)
+
+    def written(kv):
+        pages, scales = pool()
+        hip.kv_write_q8(*kv, pages, scales, wp, wo, 16)
+        return torch.stack(hip.kv_read_q8(pages, scales, wp, wo, 16))
+
+    def tensors(x):
+        if torch.is_tensor(x):
+            return [x]
+        if isinstance(x, dict):
+            return [t for y in x.values() for t in tensors(y)]
+        if isinstance(x, (list, tuple)):
+            return [t for y in x for t in tensors(y)]
+        return tensors(vars(x)) if hasattr(x, "__dict__") else []
+
+    import copy
+    for op, inputs in ((attend, steps), (prefixed, groups), (lambda s: torch.cat([t.flatten() for t in hip.verify_drafts(**s)]), judged),
+                       (written, [(k, v), (v, k)])):
+        want = [op(s).clone() for s in inputs]
+        held = copy.deepcopy(inputs[0])
+        op(held)
+        torch.cuda.synchronize()
+        graphs = []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with capture(graph):
+                out = op(held)
+            graphs.append((graph, out))
+        for turn in (0, 1, 1, 0, 1):
+            for to, src in zip(tensors(held), tensors(inputs[turn]), strict=True):
+                if to.shape == src.shape:
+                    to.copy_(src)
+            assert torch.equal(op(held), want[turn])
+            for graph, _ in graphs:
+                graph.replay()
+            torch.randn(1 << 20, device="cuda").sort()
+            torch.cuda.synchronize()
+            for _, out in graphs:
+                assert torch.equal(out, want[turn]), turn
+            assert torch.equal(op(held), want[turn])
 
 
 @gpu
