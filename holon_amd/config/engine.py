@@ -10,6 +10,7 @@ import dataclasses
 from typing import Any
 
 DTYPES = ("bfloat16", "float32")
+CACHE_FORMATS = ("model", "q8")
 
 
 def _setting(default: object, text: str) -> Any:
@@ -31,6 +32,9 @@ class EngineConfig:
     memory_fraction: float = _setting(0.9, "the share of the GPU memory still free once the weights are loaded that steps and the cache may use")
     state_memory: int | None = _setting(None, "the cache's size in bytes, instead of deriving it from memory_fraction")
     cache_tokens: int | None = _setting(None, "tokens of paged state per pool (overrides state_memory)")
+    cache_format: str = _setting("model", "what attention keeps keys and values in: model (the engine's dtype), or q8 (8-bit codes "
+                                          "and a power of two a token and head: half of bfloat16's bytes; architectures of "
+                                          "grouped-query attention, heads of 64, 128 or 256, pages of a multiple of 16)")
     prefix_cache: bool = _setting(True, "let a request start from the pages of an earlier request with the same first tokens")
     overlap: bool = _setting(True, "schedule and launch the next step while the last one runs")
     graphs: bool = _setting(True, "replay decode steps from HIP graphs, per batch-size bucket")
@@ -52,6 +56,8 @@ class EngineConfig:
                              "chunk_with_decode, 1 for the others)")
         if self.dtype not in DTYPES:
             raise ValueError(f"EngineConfig.dtype must be one of {DTYPES}, got {self.dtype!r}")
+        if self.cache_format not in CACHE_FORMATS:
+            raise ValueError(f"EngineConfig.cache_format must be one of {CACHE_FORMATS}, got {self.cache_format!r}")
         if self.chunk_with_decode and self.max_step_tokens < self.max_seqs + self.chunk_with_decode:
             raise ValueError("mixed steps need max_step_tokens >= max_seqs + chunk_with_decode")
         from .products import MODES, check_pins

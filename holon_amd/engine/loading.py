@@ -53,11 +53,17 @@ class Loaded:
 
 
 def build_from_spec(spec: ModelSpec, *, device: torch.device, dtype: torch.dtype, kernels, page_size: int,
-                    max_seqs: int, max_model_len: int, max_step_tokens: int, decode_copy: bool = True
-                    ) -> tuple[Model, Build]:
+                    max_seqs: int, max_model_len: int, max_step_tokens: int, decode_copy: bool = True,
+                    cache_format: str = "model") -> tuple[Model, Build]:
     build = Build(kernels=kernels, device=device, dtype=dtype, page_size=page_size, max_model_len=max_model_len,
-                  max_seqs=max_seqs, max_step_tokens=max_step_tokens, decode_copy=decode_copy)
-    return build_model(spec, build), build
+                  max_seqs=max_seqs, max_step_tokens=max_step_tokens, decode_copy=decode_copy,
+                  cache_format=cache_format)
+    model = build_model(spec, build)
+    if cache_format == "q8":
+        others = sorted({d.name for decls in model.state_decls() for d in decls if hasattr(d, "elems") and d.dtype is not torch.uint8})
+        if others:
+            raise ValueError(f"cache_format q8 is served by grouped-query attention alone: this model also keeps {', '.join(others)}")
+    return model, build
 
 
 def attach_cache(model: Model, *, device: torch.device, dtype: torch.dtype, kernels, page_size: int, max_seqs: int,
@@ -100,7 +106,8 @@ def assemble(cfg: EngineConfig, kernels=None, *, random_config: dict | None = No
     model_config, spec = resolve(config_json, generation)
     model, _ = build_from_spec(spec, device=device, dtype=dtype, kernels=kernels, page_size=cfg.page_size,
                                max_seqs=cfg.max_seqs, max_model_len=cfg.max_model_len,
-                               max_step_tokens=cfg.max_step_tokens, decode_copy=cfg.decode_weight_copy)
+                               max_step_tokens=cfg.max_step_tokens, decode_copy=cfg.decode_weight_copy,
+                               cache_format=cfg.cache_format)
     if configured is not None:
         kernels.settled = any(part.amplifies for part in model.walk())
     if random_config is not None:
@@ -158,13 +165,13 @@ def load_model(folder: str | pathlib.Path, *, device: str | torch.device = "cuda
                kernels=None, page_size: int = 16, max_seqs: int = 64, max_model_len: int = 8192,
                max_step_tokens: int = 4096, cache_tokens: int | None = None, graphs: bool = False,
                products: str = "own", product_pins: dict | None = None, decode_weight_copy: bool = True,
-               random_config: dict | None = None, seed: int = 0) -> Loaded:
+               random_config: dict | None = None, seed: int = 0, cache_format: str = "model") -> Loaded:
     """Read config.json, pick the model by its architecture name, load the weights, allocate the cache. With
     `random_config` (a config.json as a dict) no folder is read: the weights are drawn on the device from `seed`."""
     dtype_name = dtype if isinstance(dtype, str) else {v: k for k, v in TORCH_DTYPES.items()}[torch_dtype(dtype)]
     cfg = EngineConfig(model=str(folder), device=str(device), dtype=dtype_name, page_size=page_size, max_seqs=max_seqs,
                        max_model_len=max_model_len, max_step_tokens=max_step_tokens, graphs=graphs, products=products,
-                       product_pins=product_pins, decode_weight_copy=decode_weight_copy)
+                       product_pins=product_pins, decode_weight_copy=decode_weight_copy, cache_format=cache_format)
     a = assemble(cfg, kernels, random_config=random_config, seed=seed)
     tokens = cache_tokens if cache_tokens is not None else max_model_len
     cache, runner = attach_cache(a.model, cache_tokens=tokens, graphs=graphs, **a.shape(cfg))

@@ -102,6 +102,7 @@ class Build:
     max_seqs: int = 64
     max_step_tokens: int = 4096
     decode_copy: bool = True                      # keep a second, tiled copy of every projection for decode steps
+    cache_format: str = "model"                   # what attention keeps keys and values in (EngineConfig.cache_format)
 
     def make(self, ref: PartRef, **site: Any) -> "Part":
         return part_class(ref)(self, **ref.get(), **site)

@@ -18,7 +18,10 @@ class GQA(Part):
     position encoding on q and k, keys and values written to the cache, causal attention over the cache (optionally
     within a window), output projection. `heads * head_dim` need not equal `hidden`.
 
-    A run that reads another run's cache (`site.writes` false) projects and encodes queries only."""
+    A run that reads another run's cache (`site.writes` false) projects and encodes queries only.
+
+    With `cache_format` "q8" keys and values lie in an 8-bit cache (`Kernels.kv_write_q8`): a page is its codes and then
+    its scales, and the operations run one after the other."""
 
     graph_safe = True
 
@@ -29,7 +32,11 @@ class GQA(Part):
         if heads % kv_heads:
             raise ValueError(f"gqa: {heads} heads are not a multiple of {kv_heads} kv heads")
         if build.kernels is not None:             # a size no attention kernel serves is refused now, not at the first step
-            build.kernels.check_attention(head_dim, build.page_size, build.dtype)
+            if build.cache_format == "q8":
+                build.kernels.check_cache_q8(head_dim, build.page_size)
+            else:
+                build.kernels.check_attention(head_dim, build.page_size, build.dtype)
+        self.q8 = build.cache_format == "q8"
         self.heads, self.kv_heads, self.head_dim, self.hidden, self.layer = heads, kv_heads, head_dim, hidden, layer
         self.window = int(window)
         self.scale = float(scale) if scale is not None else head_dim ** -0.5
@@ -48,6 +55,8 @@ class GQA(Part):
         self._fused: dict | None = None
 
     def state(self) -> list[PagedState]:
+        if self.q8:                               # a byte a value and one a (token, head)
+            return [PagedState("kv", elems=2 * self.kv_heads * (self.head_dim + 1), window=self.window, dtype=torch.uint8)]
         return [PagedState("kv", elems=2 * self.kv_heads * self.head_dim, window=self.window)]
 
     def finalize(self) -> None:
@@ -72,9 +81,14 @@ class GQA(Part):
         k = self.kernels
         t, hq, hkv, d = x.shape[0], self.heads, self.kv_heads, self.head_dim
         view = step.paged[site.group]
-        pages = site.pages.view(-1, 2, hkv, view.page_size * d)
+        if self.q8:
+            codes = 2 * hkv * view.page_size * d
+            pages = site.pages[:, :codes].view(-1, 2, hkv, view.page_size * d)
+            scales = site.pages[:, codes:].view(-1, 2, hkv, view.page_size)
+        else:
+            pages = site.pages.view(-1, 2, hkv, view.page_size * d)
         qkv = self.qkv(x)
-        if self._fused is not None:
+        if self._fused is not None and not self.q8:
             out = k.qkv_attention(
                 qkv, hq, hkv, d, self.q_norm.weight if self.q_norm is not None else None,
                 self.k_norm.weight if self.k_norm is not None else None, self._fused["eps"], self._fused["table"],
@@ -91,8 +105,14 @@ class GQA(Part):
                 self.position.apply(q, kk, step.positions)
             if site.writes:
                 v = qkv[:, (hq + hkv) * d:].contiguous().view(t, hkv, d)
-                k.kv_write(kk, v, pages, view.write_page, view.write_off, view.page_size)
-        out = k.paged_attention(q, pages, view.table, step.rows, view.page_size, self.scale, self.window)
+                if self.q8:
+                    k.kv_write_q8(kk, v, pages, scales, view.write_page, view.write_off, view.page_size)
+                else:
+                    k.kv_write(kk, v, pages, view.write_page, view.write_off, view.page_size)
+        if self.q8:
+            out = k.paged_attention_q8(q, pages, scales, view.table, step.rows, view.page_size, self.scale, self.window)
+        else:
+            out = k.paged_attention(q, pages, view.table, step.rows, view.page_size, self.scale, self.window)
         return self.o_proj(out.view(t, hq * d), residual=residual)
 
     __call__ = forward
