@@ -6,20 +6,33 @@ namespace {
 
 constexpr int RUN = 16;      // tokens a block takes of one head: a run of 16 tokens of a page is 16 bytes of every dim's values
 
-// The place of token t0 + i (i < 16) by lane i of each row of 16 lanes, as page * page_size + offset; -1: none (or no such token).
-__device__ __forceinline__ int64_t place_of(const int32_t* __restrict__ page, const int32_t* __restrict__ off, int t, int tokens,
-                                            int page_size, int num_pages) {
-  if (t >= tokens) return -1;
+// The place of a token; page -1: none, or no such token.
+struct Place {
+  int page, off;
+};
+__device__ __forceinline__ Place place_of(const int32_t* __restrict__ page, const int32_t* __restrict__ off, int t, int tokens,
+                                          int page_size, int num_pages) {
+  if (t >= tokens) return Place{-1, 0};
   const int pg = page[t], at = off[t];
-  return pg >= 0 && pg < num_pages && at >= 0 && at < page_size ? (int64_t)pg * page_size + at : -1;
+  return pg >= 0 && pg < num_pages && at >= 0 && at < page_size ? Place{pg, at} : Place{-1, 0};
 }
-// Whether 16 places are a run: one after the other from a border of 16 on (pages are multiples of 16, so they share one).
-__device__ __forceinline__ bool is_run(const int64_t* places) {
-  bool run = places[0] >= 0 && places[0] % RUN == 0;
-#pragma unroll
-  for (int i = 1; i < RUN; ++i) run &= places[i] == places[0] + i;
-  return run;
-}
+// Sixteen tokens in two stretches at most, each of neighbours within 16 bytes of every dim's values: tokens 0 .. first - 1, and from
+// there to count - 1; no token behind those has a place. A portion of a sequence is that wherever it begins (16 tokens from an odd
+// place on lie on both sides of one border), and so are most ends of one sequence and beginnings of the next. `any` is false of others.
+struct Stretches {
+  bool any;
+  int first, count;
+  // By every wave for itself, from the places in LDS.
+  __device__ __forceinline__ explicit Stretches(const Place* places) {
+    const int lane = threadIdx.x % RUN;
+    const Place mine = places[lane], before = places[max(lane - 1, 0)];
+    const bool goes_on = mine.page == before.page && mine.off == before.off + 1 && mine.off % RUN != 0;
+    const uint32_t there = (uint32_t)__ballot(mine.page >= 0) & 0xffffu, breaks = (uint32_t)__ballot(lane > 0 && !goes_on) & there;
+    any = (there & (there + 1)) == 0 && (breaks & (breaks - 1)) == 0;
+    count = __popc(there);
+    first = breaks ? __ffs(breaks) - 1 : count;
+  }
+};
 
 template <typename T, int N>
 __device__ __forceinline__ void load_values(const T* x, bool wide, float (&f)[N]) {
@@ -43,8 +56,34 @@ __device__ __forceinline__ void load_values(const T* x, bool wide, float (&f)[N]
   }
 }
 
+// Bytes lo .. hi - 1 of 16, in the widest pieces that lie on borders of their own width.
+__device__ __forceinline__ void store_bytes(uint8_t* to, const uint8_t* from, int lo, int hi) {
+  if (hi - lo == RUN) {
+    *reinterpret_cast<q8x4_t*>(to) = *reinterpret_cast<const q8x4_t*>(from);
+    return;
+  }
+  while (lo < hi) {
+    if (lo % 8 == 0 && lo + 8 <= hi) {
+      *reinterpret_cast<uint64_t*>(to + lo) = *reinterpret_cast<const uint64_t*>(from + lo);
+      lo += 8;
+    } else if (lo % 4 == 0 && lo + 4 <= hi) {
+      *reinterpret_cast<uint32_t*>(to + lo) = *reinterpret_cast<const uint32_t*>(from + lo);
+      lo += 4;
+    } else if (lo % 2 == 0 && lo + 2 <= hi) {
+      *reinterpret_cast<uint16_t*>(to + lo) = *reinterpret_cast<const uint16_t*>(from + lo);
+      lo += 2;
+    } else {
+      to[lo] = from[lo];
+      lo += 1;
+    }
+  }
+}
+
 // A block takes 16 tokens of one head: 16 lanes a token, D / 16 values of its key and of its value a lane. Values go through LDS
-// where their tokens are a run, so that 16 bytes of a dim are written at once; tokens anywhere else have theirs written one by one.
+// where their tokens lie in two stretches, so that what a stretch has of a dim's 16 bytes is written at once; tokens anywhere else
+// have theirs written one by one. Memory bounds it: 8 heads of 128 in bfloat16, 4,096 tokens from a page's begin on (25 MB) 9.0 us a
+// call, from its sixth place on 10.6, anywhere 27; 32,768 tokens 46, 54 and 169 (4.4, 3.7 and 1.2 TB/s). With one stretch alone, a byte
+// at a time from the sixth place on, the second of these took 14.9 and 87. Below some 1,000 tokens the host's 8 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t stride, int wide,
                                                           uint8_t* __restrict__ pages, uint8_t* __restrict__ scales,
@@ -53,10 +92,10 @@ __global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ 
                                                           const int32_t* __restrict__ write_off, int tokens, int kv_heads,
                                                           int page_size, int num_pages) {
   constexpr int E = D / 16;                                // values a lane
-  __shared__ int64_t places[RUN];
-  __shared__ __attribute__((aligned(16))) uint8_t turned[D][RUN];
+  __shared__ Place places[RUN];
+  __shared__ __attribute__((aligned(16))) uint8_t turned[2][D][RUN];
   const int t0 = blockIdx.x * RUN, hk = blockIdx.y, i = threadIdx.x / 16, lane = threadIdx.x % 16, t = t0 + i;
-  const int64_t place = place_of(write_page, write_off, t, tokens, page_size, num_pages);
+  const Place place = place_of(write_page, write_off, t, tokens, page_size, num_pages);
   if (lane == 0) places[i] = place;
   float x[2][E];
   if (t < tokens) {
@@ -80,24 +119,29 @@ __global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ 
       codes[part][e / 4] = q8_codes(x[part][e] * inverse, x[part][e + 1] * inverse, x[part][e + 2] * inverse, x[part][e + 3] * inverse);
   }
   __syncthreads();
-  const bool run = is_run(places);
-  const int64_t plane = (int64_t)page_size * D, page = place >= 0 ? place / page_size : 0;
-  const int off = place >= 0 ? (int)(place % page_size) : 0;
-  if (place >= 0) {
-    uint32_t* to = reinterpret_cast<uint32_t*>(pages + page * page_stride + hk * plane + (int64_t)off * D + lane * E);
+  const Stretches two(places);
+  const int64_t plane = (int64_t)page_size * D;
+  if (place.page >= 0) {
+    uint32_t* to = reinterpret_cast<uint32_t*>(pages + place.page * page_stride + hk * plane + (int64_t)place.off * D + lane * E);
 #pragma unroll
     for (int e = 0; e < E / 4; ++e) to[e] = codes[0][e];
-    if (lane < 2) scales[page * scale_stride + ((int64_t)lane * kv_heads + hk) * page_size + off] = (uint8_t)(lane ? byte[1] : byte[0]);
+    if (lane < 2) scales[place.page * scale_stride + ((int64_t)lane * kv_heads + hk) * page_size + place.off] = (uint8_t)(lane ? byte[1] : byte[0]);
   }
-  if (run) {
+  if (two.any) {
+    if (place.page >= 0) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) turned[lane * E + e][i] = (uint8_t)(codes[1][e / 4] >> (8 * (e % 4)));
+      for (int e = 0; e < E; ++e) turned[i >= two.first][lane * E + e][place.off % RUN] = (uint8_t)(codes[1][e / 4] >> (8 * (e % 4)));
+    }
     __syncthreads();
-    uint8_t* to = pages + page * page_stride + (kv_heads + hk) * plane + places[0] % page_size;
-    for (int d = threadIdx.x; d < D; d += 256)
-      *reinterpret_cast<q8x4_t*>(to + (int64_t)d * page_size) = *reinterpret_cast<const q8x4_t*>(turned[d]);
-  } else if (place >= 0) {
-    uint8_t* to = pages + page * page_stride + (kv_heads + hk) * plane + off;
+    for (int at = threadIdx.x; at < 2 * D; at += 256) {
+      const int x = at / D, d = at % D, from = x ? two.first : 0, n = (x ? two.count : two.first) - from;
+      if (n <= 0) break;
+      const Place begin = places[from];
+      const int lo = begin.off % RUN;
+      store_bytes(pages + begin.page * page_stride + (kv_heads + hk) * plane + (int64_t)d * page_size + begin.off - lo, turned[x][d], lo, lo + n);
+    }
+  } else if (place.page >= 0) {
+    uint8_t* to = pages + place.page * page_stride + (kv_heads + hk) * plane + place.off;
 #pragma unroll
     for (int e = 0; e < E; ++e) to[(int64_t)(lane * E + e) * page_size] = (uint8_t)(codes[1][e / 4] >> (8 * (e % 4)));
   }
@@ -120,7 +164,9 @@ __device__ __forceinline__ void store4(T* to, const float (&f)[4]) {
   }
 }
 
-// The same blocks the other way round: 16 lanes a token, D / 16 of its codes a lane.
+// The same blocks the other way round: 16 lanes a token, D / 16 of its codes a lane. Two thirds of what it moves are the values it
+// writes: 32,768 tokens of 8 heads of 128 into bfloat16 (202 MB) 36 us from a page's begin on, 40 from its sixth place on, 84 anywhere;
+// into 32 bits (336 MB) 92, 97 and 147.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_read_q8_kernel(T* __restrict__ k, T* __restrict__ v, const uint8_t* __restrict__ pages,
                                                          const uint8_t* __restrict__ scales, int64_t page_stride,
@@ -128,13 +174,14 @@ __global__ void __launch_bounds__(256) kv_read_q8_kernel(T* __restrict__ k, T* _
                                                          const int32_t* __restrict__ read_off, int tokens, int kv_heads,
                                                          int page_size, int num_pages) {
   constexpr int E = D / 16;
-  __shared__ int64_t places[RUN];
-  __shared__ __attribute__((aligned(16))) uint8_t turned[RUN][D + 16];
+  __shared__ Place places[RUN];
+  __shared__ __attribute__((aligned(16))) uint8_t turned[2][RUN][D + 16];
   const int t0 = blockIdx.x * RUN, hk = blockIdx.y, i = threadIdx.x / 16, lane = threadIdx.x % 16, t = t0 + i;
-  const int64_t place = place_of(read_page, read_off, t, tokens, page_size, num_pages);
+  const Place place = place_of(read_page, read_off, t, tokens, page_size, num_pages);
   if (lane == 0) places[i] = place;
-  const int64_t plane = (int64_t)page_size * D, page = place >= 0 ? place / page_size : 0;
-  const int off = place >= 0 ? (int)(place % page_size) : 0;
+  const bool there = place.page >= 0;
+  const int64_t plane = (int64_t)page_size * D, page = there ? place.page : 0;
+  const int off = place.off;
   const uint8_t* from = pages + page * page_stride + hk * plane;
   const uint8_t* powers = scales + page * scale_stride + (int64_t)hk * page_size + off;
   uint32_t codes[2][E / 4];
@@ -143,15 +190,20 @@ __global__ void __launch_bounds__(256) kv_read_q8_kernel(T* __restrict__ k, T* _
   for (int e = 0; e < E / 4; ++e) codes[0][e] = *reinterpret_cast<const uint32_t*>(from + (int64_t)off * D + lane * E + 4 * e);
   from += kv_heads * plane;
   __syncthreads();
-  if (is_run(places)) {
-    for (int d = threadIdx.x; d < D; d += 256) {
-      const q8x4_t w = *reinterpret_cast<const q8x4_t*>(from + (int64_t)d * page_size + places[0] % page_size);
+  const Stretches two(places);
+  if (two.any) {
+    for (int at = threadIdx.x; at < 2 * D; at += 256) {    // (all 16 bytes of a dim, also where the stretch has some of them alone)
+      const int x = at / D, d = at % D, start = x ? two.first : 0;
+      if ((x ? two.count : two.first) <= start) break;
+      const Place begin = places[start];
+      const q8x4_t w = *reinterpret_cast<const q8x4_t*>(pages + begin.page * page_stride + (kv_heads + hk) * plane + (int64_t)d * page_size +
+                                                        begin.off / RUN * RUN);
 #pragma unroll
-      for (int r = 0; r < RUN; ++r) turned[r][d] = (uint8_t)(w[r / 4] >> (8 * (r % 4)));
+      for (int r = 0; r < RUN; ++r) turned[x][r][d] = (uint8_t)(w[r / 4] >> (8 * (r % 4)));
     }
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E / 4; ++e) codes[1][e] = *reinterpret_cast<const uint32_t*>(&turned[i][lane * E + 4 * e]);
+    for (int e = 0; e < E / 4; ++e) codes[1][e] = *reinterpret_cast<const uint32_t*>(&turned[i >= two.first][off % RUN][lane * E + 4 * e]);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -160,7 +212,6 @@ __global__ void __launch_bounds__(256) kv_read_q8_kernel(T* __restrict__ k, T* _
     }
   }
   if (t >= tokens) return;
-  const bool there = place >= 0;
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     T* to = (part ? v : k) + ((int64_t)t * kv_heads + hk) * D + lane * E;

@@ -356,6 +356,35 @@ def test_write_and_read_back(hip, t, kv, d, page, gap, dtype):
 
 
 @gpu
+@pytest.mark.parametrize(("d", "page"), [(64, 16), (128, 48), (256, 32)])
+@pytest.mark.parametrize("holes", [0.0, 0.02])
+def test_stretches_that_begin_and_end_anywhere(hip, d, page, holes):
+    """Portions of every length up to 35 from every place of a page on, one behind the other: however a stretch of neighbours meets
+    the blocks' borders and those of 16 tokens, exactly its bytes are written, and the same come back."""
+    rng = np.random.default_rng(d)
+    portions = [(first, n) for first in range(page) for n in rng.permutation(np.arange(1, 36))[:12]]
+    n = sum(-(-(first + more) // page) for first, more in portions)
+    order, at, wp, wo = rng.permutation(n), 0, [], []
+    for first, more in portions:
+        place = at * page + first + np.arange(more)
+        wp.append(order[place // page])
+        wo.append(place % page)
+        at += -(-(first + more) // page)
+    wp, wo = np.concatenate(wp), np.concatenate(wo)
+    wp[rng.random(len(wp)) < holes] = -1
+    wp, wo = (torch.as_tensor(x.astype(np.int32)) for x in (wp, wo))
+    k, v = torch.randn(2, len(wp), 2, d, generator=torch.Generator().manual_seed(d))
+    both, views = _blank(n, 2, page, d, d)
+    want, got = both.clone(), both.cuda()
+    PLAIN.kv_write_q8(k, v, *views(want), wp, wo, page)
+    hip.kv_write_q8(k.cuda(), v.cuda(), *views(got), wp.cuda(), wo.cuda(), page)
+    assert torch.equal(got.cpu(), want)
+    for x, y in zip(hip.kv_read_q8(*views(got), wp.cuda(), wo.cuda(), page, torch.float32),
+                    PLAIN.kv_read_q8(*views(want), wp, wo, page, torch.float32)):
+        assert torch.equal(x.cpu(), y)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("step", range(len(STEPS)))
 def test_attention_over_the_8_bit_cache(hip, step, dtype):
