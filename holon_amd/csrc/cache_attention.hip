@@ -114,8 +114,8 @@ struct RowShares {
     n = a.lens[row];
     slot = a.slots[row];
     const int units = r < a.n_rows && n > 0 ? (n - 1) / 64 - max(0, first_seen(n - 1, a.window)) / 64 + 1 : 0;
-    const float sum = wave_sum((float)units);              // (whole numbers below 2^24)
-    per = max(1, ((int)sum + a.budget - 1) / a.budget);
+    // (A sum past 2^24 is rounded; one step makes `per` large enough then: never more than budget + n_rows blocks, the launch's.)
+    per = max(1, (int)ceilf(wave_sum((float)units) / (float)a.budget));
     for (int step = 0; step < 8; ++step) {
       blocks = r < a.n_rows ? max(1, (units + per - 1) / per) : 0;
       if (wave_sum((float)blocks) <= (float)a.budget) break;

@@ -79,33 +79,38 @@ __device__ __forceinline__ void store_bytes(uint8_t* to, const uint8_t* from, in
   }
 }
 
-// A block takes 16 tokens of one head: 16 lanes a token, D / 16 values of its key and of its value a lane. Values go through LDS
-// where their tokens lie in two stretches, so that what a stretch has of a dim's 16 bytes is written at once; tokens anywhere else
-// have theirs written one by one. Memory bounds it: 8 heads of 128 in bfloat16, 4,096 tokens from a page's begin on (25 MB) 9.0 us a
-// call, from its sixth place on 10.6, anywhere 27; 32,768 tokens 46, 54 and 169 (4.4, 3.7 and 1.2 TB/s). With one stretch alone, a byte
-// at a time from the sixth place on, the second of these took 14.9 and 87. Below some 1,000 tokens the host's 8 us.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t stride, int wide,
-                                                          uint8_t* __restrict__ pages, uint8_t* __restrict__ scales,
-                                                          int64_t page_stride, int64_t scale_stride,
-                                                          const int32_t* __restrict__ write_page,
-                                                          const int32_t* __restrict__ write_off, int tokens, int kv_heads,
-                                                          int page_size, int num_pages) {
-  constexpr int E = D / 16;                                // values a lane
-  __shared__ Place places[RUN];
-  __shared__ __attribute__((aligned(16))) uint8_t turned[2][D][RUN];
-  const int t0 = blockIdx.x * RUN, hk = blockIdx.y, i = threadIdx.x / 16, lane = threadIdx.x % 16, t = t0 + i;
-  const Place place = place_of(write_page, write_off, t, tokens, page_size, num_pages);
-  if (lane == 0) places[i] = place;
-  float x[2][E];
-  if (t < tokens) {
-    const int64_t at = (int64_t)t * stride + (int64_t)hk * D + lane * E;
-    load_values<T, E>(k + at, wide, x[0]);
-    load_values<T, E>(v + at, wide, x[1]);
+template <typename T>
+__device__ __forceinline__ void store4(T* to, const float (&f)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(to) = float4{f[0], f[1], f[2], f[3]};
   } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[0][e] = x[1][e] = 0.f;
+    ushort4 w;
+    w.x = float_to_bf16(f[0]); w.y = float_to_bf16(f[1]); w.z = float_to_bf16(f[2]); w.w = float_to_bf16(f[3]);
+    *reinterpret_cast<ushort4*>(to) = w;
   }
+}
+
+// Where a block's 16 tokens go.
+struct Target {
+  uint8_t* pages;
+  uint8_t* scales;
+  int64_t page_stride, scale_stride;
+  const int32_t* page;         // [tokens]
+  const int32_t* off;
+  int tokens, kv_heads, page_size, num_pages;
+};
+
+// A block's 16 tokens of head hk into the cache: thread 16 i + lane has values D / 16 lane .. of token t0 + i, x[0] of its key and
+// x[1] of its value.
+template <int D>
+__device__ __forceinline__ void write_block(const Target& w, int hk, const Place& place, Place* places, const float (&x)[2][D / 16]) {
+  constexpr int E = D / 16;
+  __shared__ __attribute__((aligned(16))) uint8_t turned[2][D][RUN];
+  const int i = threadIdx.x / 16, lane = threadIdx.x % 16;
+  uint8_t* const pages = w.pages;
+  const int64_t page_stride = w.page_stride, scale_stride = w.scale_stride;
+  const int kv_heads = w.kv_heads, page_size = w.page_size;
+  if (lane == 0) places[i] = place;
   uint32_t codes[2][E / 4], byte[2];
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ 
     uint32_t* to = reinterpret_cast<uint32_t*>(pages + place.page * page_stride + hk * plane + (int64_t)place.off * D + lane * E);
 #pragma unroll
     for (int e = 0; e < E / 4; ++e) to[e] = codes[0][e];
-    if (lane < 2) scales[place.page * scale_stride + ((int64_t)lane * kv_heads + hk) * page_size + place.off] = (uint8_t)(lane ? byte[1] : byte[0]);
+    if (lane < 2) w.scales[place.page * scale_stride + ((int64_t)lane * kv_heads + hk) * page_size + place.off] = (uint8_t)(lane ? byte[1] : byte[0]);
   }
   if (two.any) {
     if (place.page >= 0) {
@@ -147,23 +152,89 @@ __global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ 
   }
 }
 
+// A block takes 16 tokens of one head: 16 lanes a token, D / 16 values of its key and of its value a lane. Values go through LDS
+// where their tokens lie in two stretches, so that what a stretch has of a dim's 16 bytes is written at once; tokens anywhere else
+// have theirs written one by one. Memory bounds it: 8 heads of 128 in bfloat16, 4,096 tokens from a page's begin on (25 MB) 9.0 us a
+// call, from its sixth place on 10.6, anywhere 27; 32,768 tokens 46, 54 and 169 (4.4, 3.7 and 1.2 TB/s). With one stretch alone, a byte
+// at a time from the sixth place on, the second of these took 14.9 and 87. Below some 1,000 tokens the host's 8 us.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t stride, int wide, Target w) {
+  constexpr int E = D / 16;
+  __shared__ Place places[RUN];
+  const int hk = blockIdx.y, lane = threadIdx.x % 16, t = blockIdx.x * RUN + threadIdx.x / 16;
+  const Place place = place_of(w.page, w.off, t, w.tokens, w.page_size, w.num_pages);
+  float x[2][E];
+  if (t < w.tokens) {
+    const int64_t at = (int64_t)t * stride + (int64_t)hk * D + lane * E;
+    load_values<T, E>(k + at, wide, x[0]);
+    load_values<T, E>(v + at, wide, x[1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[0][e] = x[1][e] = 0.f;
+  }
+  write_block<D>(w, hk, place, places, x);
+}
+
+// The merged projection's heads: queries and keys normed and turned, queries to q_out, keys and values into the cache. A block takes
+// 16 tokens of one kv head, or of one query head; a value's partner in the rotation is eight lanes away.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) qk_norm_rope_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, int heads,
+                                                                    const T* __restrict__ q_weight, const T* __restrict__ k_weight,
+                                                                    int wide_weights, float eps, const float* __restrict__ table,
+                                                                    int max_positions, const int32_t* __restrict__ positions, Target w) {
+  constexpr int E = D / 16;
+  __shared__ Place places[RUN];
+  const int lane = threadIdx.x % 16, t = blockIdx.x * RUN + threadIdx.x / 16, row = min(t, w.tokens - 1);
+  const bool is_q = (int)blockIdx.y >= w.kv_heads;
+  const int head = is_q ? blockIdx.y - w.kv_heads : blockIdx.y;
+  // all that a block reads is asked for before anything waits, the longest chain first
+  const int pos = table != nullptr ? min(max(positions[row], 0), max_positions - 1) : 0;
+  Place place = {-1, 0};
+  if (!is_q) place = place_of(w.page, w.off, t, w.tokens, w.page_size, w.num_pages);
+  const T* src = qkv + (int64_t)row * (heads + 2 * w.kv_heads) * D + lane * E;
+  float x[2][E], weight[E], co[E], si[E];
+  load_values<T, E>(src + (int64_t)(is_q ? head : heads + head) * D, true, x[0]);
+  if (!is_q) load_values<T, E>(src + (int64_t)(heads + w.kv_heads + head) * D, true, x[1]);
+  const bool norm = q_weight != nullptr;
+  if (norm) load_values<T, E>((is_q ? q_weight : k_weight) + lane * E, wide_weights, weight);
+  if (table != nullptr) {
+    const float* cs = table + (int64_t)pos * D + lane % 8 * E;
+    load_values<float, E>(cs, true, co);
+    load_values<float, E>(cs + D / 2, true, si);
+  }
+  if (norm) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += x[0][e] * x[0][e];
+    const float inv = 1.0f / sqrtf(lanes_sum<16>(sum) / (float)D + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[0][e] = Elem<T>::round((x[0][e] * inv) * weight[e]);
+  }
+  if (table != nullptr) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float other = lane_xor<8>(x[0][e]);
+      x[0][e] = Elem<T>::round(lane < 8 ? x[0][e] * co[e] - other * si[e] : x[0][e] * co[e] + other * si[e]);
+    }
+  }
+  if (!is_q) {
+    write_block<D>(w, head, place, places, x);
+  } else if (t < w.tokens) {
+    T* to = q_out + ((int64_t)t * heads + head) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float four[4] = {x[0][e], x[0][e + 1], x[0][e + 2], x[0][e + 3]};
+      store4<T>(to + e, four);
+    }
+  }
+}
+
 __device__ __forceinline__ void widen4(uint32_t w, float power, float (&f)[4]) {
   f[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0) * power;
   f[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * power;
   f[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * power;
   f[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * power;
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* to, const float (&f)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(to) = float4{f[0], f[1], f[2], f[3]};
-  } else {
-    ushort4 w;
-    w.x = float_to_bf16(f[0]); w.y = float_to_bf16(f[1]); w.z = float_to_bf16(f[2]); w.w = float_to_bf16(f[3]);
-    *reinterpret_cast<ushort4*>(to) = w;
-  }
-}
-
 // The same blocks the other way round: 16 lanes a token, D / 16 of its codes a lane. Two thirds of what it moves are the values it
 // writes: 32,768 tokens of 8 heads of 128 into bfloat16 (202 MB) 36 us from a page's begin on, 40 from its sixth place on, 84 anywhere;
 // into 32 bits (336 MB) 92, 97 and 147.
@@ -259,10 +330,30 @@ extern "C" int holon_kv_write_q8(const void* k, const void* v, int64_t stride, v
   if (tokens == 0) return 0;
   const int size = dtype == HOLON_F32 ? 4 : 2;             // four values at once where every token's begin on a border of as many
   const int wide = ((uintptr_t)k | (uintptr_t)v | (uintptr_t)(stride * size)) % (4 * size) == 0;
+  const Target to{(uint8_t*)pages, (uint8_t*)scales, page_stride, scale_stride, write_page, write_off, tokens, kv_heads, page_size, num_pages};
 #define CALL(T, D)                                                                                                              \
-  kv_write_q8_kernel<T, D><<<dim3((tokens + RUN - 1) / RUN, kv_heads), 256, 0, (hipStream_t)stream>>>(                          \
-      (const T*)k, (const T*)v, stride, wide, (uint8_t*)pages, (uint8_t*)scales, page_stride, scale_stride, write_page,         \
-      write_off, tokens, kv_heads, page_size, num_pages)
+  kv_write_q8_kernel<T, D><<<dim3((tokens + RUN - 1) / RUN, kv_heads), 256, 0, (hipStream_t)stream>>>((const T*)k, (const T*)v, stride, wide, to)
+  FOR_TYPE_AND_SIZE(CALL);
+#undef CALL
+  HOLON_LAUNCH_OK();
+  return 0;
+}
+
+extern "C" int holon_qk_norm_rope_write_q8(const void* qkv, void* q_out, int tokens, int heads, int kv_heads, int head_dim, const void* q_weight,
+                                           const void* k_weight, float eps, const float* table, int max_positions, const int32_t* positions,
+                                           void* pages, void* scales, int64_t page_stride, int64_t scale_stride, const int32_t* write_page,
+                                           const int32_t* write_off, int page_size, int num_pages, int dtype, void* stream) {
+  if (int rc = q8_sizes("qk_norm_rope_write_q8", tokens, kv_heads, head_dim, page_size, num_pages, page_stride, scale_stride, dtype)) return rc;
+  HOLON_CHECK(heads > 0 && heads <= 65535 - kv_heads, "qk_norm_rope_write_q8: %d heads", heads);
+  HOLON_CHECK((q_weight == nullptr) == (k_weight == nullptr), "qk_norm_rope_write_q8: q and k norm weights must both be given or both be absent");
+  HOLON_CHECK(table == nullptr || (positions != nullptr && max_positions > 0), "qk_norm_rope_write_q8: a rotation needs positions");
+  HOLON_CHECK(((uintptr_t)qkv | (uintptr_t)table) % 16 == 0, "qk_norm_rope_write_q8: tensors have to lie on borders of 16 bytes");
+  if (tokens == 0) return 0;
+  const int wide = ((uintptr_t)q_weight | (uintptr_t)k_weight) % (dtype == HOLON_F32 ? 16 : 8) == 0;
+  const Target to{(uint8_t*)pages, (uint8_t*)scales, page_stride, scale_stride, write_page, write_off, tokens, kv_heads, page_size, num_pages};
+#define CALL(T, D)                                                                                                              \
+  qk_norm_rope_write_q8_kernel<T, D><<<dim3((tokens + RUN - 1) / RUN, kv_heads + heads), 256, 0, (hipStream_t)stream>>>(        \
+      (const T*)qkv, (T*)q_out, heads, (const T*)q_weight, (const T*)k_weight, wide, eps, table, max_positions, positions, to)
   FOR_TYPE_AND_SIZE(CALL);
 #undef CALL
   HOLON_LAUNCH_OK();

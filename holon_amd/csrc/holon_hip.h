@@ -551,6 +551,11 @@ int holon_bigram_embedding(const int32_t* ids, const int32_t* take_slot, const i
 int holon_kv_write_q8(const void* k, const void* v, int64_t stride, void* pages, void* scales, int64_t page_stride,
                       int64_t scale_stride, const int32_t* write_page, const int32_t* write_off, int tokens, int kv_heads,
                       int head_dim, int page_size, int num_pages, int dtype, void* stream);
+// holon_qk_norm_rope_write (whole heads turned: table [max_positions, head_dim]) into the 8-bit cache.
+int holon_qk_norm_rope_write_q8(const void* qkv, void* q_out, int tokens, int heads, int kv_heads, int head_dim, const void* q_weight,
+                                const void* k_weight, float eps, const float* table, int max_positions, const int32_t* positions,
+                                void* pages, void* scales, int64_t page_stride, int64_t scale_stride, const int32_t* write_page,
+                                const int32_t* write_off, int page_size, int num_pages, int dtype, void* stream);
 int holon_kv_read_q8(void* k, void* v, const void* pages, const void* scales, int64_t page_stride, int64_t scale_stride,
                      const int32_t* read_page, const int32_t* read_off, int tokens, int kv_heads, int head_dim, int page_size,
                      int num_pages, int dtype, void* stream);

@@ -182,6 +182,13 @@ class Kernels(Protocol):
         k and v may be columns of wider rows (equally far apart). A token whose place lies outside the pool or the page is not
         written. Two tokens of one place: their bytes mix (the padding rows of a captured step share the null page)."""
 
+    def qk_norm_rope_write_q8(self, qkv: torch.Tensor, heads: int, kv_heads: int, head_dim: int, q_weight: torch.Tensor | None,
+                              k_weight: torch.Tensor | None, eps: float, table: torch.Tensor | None, positions: torch.Tensor,
+                              pages: torch.Tensor, scales: torch.Tensor, write_page: torch.Tensor, write_off: torch.Tensor,
+                              page_size: int) -> torch.Tensor:
+        """`qk_norm_rope_write` with keys and values into an 8-bit cache (`kv_write_q8`), the roundings of the two one after the
+        other; the whole head is rotated or none of it. A position outside the table takes its first or its last row."""
+
     def kv_read_q8(self, pages: torch.Tensor, scales: torch.Tensor, read_page: torch.Tensor, read_off: torch.Tensor, page_size: int,
                    dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         """What the places (read_page[t], read_off[t]) of an 8-bit cache stand for: (k, v), new tensors [T, Hkv, D], code * 2^e

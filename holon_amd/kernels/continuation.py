@@ -22,6 +22,7 @@ _INT32 = torch.int32
 
 SYMBOLS = {
     "holon_kv_write_q8": ([_P, _P, _L, _P, _P, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _P], _I),
+    "holon_qk_norm_rope_write_q8": ([_P, _P, _I, _I, _I, _I, _P, _P, ctypes.c_float, _P, _I, _P, _P, _P, _L, _L, _P, _P, _I, _I, _I, _P], _I),
     "holon_kv_read_q8": ([_P, _P, _P, _P, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _P], _I),
     "holon_cache_attention_room": ([ctypes.c_char_p], _L),
     "holon_cache_attention": ([ctypes.c_char_p, _P, _P, _P, _P], _I),
@@ -90,6 +91,11 @@ class ContinuationOps:
             _fail(f"{what}: pages and scales have to lie on borders of 16 bytes")
         return n, kv, wide // page_size, at, step, to, gap
 
+    def _paged_q8(self, what: str, pages: torch.Tensor, scales: torch.Tensor, page_size: int, device: int) -> tuple:
+        if scales is None:
+            _fail(f"{what}: an 8-bit cache has scales")
+        return self._paged(what, pages, scales, page_size, device)
+
     def check_cache_q8(self, head_dim: int, page_size: int) -> None:
         if head_dim not in (64, 128, 256) or page_size <= 0 or page_size % 16:
             _fail(f"8-bit cache: heads of {head_dim} in pages of {page_size} tokens are not served (64, 128 and 256; multiples of 16)")
@@ -97,7 +103,7 @@ class ContinuationOps:
     def kv_write_q8(self, k, v, pages, scales, write_page, write_off, page_size) -> None:
         what = "kv_write_q8"
         device = self._place(what, k)
-        n, kv, dim, at, step, to, gap = self._paged(what, pages, scales, page_size, device)
+        n, kv, dim, at, step, to, gap = self._paged_q8(what, pages, scales, page_size, device)
         shape, dtype = k.shape, k.dtype
         t = shape[0] if shape else -1
         if dtype not in _DT or v.dtype is not dtype or shape != (t, kv, dim) or v.shape != shape or v.get_device() != device:
@@ -111,10 +117,39 @@ class ContinuationOps:
         self._call(self.lib.holon_kv_write_q8, k.data_ptr(), v.data_ptr(), row, at, to, step, gap, _ints(what + " pages", write_page, t, device),
                    _ints(what + " offsets", write_off, t, device), t, kv, dim, page_size, n, _DT[dtype], self._stream_of(device))
 
+    def qk_norm_rope_write_q8(self, qkv, heads, kv_heads, head_dim, q_weight, k_weight, eps, table, positions, pages, scales, write_page,
+                              write_off, page_size):
+        what = "qk_norm_rope_write_q8"
+        device = self._place(what, qkv)
+        n, kv, dim, at, step, to, gap = self._paged_q8(what, pages, scales, page_size, device)
+        dtype, shape = qkv.dtype, qkv.shape
+        if dtype not in _DT or heads < 1 or (kv, dim) != (kv_heads, head_dim) or len(shape) != 2 or shape[1] != (heads + 2 * kv) * dim \
+                or not qkv.is_contiguous():
+            _fail(f"{what}: a projection {tuple(shape)} {dtype} (strides {qkv.stride()}) of {heads} heads over {kv_heads} of {head_dim}, "
+                  f"into a cache of {kv} of {dim}")
+        t, weights, turn, where, most = shape[0], [None, None], None, None, 0
+        if (q_weight is None) != (k_weight is None):
+            _fail(f"{what}: q and k norm weights come together")
+        if q_weight is not None:
+            for w in (q_weight, k_weight):
+                if w.dtype is not dtype or w.shape != (dim,) or not w.is_contiguous() or w.get_device() != device:
+                    _fail(f"{what}: a norm weight {tuple(w.shape)} {w.dtype} on {w.device} for heads of {dim} in {dtype}")
+            weights = [q_weight.data_ptr(), k_weight.data_ptr()]
+        if table is not None:
+            if table.dtype is not torch.float32 or table.dim() != 2 or table.shape[1] != dim or table.shape[0] < 1 or not table.is_contiguous() \
+                    or table.get_device() != device:
+                _fail(f"{what}: a rope table {tuple(table.shape)} {table.dtype} on {table.device} (whole heads of {dim} are turned)")
+            turn, most, where = table.data_ptr(), table.shape[0], _ints(what + " positions", positions, t, device)
+        q = torch.empty((t, heads, dim), dtype=dtype, device=qkv.device)
+        self._call(self.lib.holon_qk_norm_rope_write_q8, qkv.data_ptr(), q.data_ptr(), t, heads, kv, dim, *weights, float(eps), turn, most, where,
+                   at, to, step, gap, _ints(what + " pages", write_page, t, device), _ints(what + " offsets", write_off, t, device), page_size, n,
+                   _DT[dtype], self._stream_of(device))
+        return q
+
     def kv_read_q8(self, pages, scales, read_page, read_off, page_size, dtype=torch.bfloat16):
         what = "kv_read_q8"
         device = self._place(what, pages)
-        n, kv, dim, at, step, to, gap = self._paged(what, pages, scales, page_size, device)
+        n, kv, dim, at, step, to, gap = self._paged_q8(what, pages, scales, page_size, device)
         if dtype not in _DT:
             _fail(f"{what}: into {dtype} (float32 and bfloat16 are served)")
         t = read_page.shape[0] if read_page.dim() == 1 else -1

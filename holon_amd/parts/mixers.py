@@ -95,6 +95,11 @@ class GQA(Part):
                 step.positions, pages, view.table, view.write_page, view.write_off, step.rows, view.page_size,
                 self.scale, self.window, writes=site.writes)
             return self.o_proj(out.view(t, hq * d), residual=residual)
+        if self.q8 and self._fused is not None and site.writes and (self._fused["table"] is None or self._fused["table"].shape[1] == d):
+            q = k.qk_norm_rope_write_q8(
+                qkv, hq, hkv, d, self.q_norm.weight if self.q_norm is not None else None,
+                self.k_norm.weight if self.k_norm is not None else None, self._fused["eps"], self._fused["table"],
+                step.positions, pages, scales, view.write_page, view.write_off, view.page_size)
         else:
             q = qkv[:, : hq * d].contiguous().view(t, hq, d)
             kk = qkv[:, hq * d: (hq + hkv) * d].contiguous().view(t, hkv, d) if site.writes else None

@@ -267,6 +267,17 @@ class TorchKernels:
                 vp[page, :, :, off] = code
             powers[page, part, :, off] = power
 
+    def qk_norm_rope_write_q8(self, qkv, heads, kv_heads, head_dim, q_weight, k_weight, eps, table, positions, pages, scales, write_page,
+                              write_off, page_size):
+        t = qkv.shape[0]
+        q, k, v = (x.reshape(t, -1, head_dim) for x in qkv.split([heads * head_dim, kv_heads * head_dim, kv_heads * head_dim], 1))
+        if q_weight is not None:
+            q, k = _rmsnorm(q, q_weight, eps), _rmsnorm(k, k_weight, eps)
+        if table is not None:
+            q, k = _rope(q, positions, table), _rope(k, positions, table)
+        self.kv_write_q8(k, v, pages, scales, write_page, write_off, page_size)
+        return q.contiguous()
+
     def kv_read_q8(self, pages, scales, read_page, read_off, page_size, dtype=torch.bfloat16):
         n, _, hkv, wide = pages.shape
         k, v = dequantise_q8(pages, scales, page_size)

@@ -193,7 +193,7 @@ class Refusing(ContinuationOps):
     """The checks alone: tensors may lie anywhere, nothing is launched."""
 
     class lib:
-        holon_kv_write_q8 = holon_kv_read_q8 = holon_cache_attention = holon_verify_drafts = None
+        holon_kv_write_q8 = holon_kv_read_q8 = holon_cache_attention = holon_verify_drafts = holon_qk_norm_rope_write_q8 = None
         holon_cache_attention_room = staticmethod(lambda *a: 0)
         holon_verify_drafts_room = staticmethod(lambda *a: 16)
 
@@ -261,6 +261,35 @@ def test_refused_caches_and_rows():
     with pytest.raises(KernelError, match="borders of 16"):
         ops.kv_read_q8(shifted, torch.zeros(4, 2, 1, 16, dtype=torch.uint8), at, at, 16)
     assert len(ops.launched) == 5
+
+
+def test_refused_caches_without_scales():
+    """A bfloat16 cache has pages of the same shape: without scales it is no 8-bit cache."""
+    ops, at = Refusing(), torch.zeros(5, dtype=torch.int32)
+    k, pages = torch.randn(5, 2, 64).bfloat16(), torch.zeros(3, 2, 2, 1024).bfloat16()
+    for bad in (lambda: ops.kv_write_q8(k, k, pages, None, at, at, 16), lambda: ops.kv_read_q8(pages, None, at, at, 16),
+                lambda: ops.qk_norm_rope_write_q8(torch.zeros(5, 512).bfloat16(), 4, 2, 64, None, None, 1e-6, None, at, pages, None, at, at, 16)):
+        with pytest.raises(KernelError, match="an 8-bit cache has scales"):
+            bad()
+    assert not ops.launched
+
+
+def test_refused_projections():
+    ops = Refusing()
+    at, w, table = torch.zeros(5, dtype=torch.int32), torch.ones(64).bfloat16(), torch.zeros(9, 64)
+    pages, scales = torch.zeros(3, 2, 2, 1024, dtype=torch.uint8), torch.zeros(3, 2, 2, 16, dtype=torch.uint8)
+    qkv = torch.zeros(5, 512).bfloat16()
+    good = dict(qkv=qkv, heads=4, kv_heads=2, head_dim=64, q_weight=w, k_weight=w, eps=1e-6, table=table, positions=at, pages=pages, scales=scales,
+                write_page=at, write_off=at, page_size=16)
+    ops.qk_norm_rope_write_q8(**good)
+    ops.qk_norm_rope_write_q8(**{**good, "q_weight": None, "k_weight": None, "table": None, "positions": None})
+    for name, bad in (("qkv", qkv.half()), ("qkv", torch.zeros(512, 5).bfloat16().t()), ("qkv", qkv[:, :448]), ("heads", 3), ("kv_heads", 1),
+                      ("head_dim", 128), ("q_weight", None), ("k_weight", w.float()), ("k_weight", w[:32]), ("table", table[:, :32]),
+                      ("table", table.bfloat16()), ("table", table[:0]), ("positions", at.long()), ("positions", at[:4]), ("scales", scales[:2]),
+                      ("write_page", at[:4]), ("write_off", at.float()), ("page_size", 32)):
+        with pytest.raises(KernelError):
+            ops.qk_norm_rope_write_q8(**{**good, name: bad})
+    assert len(ops.launched) == 2
 
 
 def test_refused_prefixes():
@@ -382,6 +411,49 @@ def test_stretches_that_begin_and_end_anywhere(hip, d, page, holes):
     for x, y in zip(hip.kv_read_q8(*views(got), wp.cuda(), wo.cuda(), page, torch.float32),
                     PLAIN.kv_read_q8(*views(want), wp, wo, page, torch.float32)):
         assert torch.equal(x.cpu(), y)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(("t", "heads", "kv", "d", "page", "norm", "turn"),
+                         [(1, 1, 1, 64, 16, True, True), (8, 32, 8, 128, 16, True, True), (37, 6, 2, 64, 32, True, True), (100, 4, 2, 256, 16, True, True),
+                          (70, 4, 4, 128, 48, False, True), (33, 6, 3, 64, 16, True, False), (50, 5, 1, 256, 16, False, False), (513, 8, 2, 128, 16, True, True)])
+def test_projections_normed_turned_and_written(hip, t, heads, kv, d, page, norm, turn, dtype):
+    """The merged projection in one kernel. Roundings of `dtype` may fall the other way (a norm's sum is in another order, a rotation's
+    products may be fused). The norm's moves a value by eps of itself, which turned is eps of the pair's size |(a, b)| at most (Cauchy),
+    the rotation's own by eps more: 2 eps of that size, and 2^-20 for the arithmetic in 32 bits. What the cache holds of a key is off
+    by 2^-4 of the value or 2^-10 of its row's power besides, on either side. Values: exactly."""
+    g = torch.Generator().manual_seed(t + d)
+    qkv = (torch.randn(t, (heads + 2 * kv) * d, generator=g) * torch.exp(torch.randn(t, 1, generator=g))).to(dtype)
+    qw, kw = ((1 + 0.3 * torch.randn(d, generator=g)).to(dtype) for _ in range(2)) if norm else (None, None)
+    angle = torch.arange(600.0)[:, None] * 10000.0 ** (-torch.arange(0, d, 2) / d)
+    table = torch.cat((angle.cos(), angle.sin()), 1).contiguous() if turn else None
+    rng = np.random.default_rng(t)
+    n = t // page + 4
+    place = rng.permutation(n)[(np.arange(t) + 5) // page] * page + (np.arange(t) + 5) % page
+    place[t // 2 + 1: t // 2 + 3] = -1
+    wp, wo, pos = (torch.as_tensor(x.astype(np.int32)) for x in (place // page, place % page, rng.integers(0, 600, t)))
+    both, views = _blank(n, kv, page, d, t)
+    want, got = both.clone(), both.cuda()
+    wq = PLAIN.qk_norm_rope_write_q8(qkv, heads, kv, d, qw, kw, 1e-6, table, pos, *views(want), wp, wo, page)
+    on = lambda x: None if x is None else x.cuda()                                                  # noqa: E731
+    gq = hip.qk_norm_rope_write_q8(on(qkv), heads, kv, d, on(qw), on(kw), 1e-6, on(table), on(pos), *views(got), wp.cuda(), wo.cuda(), page)
+    assert gq.dtype == dtype and gq.shape == (t, heads, d)
+    gq, wq = gq.double().cpu(), wq.double()
+    size = torch.hypot(wq[..., : d // 2], wq[..., d // 2:]).repeat(1, 1, 2)
+    off = 2 * torch.finfo(dtype).eps + 2 ** -20
+    assert ((gq - wq).abs() <= off * size).all()
+    (a, sa), (b, sb) = views(want), views(got.cpu())
+    assert torch.equal(a[:, 1], b[:, 1]) and torch.equal(sa[:, 1], sb[:, 1])
+    there = torch.zeros(n, page, dtype=torch.bool)
+    there[wp[wp >= 0].long(), wo[wp >= 0].long()] = True
+    rows = lambda x: x[:, 0].view(n, kv, page, d).transpose(1, 2)                                   # noqa: E731
+    assert torch.equal(rows(a)[~there], rows(b)[~there]) and torch.equal(sa[:, 0].transpose(1, 2)[~there], sb[:, 0].transpose(1, 2)[~there])
+    x, y = (dequantise_q8(c, s, page)[0].double().transpose(1, 2)[there] for c, s in ((a, sa), (b, sb)))
+    power = torch.exp2(torch.maximum(sa[:, 0], sb[:, 0]).double() - 127).transpose(1, 2)[there][..., None]
+    size = torch.hypot(x[..., : d // 2], x[..., d // 2:]).repeat(1, 1, 2) * (1 + 2 ** -3) + 2.0 ** -9 * power
+    assert ((x - y).abs() <= off * size + 2.0 ** -4 * (1 + 2 ** -3) * (x.abs() + y.abs()) + 2.0 ** -9 * power).all()
+    assert (x != y).double().mean() < 0.02              # (2^-20 passes a border between steps of 2^-8 once in 2^11)
 
 
 @gpu
