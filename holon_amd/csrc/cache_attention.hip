@@ -196,6 +196,9 @@ __device__ __forceinline__ Column column_of(const CacheArgs& a, int f, int hk, i
 //   O^T = V^T P^T: A = 16 dims x 32 keys straight from the transposed values (a run is one 16-byte load), B = the probabilities.
 // Codes: KB = 64, and a lane's 16-byte load of a key is 16 dims, its first 8 the operand of one product and its last 8 of the
 // next; the queries lie the same way. bfloat16: KB = 32.
+// Memory bounds it behind long contexts, a chain of loads (length and slot, table, keys, values) behind short ones. 32 heads over 8 of
+// 128: 8 rows of up to 32,768 keys of 8 bits 74 us and the merge 7 (4.9 TB/s), 64 of 4,096 102 with it (5.3), of bfloat16 180 (5.9); one
+// row of 300 7.8.
 // Waves a block at most: eight where a lane needs no more than 256 registers.
 constexpr int most_waves(int D, bool f32, int NT) { return D == 256 || f32 || NT > 1 ? 4 : 8; }
 
@@ -546,6 +549,9 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
 //     of the stage's first 16 and of its last: the B operands of
 //   O^T (32 dims x 32 columns) += V^T P^T: A = 32 dims x 16 keys, the values transposed as in the pages.
 // Rows of LDS are swizzled by pieces of 16 bytes, so that 16 lanes that read one piece of 16 rows touch every bank once.
+// A wave's own chain bounds it, scores, softmax, products, with two waves a SIMD: 32 heads over 8 of 128, 2,048 tokens behind 6,144 354
+// us over codes and 331 over bfloat16 (0.68, 0.73 PFLOP/s), 4,096 behind 28,672 0.78 and 0.88. The next stage's scores beside this one's
+// softmax would need more registers than there are (spilled: 498 us), and a second stage ahead in registers brings nothing (407).
 constexpr float SLACK = 8.f;   // see where it is used
 
 template <int D, bool Q8, int WAVES>
@@ -932,6 +938,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) 
 
 // The groups' prefixes and the rows' own keys in one launch: neither fills the GPU by itself for long (the first are few long
 // walks, the second many short ones), and a block of one kind waits beside a block of the other. Blocks of the first kind come first.
+// 64 rows of 32 heads over 8 of 128, up to 512 keys of their own behind one prefix of up to 16,384, bfloat16: 52 us, in two launches 44 + 24.
 template <int D, bool Q8, bool TILES>
 __global__ void __launch_bounds__(256, 2) cache_prefix_kernel(CacheArgs p, CacheArgs r, int prefix_blocks, int groups, int row_blocks,
                                                               int max_query) {
@@ -948,7 +955,8 @@ __global__ void __launch_bounds__(256, 2) cache_prefix_kernel(CacheArgs p, Cache
   }
 }
 
-// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over a cell's parts, in their order: D / 4 threads a (token, head).
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over a cell's parts, in their order: D / 4 threads a (token, head). 5 to 8 us, of
+// which the launch and the chain of two loads are 4.
 template <int D, typename QT>
 __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_query, int less_than, int64_t cells) {
   constexpr int LANES = D / 4;
