@@ -936,21 +936,23 @@ __global__ void __launch_bounds__(WAVES * WAVE, D == 256 || WAVES == 8 ? 1 : 2) 
   tiles_block<D, Q8, WAVES>(a, by_group, less_than, folded, blockIdx.y, gridDim.y, blockIdx.x, blockIdx.z, sh);
 }
 
-// The groups' prefixes and the rows' own keys in one launch: neither fills the GPU by itself for long (the first are few long
-// walks, the second many short ones), and a block of one kind waits beside a block of the other. Blocks of the first kind come first.
+// Two kinds of work in one launch, blocks of the first kind first: the groups' prefixes and the rows' own keys, neither of which fills the
+// GPU by itself for long (the first are few long walks, the second many short ones); or a portion's tiles and the decode rows of the
+// step, which take the compute units that the shorter walks of the portion leave.
 // 64 rows of 32 heads over 8 of 128, up to 512 keys of their own behind one prefix of up to 16,384, bfloat16: 52 us, in two launches 44 + 24.
-template <int D, bool Q8, bool TILES>
-__global__ void __launch_bounds__(256, 2) cache_prefix_kernel(CacheArgs p, CacheArgs r, int prefix_blocks, int groups, int row_blocks,
-                                                              int max_query) {
-  using Tiles = TilesLds<D, Q8, 4>;
-  __shared__ __attribute__((aligned(1024))) unsigned char mem[TILES ? sizeof(Tiles) : 3 * (16 * D + 32) * sizeof(float)];
-  static_assert(sizeof(Tiles) >= 3 * (16 * D + 32) * sizeof(float), "the rows' sums fit where the stages lie");
+template <int D, bool Q8, bool TILES, int WAVES>
+__global__ void __launch_bounds__(WAVES* WAVE, D == 256 || WAVES == 8 ? 1 : 2)
+    cache_both_kernel(CacheArgs p, CacheArgs r, int by_group, int less_than, int folded, int first_blocks, int jobs, int row_blocks, int max_query) {
+  using Tiles = TilesLds<D, Q8, WAVES>;
+  constexpr size_t ROWS = (WAVES - 1) * (16 * D + 32) * sizeof(float);
+  __shared__ __attribute__((aligned(1024))) unsigned char mem[TILES && sizeof(Tiles) > ROWS ? sizeof(Tiles) : ROWS];
   const int hk = blockIdx.x % p.kv_heads, at = blockIdx.x / p.kv_heads;
-  if (at < prefix_blocks * groups) {
-    if constexpr (TILES) tiles_block<D, Q8, 4>(p, 1, 0, 0, at % prefix_blocks, prefix_blocks, hk, at / prefix_blocks, *reinterpret_cast<Tiles*>(mem));
-    else rows_block<D, Q8, bf16_t, 1>(p, 1, 0, at % prefix_blocks, hk, at / prefix_blocks, reinterpret_cast<float*>(mem));
+  if (at < first_blocks * jobs) {
+    if constexpr (TILES)
+      tiles_block<D, Q8, WAVES>(p, by_group, less_than, folded, at % first_blocks, first_blocks, hk, at / first_blocks, *reinterpret_cast<Tiles*>(mem));
+    else rows_block<D, Q8, bf16_t, 1>(p, by_group, 0, at % first_blocks, hk, at / first_blocks, reinterpret_cast<float*>(mem));
   } else {
-    const int x = at - prefix_blocks * groups;
+    const int x = at - first_blocks * jobs;
     rows_block<D, Q8, bf16_t, 1>(r, 0, max_query, x % row_blocks, hk, x / row_blocks, reinterpret_cast<float*>(mem));
   }
 }
@@ -1059,20 +1061,31 @@ void launch_kind(const CacheArgs& a, const Launch& w, const Cut& c, int jobs, in
   else if (w.dtype == HOLON_BF16) launch_size<D, true, bf16_t>(a, c, jobs, by_group, most, less_than, w.stream);
   else launch_size<D, true, float>(a, c, jobs, by_group, most, less_than, w.stream);
 }
-// The prefix kernel: groups cut by `shared`, `n_rows` rows of up to `most` queries that leave `own` parts each.
+// Two kinds of work in one launch: `jobs` groups (or rows) of up to `columns` columns, cut by `first`, and then n_rows rows of up to `most`
+// queries that leave `own` parts each (r.budget: as many blocks in all as that says).
 template <int D>
-void launch_prefix(const CacheArgs& p, const CacheArgs& r, const Launch& w, const Cut& shared, int groups, int64_t group_columns, int n_rows, int most,
-                   int own) {
-  const int prefix_blocks = (shared.tiles ? shared.tiles : (int)((group_columns + 15) / 16)) * shared.parts();
-  const int row_blocks = (int)(((int64_t)most * (r.heads / r.kv_heads) + 15) / 16) * own;
-  const dim3 grid((unsigned)(p.kv_heads * ((int64_t)prefix_blocks * groups + (int64_t)row_blocks * n_rows)));
-  const auto go = [&](auto q8) {
-    constexpr bool Q8 = decltype(q8)::value;
-    if (shared.tiles) cache_prefix_kernel<D, Q8, true><<<grid, 256, 0, w.stream>>>(p, r, prefix_blocks, groups, row_blocks, most);
-    else cache_prefix_kernel<D, Q8, false><<<grid, 256, 0, w.stream>>>(p, r, prefix_blocks, groups, row_blocks, most);
+void launch_both(const CacheArgs& p, const CacheArgs& r, const Launch& w, const Cut& first, int by_group, int less_than, int jobs, int64_t columns,
+                 int n_rows, int most, int own) {
+  const int first_blocks = (first.tiles ? first.tiles : (int)((columns + 15) / 16)) * first.parts();
+  const int row_tiles = (int)(((int64_t)most * (r.heads / r.kv_heads) + 15) / 16);
+  const int row_blocks = row_tiles * (r.budget ? r.budget + n_rows : own), row_jobs = r.budget ? 1 : n_rows;
+  const dim3 grid((unsigned)(p.kv_heads * ((int64_t)first_blocks * jobs + (int64_t)row_blocks * row_jobs)));
+  const int folded = !by_group && (int64_t)p.kv_heads * first_blocks * jobs <= 512;
+  const auto go = [&](auto q8, auto tiles, auto waves) {
+    constexpr int WAVES = decltype(waves)::value;
+    cache_both_kernel<D, decltype(q8)::value, decltype(tiles)::value, WAVES><<<grid, WAVES * WAVE, 0, w.stream>>>(
+        p, r, by_group, less_than, folded, first_blocks, jobs, row_blocks, most);
   };
-  if (w.q8) go(std::true_type{});
-  else go(std::false_type{});
+  const auto kind = [&](auto q8) {
+    const std::integral_constant<int, 4> four;
+    if constexpr (D <= 128) {
+      if (!first.tiles) return go(q8, std::false_type{}, four);
+      if (first.waves == 8) return go(q8, std::true_type{}, std::integral_constant<int, 8>{});
+    }
+    go(q8, std::true_type{}, four);
+  };
+  if (w.q8) kind(std::true_type{});
+  else kind(std::false_type{});
 }
 template <int D>
 void launch_merge(const CacheArgs& a, const Launch& w, int max_query, int less_than, int64_t cells) {
@@ -1129,7 +1142,7 @@ int64_t seen_span(int64_t len, int64_t queries, int window) {
 struct Plan {
   Cut decode, few, many, shared;
   int few_query = 0;                       // rows of up to so many queries are among the few
-  bool any_decode, any_few, any_many, any_shared, by_token, together = false;
+  bool any_decode, any_few, any_many, any_shared, by_token, together = false, beside = false;
   int parts = 1;                           // of a cell, where cells go by token
   int64_t decode_cells = 0, few_cells = 0, many_cells = 0;
 };
@@ -1190,6 +1203,14 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
     // Rows of long contexts are cut by their lengths. In equal numbers of shares | by lengths, us in a graph, 32 heads over 8 of 128, 8
     // bits: 32,768 and seven of 500 keys 40 | 29, 32,768 and fifteen of 500 67 | 31, 16,384 and 47 of 700 83 | 33, eight of 11,000 to 32,768 80 |
     // 79; all alike, eight of 32,768 109 | 112, 32 of 4,096 51 | 51; where rows are short, 900 to 4,096, 12 | 16.
+    // A portion's blocks and the decode rows in one launch. Two | one, us in a graph, 8 bits, 32 heads over 8 of 128: a portion of 2,048 behind
+    // 6,144 and seven rows of 8,000 364 | 341, 512 behind 28,672 and 16 of 4,096 373 | 351, 256 and 32 of 1,000 36 | 27, 128 and one of 300
+    // 19 | 12; where the decode rows are most of the step, 512 behind 2,000 and 64 of 4,096 167 | 172 (16 over 8 of 64, bfloat16 135 | 144).
+    p.beside = p.any_decode && p.any_many && group <= 16 && !f32;
+    if (p.beside) {                                        // (in blocks of the portion's size)
+      p.decode.splits = p.decode.parts() * p.many.waves;
+      p.decode.waves = p.many.waves;
+    }
     if (p.any_decode && p.decode.parts() > 1 && n_decode > 1 && n_decode <= 64 && seen_span(max_decode_len, 1, window) > 4096)
       p.decode.budget = p.decode.parts() * n_decode;
     if (p.any_decode && p.decode.parts() > 1)
@@ -1267,8 +1288,8 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
       r.splits = own * 4;
       r.part_first = p.shared.parts();
       const int64_t columns = (int64_t)c.max_group_query * (heads / c.kv_heads);
-      if (head_dim == 64) launch_prefix<64>(a, r, w, p.shared, c.n_groups, columns, n_rows, most, own);
-      else launch_prefix<128>(a, r, w, p.shared, c.n_groups, columns, n_rows, most, own);
+      if (head_dim == 64) launch_both<64>(a, r, w, p.shared, 1, 0, c.n_groups, columns, n_rows, most, own);
+      else launch_both<128>(a, r, w, p.shared, 1, 0, c.n_groups, columns, n_rows, most, own);
       merge(1, 0, c.tokens * heads);
       HOLON_LAUNCH_OK();
       return 0;
@@ -1276,24 +1297,47 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
     launch(p.shared, c.n_groups, 1, c.max_group_query, 0);
     a.part_first = p.shared.parts();
   }
-  const auto serve = [&](bool any, const Cut& cut, const int32_t* ids, int n_rows, int most, int less_than, int64_t cells) {
-    if (!any) return;
+  const auto set = [&](const Cut& cut, const int32_t* ids, int n_rows, int most, int64_t cells) {
     a.row_ids = ids;
     a.budget = cut.budget;
     a.n_rows = n_rows;
-    if (!p.by_token) {
-      a.parts = cut.parts(); a.cell_queries = most;
-      a.part_o = at; a.part_ml = at + cells * head_dim;
-      at += cells * (head_dim + 2);
-      a.row_parts = (int2*)at;
-      if (cut.budget) at += 2 * n_rows;
-    }
-    launch(cut, n_rows, 0, most, less_than);
+    a.splits = cut.splits;
+    if (p.by_token) return;
+    a.parts = cut.parts(); a.cell_queries = most;
+    a.part_o = at; a.part_ml = at + cells * head_dim;
+    at += cells * (head_dim + 2);
+    a.row_parts = (int2*)at;
+    if (cut.budget) at += 2 * n_rows;
+  };
+  const auto join = [&](int n_rows, int most, int less_than) {
     if (!p.by_token && a.parts > 1) merge(most, less_than, (int64_t)n_rows * most * heads);
   };
-  serve(p.any_decode, p.decode, c.decode_rows, c.n_decode, 1, 0, p.decode_cells);
+  const auto serve = [&](bool any, const Cut& cut, const int32_t* ids, int n_rows, int most, int less_than, int64_t cells) {
+    if (!any) return;
+    set(cut, ids, n_rows, most, cells);
+    launch(cut, n_rows, 0, most, less_than);
+    join(n_rows, most, less_than);
+  };
+  const int many_from = p.any_few ? p.few_query : 0;       // rows of up to so many queries are not among the many
   serve(p.any_few, p.few, c.chunk_rows, c.n_chunk, p.few_query, 0, p.few_cells);
-  serve(p.any_many, p.many, c.chunk_rows, c.n_chunk, c.max_chunk_query, p.any_few ? p.few_query : 0, p.many_cells);
+  if (p.beside) {
+    set(p.decode, c.decode_rows, c.n_decode, 1, p.decode_cells);
+    const CacheArgs rows = a;
+    set(p.many, c.chunk_rows, c.n_chunk, c.max_chunk_query, p.many_cells);
+    const CacheArgs tiles = a;
+    const int64_t columns = (int64_t)c.max_chunk_query * (heads / c.kv_heads);
+    const int own = p.decode.parts();
+    if (head_dim == 64) launch_both<64>(tiles, rows, w, p.many, 0, many_from, c.n_chunk, columns, c.n_decode, 1, own);
+    else if (head_dim == 128) launch_both<128>(tiles, rows, w, p.many, 0, many_from, c.n_chunk, columns, c.n_decode, 1, own);
+    else launch_both<256>(tiles, rows, w, p.many, 0, many_from, c.n_chunk, columns, c.n_decode, 1, own);
+    a = rows;
+    join(c.n_decode, 1, 0);
+    a = tiles;
+    join(c.n_chunk, c.max_chunk_query, many_from);
+  } else {
+    serve(p.any_decode, p.decode, c.decode_rows, c.n_decode, 1, 0, p.decode_cells);
+    serve(p.any_many, p.many, c.chunk_rows, c.n_chunk, c.max_chunk_query, many_from, p.many_cells);
+  }
   if (p.by_token) merge(1, 0, c.tokens * heads);
   HOLON_LAUNCH_OK();
   return 0;

@@ -485,6 +485,33 @@ def test_long_contexts_are_cut_and_joined(hip):
         _check(got, q, pages, scales, table, attn, 16, d ** -0.5, 4150)
 
 
+BESIDE = [
+    # (rows, heads, kv heads, head size, page, window): decode rows of short contexts and long beside portions, rows of a few queries between
+    ([(5000, 1), (37, 1), (9000, 1), (10, 1), (200, 70)], 8, 2, 128, 16, 0),
+    ([(0, 1), (600, 1), (0, 3), (100, 40), (5, 20)], 8, 2, 64, 16, 0),
+    ([(700, 1), (31, 1), (100, 40)], 16, 1, 256, 48, 0),
+    ([(4500, 1), (3, 1), (4200, 60)], 4, 1, 64, 32, 0),
+    ([(300, 1), (50, 1), (90, 80), (0, 65)], 5, 1, 128, 16, 100),
+    ([(3000, 1), (100, 1)] + [(7 * i, 65) for i in range(33)], 32, 8, 64, 16, 0),                # blocks of eight waves
+    ([(4300, 1), (1, 1), (2500, 1)] + [(3 * i, 65) for i in range(33)], 32, 8, 128, 16, -64),
+    ([(40, 1), (2000, 1), (33, 90)], 20, 1, 128, 16, 0),                                          # more heads on one than a tile has columns
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", range(len(BESIDE)))
+def test_decode_rows_beside_portions(hip, case):
+    """One launch for a step's decode rows and its portions: over codes, and over the bfloat16 cache."""
+    rows, heads, kv, d, page, window = BESIDE[case]
+    print(f"case {case}", flush=True)
+    q, pages, scales, table, attn, _ = _step(rows, heads, kv, d, page, seed=case, device="cuda")
+    got = hip.paged_attention_q8(q, pages, scales, table, attn, page, d ** -0.5, window)
+    _check(got, q, pages, scales, table, attn, page, d ** -0.5, window)
+    assert torch.equal(hip.paged_attention_q8(q, pages, scales, table, attn, page, d ** -0.5, window), got)
+    q, pages, _, table, attn, _ = _step(rows, heads, kv, d, page, seed=case, q8=False, device="cuda")
+    _check(hip.prefix_attention(q, pages, table, attn, None, page, d ** -0.5), q, pages, None, table, attn, page, d ** -0.5)
+
+
 @gpu
 def test_a_call_gives_the_same_bits_again(hip):
     """Sums have an order that the step's shapes and lengths decide: with other work between, and from another stream."""
