@@ -513,6 +513,88 @@ def test_decode_rows_beside_portions(hip, case):
 
 
 @gpu
+def test_nothing_to_do(hip):
+    """Calls of no token, no row, no request: results of their shapes, and nothing is touched."""
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    both, views = _blank(3, 2, 16, 64, 0)
+    got = both.cuda()
+    pages, scales = views(got)
+    k = torch.zeros(0, 2, 64, device="cuda")
+    hip.kv_write_q8(k, k, pages, scales, none, none, 16)
+    assert all(x.shape == (0, 2, 64) for x in hip.kv_read_q8(pages, scales, none, none, 16))
+    q = hip.qk_norm_rope_write_q8(torch.zeros(0, 512, device="cuda"), 4, 2, 64, None, None, 1e-6, None, None, pages, scales, none, none, 16)
+    assert q.shape == (0, 4, 64) and torch.equal(got.cpu(), both)
+    start = torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows = AttnRows(none, none, start, none, none, 0, 0, 0, 0, 0)
+    table = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    assert hip.paged_attention_q8(q, pages, scales, table, rows, 16, 0.1).shape == (0, 4, 64)
+    empty = torch.zeros(0, device="cuda")
+    tokens, taken = hip.verify_drafts(torch.zeros(0, 9, device="cuda"), none, None, empty, empty, empty, start, 3)
+    assert tokens.shape == (0, 4) and taken.shape == (0,)
+    one, starts = torch.full((2,), 0.5, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    tokens, taken = hip.verify_drafts(torch.zeros(0, 9, device="cuda"), none, None, empty, one, one, starts, 3)      # requests of no rows
+    assert (tokens == -1).all() and (taken == 0).all()
+
+
+@gpu
+def test_pools_past_32_bits(hip):
+    """Pages that lie more than 2^32 bytes into the pool, over both caches: written, read and attended over like any others."""
+    heads, kv, d, page = 8, 8, 128, 16
+    n, t = (1 << 32) // (2 * kv * page * d) + 200, 100
+    pages = torch.empty(n, 2, kv, page * d, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(n, 2, kv, page, dtype=torch.uint8, device="cuda")
+    order = torch.tensor([n - 1, 3, n - 7, n - 150, 0, n - 2, n - 90], dtype=torch.int32)
+    at = torch.arange(t)
+    wp, wo = order[at // page], (at % page).int()
+    k, v = torch.randn(2, t, kv, d, generator=torch.Generator().manual_seed(4)).bfloat16()
+    hip.kv_write_q8(k.cuda(), v.cuda(), pages, scales, wp.cuda(), wo.cuda(), page)
+    small = torch.zeros(7, 2, kv, page * d, dtype=torch.uint8), torch.zeros(7, 2, kv, page, dtype=torch.uint8)
+    low = (at // page).int()
+    PLAIN.kv_write_q8(k, v, *small, low, wo, page)
+    for x, y in zip(hip.kv_read_q8(pages, scales, wp.cuda(), wo.cuda(), page), PLAIN.kv_read_q8(*small, low, wo, page)):
+        assert torch.equal(x.cpu(), y)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)                                             # noqa: E731
+    q = torch.randn(71, heads, d, generator=torch.Generator().manual_seed(5)).bfloat16()
+    rows = AttnRows(i32(0, 0), i32(t, t), i32(0, 1, 71), i32(0), i32(1), 1, 1, t, 70, t)
+    there = AttnRows(*(x.cuda() if torch.is_tensor(x) else x for x in (rows.slots, rows.lens, rows.query_start, rows.decode_rows, rows.chunk_rows)),
+                     1, 1, t, 70, t)
+    got = hip.paged_attention_q8(q.cuda(), pages, scales, order[None].cuda(), there, page, d ** -0.5)
+    _check(got, q, *small, i32(*range(7))[None], rows, page, d ** -0.5)
+    del pages, scales
+    wide = torch.empty(n // 2 + 200, 2, kv, page * d, dtype=torch.bfloat16, device="cuda")
+    order = torch.where(order > 9, order - (n - n // 2 - 200), order).int()
+    held = [x.bfloat16() for x in dequantise_q8(*small, page)]
+    wide[order.long().cuda()] = torch.stack([x.reshape(7, kv, page * d) for x in held], 1).cuda()
+    got = hip.prefix_attention(q.cuda(), wide, order[None].cuda(), there, None, page, d ** -0.5)
+    _check(got, q, *small, i32(*range(7))[None], rows, page, d ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_values_off_every_border(hip, dtype):
+    """Keys, values and weights that begin at an odd element: read one by one, to the same bytes."""
+    t, kv, d, page = 40, 2, 128, 16
+    g = torch.Generator().manual_seed(8)
+    rows = torch.randn(t, 1 + 2 * kv * d, generator=g).to(dtype)
+    weights = torch.randn(2, 1 + d, generator=g).to(dtype)
+    qkv = torch.randn(t, 4 * d, generator=g).to(dtype)
+    at = torch.arange(t, dtype=torch.int32)
+    wp, wo = (at // page + 1), at % page
+    both, views = _blank(5, kv, page, d, 1)
+    want, got = both.clone(), both.cuda()
+    split = lambda x: (x[:, 1: 1 + kv * d].view(t, kv, d), x[:, 1 + kv * d:].view(t, kv, d))        # noqa: E731
+    PLAIN.kv_write_q8(*split(rows), *views(want), wp, wo, page)
+    hip.kv_write_q8(*split(rows.cuda()), *views(got), wp.cuda(), wo.cuda(), page)
+    assert torch.equal(got.cpu(), want)
+    both, views = _blank(5, 1, page, d, 1)
+    at, w = at.cuda(), weights.cuda()
+    pools = [both.cuda(), both.cuda()]
+    outs = [hip.qk_norm_rope_write_q8(qkv.cuda(), 2, 1, d, a, b, 1e-6, None, None, *views(pool), wp.cuda(), wo.cuda(), page)
+            for pool, (a, b) in zip(pools, ((w[0, 1:], w[1, 1:]), (w[0, 1:].clone(), w[1, 1:].clone())))]
+    assert torch.equal(*outs) and torch.equal(*pools)
+
+
+@gpu
 def test_a_call_gives_the_same_bits_again(hip):
     """Sums have an order that the step's shapes and lengths decide: with other work between, and from another stream."""
     other = torch.cuda.Stream()
