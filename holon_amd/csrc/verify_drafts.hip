@@ -10,10 +10,12 @@
 // of thousands of masses with a given number: exponentials and sums are in 64 bits, where the order of a sum moves a border
 // between two tokens by 1e-16 of the whole, not by more than a token's own mass as in 32.
 //
-// Three launches over pieces of 4,096 values: every row's largest value and sum of exponentials; the judgement (each block of a
-// request works it out for itself from those) and its masses; the walk through the one piece that the drawn number falls into.
-// 151,936 tokens, 64 requests of up to four drafts: 47 us (177 MB of logits, 3.8 TB/s: memory, and 64-bit arithmetic beside it), 25 and 10;
-// one request of three 4.6, 7.0 and 8.5, each a chain of loads.
+// Two launches over pieces of 4,096 values: every row's largest value and sum of exponentials; the judgement and the walk through the
+// one piece that the drawn number falls into, by a block a request. The masses of p are the pieces' sums, those of p without a certain
+// draft too but for its own piece; where drafts came with probabilities, a launch between judges (every block for itself) and sums
+// max(p - q, 0) of the rows whose draft was turned down. 151,936 tokens, 64 requests of four drafts: 45 us (177 MB of logits, 3.9 TB/s:
+// memory, and beside it 64-bit arithmetic, 34 us by its count), 22 and 11; one request of three 4.4, 6.4 and 9.0, each a chain of loads.
+// Without probabilities 85 us a call of 64 requests with the launch between, 72 without it, 18.4 and 17.2 a call of one.
 // (The walk by the last block to leave its masses, which saves a launch, took the judgement's launch over 64 requests from 28 to 111 us:
 // to see the others' masses across the XCDs each block writes back and drops what its L2 holds of the logits.)
 #include "common.h"
@@ -35,9 +37,6 @@ struct Judged {         // of one request
   float max;            // of the end row
   int row, accepted, draft;   // the end row (-1: no rows), how many drafts were taken, the one that was not (-1: none was judged)
   int token;
-};
-struct Masses {
-  double left, all;     // of max(p - q, 0), of p
 };
 
 // exp((l - max) / T) as 2^z, z = (l - max) c with c = log2(e) / T: 2^n times, on [-1/2, 1/2], the sum of (r ln 2)^k / k! up to
@@ -235,28 +234,31 @@ __device__ __forceinline__ int block_min(int v, int* part) {
   return v;
 }
 
-__global__ void __launch_bounds__(THREADS) verify_masses_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
-                                                                const float* __restrict__ draft_probs, const float* __restrict__ accept,
-                                                                const float* __restrict__ temperature,
-                                                                const int32_t* __restrict__ start, const RowPart* __restrict__ parts,
-                                                                Judged* __restrict__ judged, Masses* __restrict__ masses, int rows,
-                                                                int vocab, int most, int wide) {
+// What a block judges by: the request's rows and all that was drafted for them.
+struct Request {
+  const float* logits;
+  const int32_t* drafted;
+  const float* draft_probs;    // nullable
+  const float* accept;
+  const float* temperature;
+  const int32_t* start;
+  const RowPart* parts;
+  int rows, pieces, vocab, most;
+};
+// The judgement of request b, by every thread of a block.
+__device__ __forceinline__ Judged judge(const Request& r, int b) {
   __shared__ RowPart whole[MOST];
   __shared__ int verdict[MOST];                               // 1: taken, 0: turned down, -1: nothing to judge
-  __shared__ double part[THREADS / WAVE];
-  const int piece = blockIdx.x, pieces = gridDim.x, b = blockIdx.y, tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
-  const int first = max(start[b], 0), n = min(min(start[b + 1], rows) - first, most + 1);
-  if (n <= 0) {
-    if (piece == 0 && tid == 0) judged[b] = Judged{0.0, 0.0, 0.f, -1, 0, -1, -1};
-    return;
-  }
-  const double c = heat_of(temperature[b]);
+  const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+  const int first = max(r.start[b], 0), n = min(min(r.start[b + 1], r.rows) - first, r.most + 1);
+  if (n <= 0) return Judged{0.0, 0.0, 0.f, -1, 0, -1, -1};
+  const double c = heat_of(r.temperature[b]);
   for (int i = wave; i < n; i += THREADS / WAVE) {
-    const int row = first + i, x = drafted[row];              // (what the judgement needs is asked for before the sums are added)
-    const bool may = i + 1 < n && x >= 0 && x < vocab;
-    const int64_t at = (int64_t)row * vocab + (may ? x : 0);
-    const float lx = logits[at], qx = draft_probs != nullptr ? draft_probs[at] : 1.f, u = accept[row];
-    const RowPart w = whole_row(parts + (int64_t)row * pieces, pieces, c);
+    const int row = first + i, x = r.drafted[row];            // (what the judgement needs is asked for before the sums are added)
+    const bool may = i + 1 < n && x >= 0 && x < r.vocab;
+    const int64_t at = (int64_t)row * r.vocab + (may ? x : 0);
+    const float lx = r.logits[at], qx = r.draft_probs != nullptr ? r.draft_probs[at] : 1.f, u = r.accept[row];
+    const RowPart w = whole_row(r.parts + (int64_t)row * r.pieces, r.pieces, c);
     const bool good = c > 0.0 ? (double)u * (double)qx * w.sum <= Weight(w.max, c)(lx) : x == (w.at == NONE ? 0 : w.at);
     if (lane == 0) {
       whole[i] = w;
@@ -266,60 +268,84 @@ __global__ void __launch_bounds__(THREADS) verify_masses_kernel(const float* __r
   __syncthreads();
   int end = 0;
   while (end < n - 1 && verdict[end] == 1) ++end;
-  const bool turned_down = verdict[end] == 0, by_probs = turned_down && draft_probs != nullptr;
   const RowPart w = whole[end];
-  const int row = first + end, draft = turned_down ? drafted[row] : -1;
-  const double inv_z = w.sum > 0.0 ? 1.0 / w.sum : 0.0;
-  if (piece == 0 && tid == 0) judged[b] = Judged{inv_z, c, w.max, row, end, draft, w.at == NONE ? 0 : w.at};
-  if (c == 0.0) return;
-  const Weight weight(w.max, c);
-  float x[EACH], q[EACH];
-  load_piece(logits + (int64_t)row * vocab, piece * PIECE, vocab, wide, -INFINITY, x);
-  if (by_probs) load_piece(draft_probs + (int64_t)row * vocab, piece * PIECE, vocab, wide, 0.f, q);
-  double left = 0.0, all = 0.0;
-  weight.prepare(x);
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const double p = weight.of_value(x[i]) * inv_z;
-    all += p;
-    left += by_probs ? fmax(p - (double)q[i], 0.0) : (place_of(piece * PIECE, i) == draft ? 0.0 : p);
-  }
-  all = block_sum64(all, part);
-  left = block_sum64(left, part);
-  if (tid == 0) masses[(int64_t)b * pieces + piece] = Masses{left, all};
+  const int row = first + end;
+  return Judged{w.sum > 0.0 ? 1.0 / w.sum : 0.0, c, w.max, row, end, verdict[end] == 0 ? r.drafted[row] : -1, w.at == NONE ? 0 : w.at};
 }
 
-__global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __restrict__ logits, const int32_t* __restrict__ drafted,
-                                                              const float* __restrict__ draft_probs, const float* __restrict__ draw,
-                                                              const Judged* __restrict__ judged, const Masses* __restrict__ masses,
-                                                              int32_t* __restrict__ tokens, int32_t* __restrict__ accepted,
-                                                              int pieces, int vocab, int most) {
+// Where drafts came with probabilities: what max(p - q, 0) leaves of each piece of a row whose draft was turned down. (All else that is
+// drawn from, the rows' own sums say.)
+__global__ void __launch_bounds__(THREADS) verify_masses_kernel(Request r, Judged* __restrict__ judged, double* __restrict__ masses, int wide) {
+  __shared__ double part[THREADS / WAVE];
+  const int piece = blockIdx.x, b = blockIdx.y;
+  const Judged j = judge(r, b);
+  if (piece == 0 && threadIdx.x == 0) judged[b] = j;
+  if (j.draft < 0 || j.heat == 0.0) return;
+  float x[EACH], q[EACH];
+  load_piece(r.logits + (int64_t)j.row * r.vocab, piece * PIECE, r.vocab, wide, -INFINITY, x);
+  load_piece(r.draft_probs + (int64_t)j.row * r.vocab, piece * PIECE, r.vocab, wide, 0.f, q);
+  const Weight weight(j.max, j.heat);
+  weight.prepare(x);
+  double left = 0.0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) left += fmax(weight.of_value(x[i]) * j.inv_z - (double)q[i], 0.0);
+  left = block_sum64(left, part);
+  if (threadIdx.x == 0) masses[(int64_t)b * r.pieces + piece] = left;
+}
+
+__global__ void __launch_bounds__(THREADS) verify_draw_kernel(Request r, const float* __restrict__ draw, const Judged* __restrict__ judged,
+                                                              const double* __restrict__ masses, int32_t* __restrict__ tokens,
+                                                              int32_t* __restrict__ accepted, int wide) {
   __shared__ double part[THREADS / WAVE];
   __shared__ int ints[THREADS / WAVE];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % WAVE;
-  const Judged j = judged[b];
-  const Masses* mine = masses + (int64_t)b * pieces;
-  const Masses early = mine[min(lane, pieces - 1)];           // (asked for with the judgement)
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % WAVE, pieces = r.pieces, vocab = r.vocab;
+  const bool probs = r.draft_probs != nullptr;
+  const double* mine = masses + (int64_t)b * pieces;
+  const double early = probs ? mine[min(lane, pieces - 1)] : 0.0;      // (asked for with the judgement)
   const float u = draw[b];
+  const Judged j = probs ? judged[b] : judge(r, b);
   int token = j.token;
   if (j.row >= 0 && j.heat > 0.0) {
+    const Weight weight(j.max, j.heat);
+    const float* row = r.logits + (int64_t)j.row * vocab;
+    const RowPart* sums = r.parts + (int64_t)j.row * pieces;
+    enum { FROM_P, BUT_DRAFT, LEFT };                        // what is drawn from: p, p without the draft that was certain, max(p - q, 0)
+    int from = j.draft < 0 ? FROM_P : probs ? LEFT : BUT_DRAFT;
+    // A certain draft's piece is summed without it: its weight taken off the piece's sum would leave rounding where nothing is.
+    double without = 0.0;
+    if (from == BUT_DRAFT) {
+      const int lo = j.draft / PIECE * PIECE;
+      float x[EACH];
+      load_piece(row, lo, vocab, wide, -INFINITY, x);
+      weight.prepare(x);
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) without += place_of(lo, i) == j.draft ? 0.0 : weight.of_value(x[i]);
+      without = block_sum64(without, part);
+    }
+    // Masses of 64 pieces, a lane's each: what is left over, or (not divided by the row's sum) what the rows' kernel summed.
+    const auto mass = [&](int at) {
+      const int i = at + lane;
+      if (i >= pieces) return 0.0;
+      if (from == LEFT) return at == 0 ? early : mine[i];
+      if (from == BUT_DRAFT && i == j.draft / PIECE) return without;
+      const RowPart p = sums[i];
+      return p.sum * weight(p.max);
+    };
     // Every wave finds the piece for itself, 64 pieces at a time: the one in which the running sum passes the target, or (a number
     // so near one that rounding passed the last border) the last one with any mass.
-    double left = 0.0, all = 0.0;
-    for (int at = 0; at < pieces; at += WAVE) {
-      const Masses m = at == 0 ? early : mine[min(at + lane, pieces - 1)];
-      left += at + lane < pieces ? m.left : 0.0;
-      all += at + lane < pieces ? m.all : 0.0;
+    double total = 0.0;
+    for (;;) {
+      for (int at = 0; at < pieces; at += WAVE) total += mass(at);
+      total = wave_sum64(total);
+      if (total > 0.0 || from == FROM_P) break;
+      from = FROM_P;                                         // (q = p everywhere leaves nothing: then from p)
+      total = 0.0;
     }
-    left = wave_sum64(left);
-    all = wave_sum64(all);
-    const bool use = left > 0.0;                              // (q = p everywhere leaves nothing: then from p)
-    const double target = (double)u * (use ? left : all);
+    const double target = (double)u * total;
     int heavy = NONE;
     double base = 0.0, carry = 0.0;
     for (int at = 0; at < pieces; at += WAVE) {
-      const Masses x = at == 0 ? early : mine[min(at + lane, pieces - 1)];
-      const double m = at + lane < pieces ? (use ? x.left : x.all) : 0.0, upto = carry + wave_upto64(m);
+      const double m = mass(at), upto = carry + wave_upto64(m);
       const uint64_t over = __ballot(m > 0.0 && upto > target), some = __ballot(m > 0.0);
       if (over | some) {
         const int pick = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
@@ -331,23 +357,22 @@ __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __res
     }
     token = 0;                                                // no token has any mass
     if (heavy != NONE) {
-      const Weight weight(j.max, j.heat);
       const int lo = heavy * PIECE + tid * EACH;
-      const float* row = logits + (int64_t)j.row * vocab;
-      const float* qrow = draft_probs != nullptr && j.draft >= 0 ? draft_probs + (int64_t)j.row * vocab : nullptr;
+      const float* qrow = r.draft_probs + (int64_t)j.row * vocab;
       float v[EACH], q[EACH];
       double m[EACH], s = 0.0;
       int last = -1;
 #pragma unroll
       for (int i = 0; i < EACH; ++i) v[i] = lo + i < vocab ? row[lo + i] : -INFINITY;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) q[i] = qrow != nullptr && lo + i < vocab ? qrow[lo + i] : 0.f;
+      for (int i = 0; i < EACH; ++i) q[i] = from == LEFT && lo + i < vocab ? qrow[lo + i] : 0.f;
       weight.prepare(v);
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int x = lo + i;
-        double p = weight.of_value(v[i]) * j.inv_z;
-        if (use) p = qrow != nullptr ? fmax(p - (double)q[i], 0.0) : (x == j.draft ? 0.0 : p);
+        double p = weight.of_value(v[i]);
+        if (from == LEFT) p = fmax(p * j.inv_z - (double)q[i], 0.0);
+        else if (from == BUT_DRAFT && x == j.draft) p = 0.0;
         m[i] = p;
         s += p;
         if (p > 0.0) last = x;
@@ -364,8 +389,8 @@ __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __res
       token = found != NONE ? found : max(last, 0);
     }
   }
-  for (int i = tid; i <= most; i += THREADS)
-    tokens[(int64_t)b * (most + 1) + i] = j.row < 0 || i > j.accepted ? -1 : i == j.accepted ? token : drafted[j.row - j.accepted + i];
+  for (int i = tid; i <= r.most; i += THREADS)
+    tokens[(int64_t)b * (r.most + 1) + i] = j.row < 0 || i > j.accepted ? -1 : i == j.accepted ? token : r.drafted[j.row - j.accepted + i];
   if (tid == 0) accepted[b] = j.accepted;
 }
 
@@ -373,7 +398,7 @@ __global__ void __launch_bounds__(THREADS) verify_draw_kernel(const float* __res
 
 extern "C" int64_t holon_verify_drafts_room(int rows, int requests, int vocab) {
   const int64_t pieces = ((int64_t)vocab + PIECE - 1) / PIECE;
-  return (rows * (int64_t)sizeof(RowPart) + requests * (int64_t)sizeof(Masses)) * pieces + requests * (int64_t)sizeof(Judged);
+  return (rows * (int64_t)sizeof(RowPart) + requests * (int64_t)sizeof(double)) * pieces + requests * (int64_t)sizeof(Judged);
 }
 
 extern "C" int holon_verify_drafts(const float* logits, const int32_t* drafted, const float* draft_probs, const float* accept,
@@ -385,7 +410,7 @@ extern "C" int holon_verify_drafts(const float* logits, const int32_t* drafted, 
   if (requests == 0) return 0;
   const int pieces = (vocab + PIECE - 1) / PIECE;
   RowPart* parts = (RowPart*)room;
-  Masses* masses = (Masses*)(parts + (int64_t)rows * pieces);
+  double* masses = (double*)(parts + (int64_t)rows * pieces);
   Judged* judged = (Judged*)(masses + (int64_t)requests * pieces);
   const bool wide = vocab % 4 == 0 && ((uintptr_t)logits | (uintptr_t)draft_probs) % 16 == 0;
   hipStream_t s = (hipStream_t)stream;
@@ -393,10 +418,12 @@ extern "C" int holon_verify_drafts(const float* logits, const int32_t* drafted, 
     verify_rows_kernel<<<dim3(pieces, rows), THREADS, 0, s>>>(logits, start, temperature, parts, requests, vocab, wide);
     HOLON_LAUNCH_OK();
   }
-  verify_masses_kernel<<<dim3(pieces, requests), THREADS, 0, s>>>(logits, drafted, draft_probs, accept, temperature, start, parts, judged,
-                                                                  masses, rows, vocab, most, wide);
-  HOLON_LAUNCH_OK();
-  verify_draw_kernel<<<requests, THREADS, 0, s>>>(logits, drafted, draft_probs, draw, judged, masses, tokens, accepted, pieces, vocab, most);
+  const Request r{logits, drafted, draft_probs, accept, temperature, start, parts, rows, pieces, vocab, most};
+  if (draft_probs != nullptr) {
+    verify_masses_kernel<<<dim3(pieces, requests), THREADS, 0, s>>>(r, judged, masses, wide);
+    HOLON_LAUNCH_OK();
+  }
+  verify_draw_kernel<<<requests, THREADS, 0, s>>>(r, draw, judged, masses, tokens, accepted, wide);
   HOLON_LAUNCH_OK();
   return 0;
 }
