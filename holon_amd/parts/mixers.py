@@ -21,7 +21,7 @@ class GQA(Part):
     A run that reads another run's cache (`site.writes` false) projects and encodes queries only.
 
     With `cache_format` "q8" keys and values lie in an 8-bit cache (`Kernels.kv_write_q8`): a page is its codes and then
-    its scales, and the operations run one after the other."""
+    its scales; the projection's heads are prepared and written by one operation, attended over by another."""
 
     graph_safe = True
 

@@ -814,6 +814,31 @@ def test_verify_at_the_borders(hip):
 
 
 @gpu
+@pytest.mark.parametrize("probs", [True, False])
+def test_verify_where_little_is_left(hip, probs):
+    """A draft that holds all but some 2^-20 of a row and is turned down all the same: what is left lies in pieces of its own, beside the
+    draft in its piece, or nowhere in that piece; drawn from its first value (0) and its last. Whatever the draft's weight is rounded to,
+    its piece has no mass without it."""
+    vocab = 3 * 4096 + 7
+    others = ([], [0, 4095], [4100, 4200], [4096, 8191, 8192, vocab - 1], [vocab - 2], [1, 12290])
+    logits = torch.full((2 * 2 * len(others), vocab), float("-inf"))
+    drafted = torch.full((len(logits),), 4100 + 57, dtype=torch.int32)
+    for i, places in enumerate(others):
+        for row in range(4 * i, 4 * i + 4):
+            logits[row, drafted[row]] = 0.0
+            logits[row, places] = -14.0 - torch.arange(float(len(places)))
+            if not places:
+                logits[row, 9] = -15.0
+    q = torch.zeros_like(logits)
+    q[torch.arange(len(logits)), drafted.long()] = 1.0
+    start = torch.arange(0, len(logits) + 1, 2, dtype=torch.int32)
+    case = dict(logits=logits, drafted=drafted, draft_probs=q if probs else None, accept=torch.full((len(logits),), 1.0 - 2.0 ** -24),
+                draw=torch.tensor([0.0, 1.0 - 2.0 ** -24] * len(others)), temperature=torch.ones(2 * len(others)), start=start, most=1)
+    want = _verify(hip, case)
+    assert (want[1] == 0).all() and (want[0][:, 0] != drafted[0]).all()
+
+
+@gpu
 def test_verify_keeps_the_targets_law(hip):
     """Whatever the drafts come from, the first token is distributed as p: frequencies over many numbers within five standard errors."""
     vocab, n = 11, 30000
@@ -827,3 +852,54 @@ def test_verify_keeps_the_targets_law(hip):
                                   torch.arange(0, 2 * n + 1, 2, dtype=torch.int32).cuda(), 1)
     seen = torch.bincount(tokens[:, 0].cpu().long(), minlength=vocab).double() / n
     assert ((seen - p).abs() <= 5 * torch.sqrt(p * (1 - p) / n)).all()
+
+
+def _answers(ops, device):
+    """Six answers to one prompt of 40 tokens, three drafted tokens checked a step: written into the 8-bit cache, attended to over the
+    prefix that all share, judged, and what was taken written over what was not. Keys, values and queries are tables' rows."""
+    heads, kv, d, page, vocab, batch, drafts = 4, 2, 64, 16, 300, 6, 3
+    g = torch.Generator().manual_seed(9)
+    keys, values = torch.randn(2, vocab, kv, d, generator=g)
+    queries, head = torch.randn(vocab, heads, d, generator=g), torch.randn(heads * d, vocab, generator=g).double() * 0.08
+    i32 = lambda x: torch.as_tensor(np.asarray(x, dtype=np.int32)).to(device)                       # noqa: E731
+    prompt = torch.randint(0, vocab, (40,), generator=g)
+    table = np.array([[0, 1] + [2 + 4 * b + i for i in range(4)] for b in range(batch)])
+    pages = torch.zeros(2 + 4 * batch, 2, kv, page * d, dtype=torch.uint8, device=device)
+    scales = torch.zeros(2 + 4 * batch, 2, kv, page, dtype=torch.uint8, device=device)
+
+    def write(tokens, rows, places):
+        page_of, off = table[rows, places // page], places % page
+        ops.kv_write_q8(keys[tokens].to(device), values[tokens].to(device), pages, scales, i32(page_of), i32(off), page)
+
+    for b in range(batch):                                    # the first two pages once, the eight tokens behind them into each row's third
+        lo = 0 if b == 0 else 32
+        write(prompt[lo:], np.full(40 - lo, b), np.arange(lo, 40))
+    held, last, out = np.full(batch, 40), torch.randint(0, vocab, (batch,), generator=g), [[] for _ in range(batch)]
+    for _ in range(6):
+        q = torch.softmax(torch.randn(batch * (drafts + 1), vocab, generator=g), -1)
+        drafted = torch.multinomial(q, 1, generator=g)[:, 0].int()
+        fed = torch.cat((last[:, None], drafted.view(batch, -1)[:, :drafts]), 1).flatten().long()
+        rows = np.repeat(np.arange(batch), drafts + 1)
+        write(fed, rows, held[rows] + np.tile(np.arange(drafts + 1), batch))
+        starts = np.arange(batch + 1) * (drafts + 1)
+        attn = AttnRows(i32(range(batch)), i32(held + drafts + 1), i32(starts), i32([]), i32(range(batch)), 0, batch, 0, drafts + 1,
+                        int(held.max()) + drafts + 1)
+        shared = SharedPrefix(i32([0, batch]), i32([32]), 1, batch * (drafts + 1), 32)
+        seen = ops.prefix_attention(queries[fed].to(device), pages, i32(table), attn, shared, page, 1.5 * d ** -0.5, scales)
+        logits = (seen.cpu().double().view(len(fed), -1) @ head).float()
+        accept, draw = torch.rand(len(fed), generator=g), torch.rand(batch, generator=g)
+        tokens, taken = ops.verify_drafts(logits.to(device), drafted.to(device), q.to(device), accept.to(device), draw.to(device),
+                                          torch.full((batch,), 0.9, device=device), i32(starts), drafts)
+        tokens, taken = tokens.cpu(), taken.cpu().numpy()
+        for b in range(batch):
+            out[b] += tokens[b, : taken[b] + 1].tolist()
+        last, held = tokens[torch.arange(batch), taken].long(), held + taken + 1
+    return out, pages.cpu(), scales.cpu()
+
+
+@gpu
+def test_answers_to_one_prompt(hip):
+    """The operations one after the other, against the twins: the same tokens, the same cache."""
+    want, got = _answers(PLAIN, "cpu"), _answers(hip, "cuda")
+    assert want[0] == got[0] and torch.equal(want[1], got[1]) and torch.equal(want[2], got[2])
+    assert 6 * 6 + 3 < sum(map(len, want[0])) < 6 * 6 * 4                    # drafts were taken, and turned down
