@@ -19,6 +19,7 @@ _DT = {torch.float32: 0, torch.bfloat16: 1}
 _CODES = (torch.float8_e4m3fn, torch.uint8)
 _SCALES = (torch.float8_e8m0fnu, torch.uint8)
 _INT32 = torch.int32
+_HEADS = (64, 128, 256)
 
 SYMBOLS = {
     "holon_kv_write_q8": ([_P, _P, _L, _P, _P, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _P], _I),
@@ -38,10 +39,10 @@ def _fail(message: str) -> None:
     raise KernelError(message)
 
 
-def _ints(what: str, t: torch.Tensor, size: int, device: int) -> int:
+def _ints(what: str, name: str, t: torch.Tensor, size: int, device: int) -> int:
     """The address of an int32 vector of `size` values."""
     if t.dtype is not _INT32 or t.shape != (size,) or t.get_device() != device or not t.is_contiguous():
-        _fail(f"{what}: expected ({size},) int32 on device {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        _fail(f"{what} {name}: expected ({size},) int32 on device {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
@@ -67,10 +68,12 @@ class ContinuationOps:
     def _paged(what: str, pages: torch.Tensor, scales: torch.Tensor | None, page_size: int, device: int) -> tuple:
         """(pages, kv heads, head size, their address, bytes from page to page, the scales' two) of a cache of 8 bits, or (scales
         None) of bfloat16: shapes, types and strides checked."""
-        if pages.dim() != 4:
+        shape = pages.shape
+        if len(shape) != 4:
             _fail(f"{what}: pages {tuple(pages.shape)} are no [n, 2, Hkv, P D]")
-        (n, two, kv, wide), (step, s1, s2, s3), at = pages.shape, pages.stride(), pages.data_ptr()
-        if page_size <= 0 or page_size % 16 or wide not in (64 * page_size, 128 * page_size, 256 * page_size):
+        (n, two, kv, wide), (step, s1, s2, s3), at = shape, pages.stride(), pages.data_ptr()
+        dim = wide // page_size if page_size > 0 else 0
+        if page_size % 16 or dim not in _HEADS or dim * page_size != wide:
             _fail(f"{what}: pages {tuple(pages.shape)} of {page_size} tokens hold no heads of 64, 128 or 256 in pages of a multiple of 16")
         if two != 2 or n < 1 or kv < 1 or s3 != 1 or s2 != wide or s1 != kv * wide or (n > 1 and step < 2 * s1) or pages.get_device() != device:
             _fail(f"{what}: pages {tuple(pages.shape)} on {pages.device}, strides {pages.stride()}: [n, 2, Hkv, P D], each in one piece, where the rest is")
@@ -79,7 +82,7 @@ class ContinuationOps:
                 _fail(f"{what}: a cache of {pages.dtype} (bfloat16, or 8 bits with scales)")
             if (at | 2 * step) % 16:
                 _fail(f"{what}: pages have to lie on borders of 16 bytes")
-            return n, kv, wide // page_size, at, 2 * step, None, 0
+            return n, kv, dim, at, 2 * step, None, 0
         if pages.dtype not in _CODES or scales.dtype not in _SCALES:
             _fail(f"{what}: pages of {pages.dtype} with scales of {scales.dtype} (float8_e4m3fn and float8_e8m0fnu, or uint8 for either)")
         if scales.shape != (n, 2, kv, page_size) or scales.get_device() != device:
@@ -89,7 +92,7 @@ class ContinuationOps:
             _fail(f"{what}: the scales of a page have to lie in one piece (strides {scales.stride()})")
         if (at | step | to | gap) % 16:
             _fail(f"{what}: pages and scales have to lie on borders of 16 bytes")
-        return n, kv, wide // page_size, at, step, to, gap
+        return n, kv, dim, at, step, to, gap
 
     def _paged_q8(self, what: str, pages: torch.Tensor, scales: torch.Tensor, page_size: int, device: int) -> tuple:
         if scales is None:
@@ -97,7 +100,7 @@ class ContinuationOps:
         return self._paged(what, pages, scales, page_size, device)
 
     def check_cache_q8(self, head_dim: int, page_size: int) -> None:
-        if head_dim not in (64, 128, 256) or page_size <= 0 or page_size % 16:
+        if head_dim not in _HEADS or page_size <= 0 or page_size % 16:
             _fail(f"8-bit cache: heads of {head_dim} in pages of {page_size} tokens are not served (64, 128 and 256; multiples of 16)")
 
     def kv_write_q8(self, k, v, pages, scales, write_page, write_off, page_size) -> None:
@@ -114,8 +117,8 @@ class ContinuationOps:
         for one, two, three in (k.stride(), v.stride()):
             if three != 1 or (kv > 1 and two != dim) or (t > 1 and one != row) or row < kv * dim:
                 _fail(f"{what}: keys and values are columns of rows as far apart, got strides {k.stride()} and {v.stride()}")
-        self._call(self.lib.holon_kv_write_q8, k.data_ptr(), v.data_ptr(), row, at, to, step, gap, _ints(what + " pages", write_page, t, device),
-                   _ints(what + " offsets", write_off, t, device), t, kv, dim, page_size, n, _DT[dtype], self._stream_of(device))
+        self._call(self.lib.holon_kv_write_q8, k.data_ptr(), v.data_ptr(), row, at, to, step, gap, _ints(what, "pages", write_page, t, device),
+                   _ints(what, "offsets", write_off, t, device), t, kv, dim, page_size, n, _DT[dtype], self._stream_of(device))
 
     def qk_norm_rope_write_q8(self, qkv, heads, kv_heads, head_dim, q_weight, k_weight, eps, table, positions, pages, scales, write_page,
                               write_off, page_size):
@@ -139,10 +142,10 @@ class ContinuationOps:
             if table.dtype is not torch.float32 or table.dim() != 2 or table.shape[1] != dim or table.shape[0] < 1 or not table.is_contiguous() \
                     or table.get_device() != device:
                 _fail(f"{what}: a rope table {tuple(table.shape)} {table.dtype} on {table.device} (whole heads of {dim} are turned)")
-            turn, most, where = table.data_ptr(), table.shape[0], _ints(what + " positions", positions, t, device)
+            turn, most, where = table.data_ptr(), table.shape[0], _ints(what, "positions", positions, t, device)
         q = torch.empty((t, heads, dim), dtype=dtype, device=qkv.device)
         self._call(self.lib.holon_qk_norm_rope_write_q8, qkv.data_ptr(), q.data_ptr(), t, heads, kv, dim, *weights, float(eps), turn, most, where,
-                   at, to, step, gap, _ints(what + " pages", write_page, t, device), _ints(what + " offsets", write_off, t, device), page_size, n,
+                   at, to, step, gap, _ints(what, "pages", write_page, t, device), _ints(what, "offsets", write_off, t, device), page_size, n,
                    _DT[dtype], self._stream_of(device))
         return q
 
@@ -153,7 +156,7 @@ class ContinuationOps:
         if dtype not in _DT:
             _fail(f"{what}: into {dtype} (float32 and bfloat16 are served)")
         t = read_page.shape[0] if read_page.dim() == 1 else -1
-        rp, ro = _ints(what + " pages", read_page, t, device), _ints(what + " offsets", read_off, t, device)
+        rp, ro = _ints(what, "pages", read_page, t, device), _ints(what, "offsets", read_off, t, device)
         k = torch.empty((t, kv, dim), dtype=dtype, device=pages.device)
         v = torch.empty_like(k)
         self._call(self.lib.holon_kv_read_q8, k.data_ptr(), v.data_ptr(), at, to, step, gap, rp, ro, t, kv, dim, page_size, n, _DT[dtype],
@@ -174,38 +177,41 @@ class ContinuationOps:
         dtype, shape = q.dtype, q.shape
         if dtype is not torch.bfloat16 and (scales is None or dtype is not torch.float32):
             _fail(f"{what}: queries of {dtype} (bfloat16; over the 8-bit cache float32 too)")
-        if len(shape) != 3 or shape[2] != dim or shape[1] % kv or shape[1] == 0 or not q.is_contiguous() or q.data_ptr() % 16:
+        if len(shape) != 3:
+            _fail(f"{what}: queries {tuple(shape)} are no [T, Hq, D]")
+        (t, heads, width), q_at = shape, q.data_ptr()
+        if width != dim or heads % kv or heads == 0 or not q.is_contiguous() or q_at % 16:
             _fail(f"{what}: queries {tuple(shape)} (strides {q.stride()}) over {kv} heads of {dim}, contiguous from a border of 16 bytes")
-        t, heads, _ = shape
         held = table.shape
         if table.dtype is not _INT32 or len(held) != 2 or not table.is_contiguous() or table.get_device() != device or 0 in held:
             _fail(f"{what}: a block table {tuple(held)} {table.dtype} on {table.device}")
         if not scale > 0:
             _fail(f"{what}: a scale of {scale}")
-        b, n_decode, n_chunk = rows.slots.numel(), rows.n_decode, rows.n_chunk
+        slots, n_decode, n_chunk = rows.slots, rows.n_decode, rows.n_chunk
+        b = slots.numel()
         sink_at = starts_at = lens_at = decode = chunk = 0
         if sink is not None:
             if sink.dtype is not torch.float32 or sink.shape != (heads,) or not sink.is_contiguous() or sink.get_device() != device:
                 _fail(f"{what}: a sink {tuple(sink.shape)} {sink.dtype} for {heads} heads")
             sink_at = sink.data_ptr()
         if n_decode and not (rows.in_order and n_decode == b == t):
-            decode = _ints(what + " decode_rows", rows.decode_rows, n_decode, device)
+            decode = _ints(what, "decode_rows", rows.decode_rows, n_decode, device)
         if n_chunk:
-            chunk = _ints(what + " chunk_rows", rows.chunk_rows, n_chunk, device)
+            chunk = _ints(what, "chunk_rows", rows.chunk_rows, n_chunk, device)
         groups = most = longest = 0
         if prefix is not None and prefix.n_groups:
             groups, most, longest = prefix.n_groups, prefix.max_queries, prefix.max_len
-            starts_at = _ints(what + " group_start", prefix.group_start, groups + 1, device)
-            lens_at = _ints(what + " prefix lens", prefix.lens, groups, device)
+            starts_at = _ints(what, "group_start", prefix.group_start, groups + 1, device)
+            lens_at = _ints(what, "prefix lens", prefix.lens, groups, device)
         packed = _ATTENTION.pack(
-            at, to or 0, table.data_ptr(), _ints(what + " slots", rows.slots, b, device), _ints(what + " lens", rows.lens, b, device),
-            _ints(what + " query_start", rows.query_start, b + 1, device), decode, chunk, starts_at, lens_at, sink_at, step, gap, t,
+            at, to or 0, table.data_ptr(), _ints(what, "slots", slots, b, device), _ints(what, "lens", rows.lens, b, device),
+            _ints(what, "query_start", rows.query_start, b + 1, device), decode, chunk, starts_at, lens_at, sink_at, step, gap, t,
             n, held[1], held[0], b, n_decode, rows.max_decode_len, n_chunk, rows.max_chunk_query, rows.max_chunk_len, groups, most, longest,
             heads, kv, dim, page_size, int(window), _DT[dtype], scale)
         out = torch.empty_like(q)
         room = self.lib.holon_cache_attention_room(packed)
         space = torch.empty((room,), dtype=torch.uint8, device=q.device) if room else None
-        self._call(self.lib.holon_cache_attention, packed, q.data_ptr(), out.data_ptr(), space.data_ptr() if room else None,
+        self._call(self.lib.holon_cache_attention, packed, q_at, out.data_ptr(), space.data_ptr() if room else None,
                    self._stream_of(device))
         return out
 
@@ -225,7 +231,7 @@ class ContinuationOps:
         for x, size, name in ((accept, n, "accept"), (draw, b, "draw"), (temperature, b, "temperature")):
             if x.dtype is not f32 or x.shape != (size,) or not x.is_contiguous() or x.get_device() != device:
                 _fail(f"{what} {name}: expected ({size},) float32 on device {device}, got {tuple(x.shape)} {x.dtype} on {x.device}")
-        d, s = _ints(what + " drafted", drafted, n, device), _ints(what + " start", start, b + 1, device)
+        d, s = _ints(what, "drafted", drafted, n, device), _ints(what, "start", start, b + 1, device)
         if not 0 <= most <= 63:
             _fail(f"{what}: up to {most} drafted tokens a request (at most 63 are served)")
         place = logits.device
