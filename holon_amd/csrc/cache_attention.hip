@@ -1181,9 +1181,12 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
     if (p.together) {
       const int64_t units = (int64_t)n_groups * kv_heads;
       if (p.shared.tiles) {                                // one block a compute unit, the rows' blocks beside them
-        p.shared.waves = 4;
-        p.shared.tiles = (int)(((int64_t)max_group_query * group + 127) / 128);
-        const int64_t want = std::max<int64_t>(1, 384 / (units * p.shared.tiles));
+        // Blocks of 256 columns, if they are full, over long prefixes. 128 columns | 256, us, 64 rows of 32 heads over 8 of 128 with 256 keys of
+        // their own, bfloat16: behind 16,384 61 | 71, 32,768 89 | 93, 65,536 151 | 121, 131,072 276 | 215.
+        const int64_t columns = (int64_t)max_group_query * group;
+        p.shared.waves = max_group_len >= 49152 && (columns + 255) / 256 * 2 == (columns + 127) / 128 ? 8 : 4;
+        p.shared.tiles = (int)((columns + 32 * p.shared.waves - 1) / (32 * p.shared.waves));
+        const int64_t want = std::max<int64_t>(1, (p.shared.waves == 8 ? 256 : 384) / (units * p.shared.tiles));
         p.shared.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (max_group_len + 127) / 128));
       } else {
         const int64_t tiles = ((int64_t)max_group_query * group + 15) / 16;
@@ -1285,7 +1288,7 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
       const int own = p.parts - p.shared.parts(), n_rows = p.any_decode ? c.n_decode : c.n_chunk, most = p.any_decode ? 1 : p.few_query;
       a.splits = p.shared.splits;
       r.row_ids = p.any_decode ? c.decode_rows : c.chunk_rows;
-      r.splits = own * 4;
+      r.splits = own * p.shared.waves;
       r.part_first = p.shared.parts();
       const int64_t columns = (int64_t)c.max_group_query * (heads / c.kv_heads);
       if (head_dim == 64) launch_both<64>(a, r, w, p.shared, 1, 0, c.n_groups, columns, n_rows, most, own);

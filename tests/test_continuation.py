@@ -755,6 +755,16 @@ def test_attention_over_a_shared_prefix(hip, step, q8):
         _check(got, q, pages, scales, table, attn, page, d ** -0.5, 0, s)
 
 
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize(("d", "rows"), [(64, [(49300, 8)] * 4), (128, [(49168, 8), (49500, 8), (49169, 8), (49200, 7), (60, 3)])])
+def test_a_long_shared_prefix(hip, d, rows, q8):
+    """Prefixes long enough for blocks of 256 columns, which eight queries of four rows by eight heads fill."""
+    q, pages, scales, table, attn, prefix = _step(rows, 8, 1, d, 16, seed=d, shared=[(0, 3, 49168)], q8=q8, device="cuda")
+    got = hip.prefix_attention(q, pages, table, attn, prefix, 16, d ** -0.5, scales)
+    _check(got, q, pages, scales, table, attn, 16, d ** -0.5)
+
+
 def _drafts(counts, vocab, seed, *, probs=True, spread=2.5):
     g = torch.Generator().manual_seed(seed)
     start = [0] + list(np.cumsum(counts))
