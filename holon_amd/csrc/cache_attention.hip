@@ -1214,7 +1214,9 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
       p.decode.splits = p.decode.parts() * p.many.waves;
       p.decode.waves = p.many.waves;
     }
-    if (p.any_decode && p.decode.parts() > 1 && n_decode > 1 && n_decode <= 64 && seen_span(max_decode_len, 1, window) > 4096)
+    // (Rows of few columns alone: the kernel of many cuts all rows into the same number of shares.)
+    if (p.any_decode && !p.decode.tiles && p.decode.parts() > 1 && n_decode > 1 && n_decode <= 64 &&
+        seen_span(max_decode_len, 1, window) > 4096)
       p.decode.budget = p.decode.parts() * n_decode;
     if (p.any_decode && p.decode.parts() > 1)
       p.decode_cells = p.decode.budget ? (int64_t)(p.decode.budget + n_decode) * heads : (int64_t)n_decode * heads * p.decode.parts();

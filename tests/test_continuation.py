@@ -485,6 +485,18 @@ def test_long_contexts_are_cut_and_joined(hip):
         _check(got, q, pages, scales, table, attn, 16, d ** -0.5, 4150)
 
 
+@gpu
+@pytest.mark.parametrize(("heads", "kv", "d"), [(71, 1, 64), (130, 2, 128), (66, 1, 256)])
+@pytest.mark.parametrize("q8", [True, False])
+def test_more_heads_on_one_behind_long_contexts(hip, heads, kv, d, q8):
+    """More than 64 heads on one kv head, several decode rows of different lengths, some past 4,096 keys: alone, and beside a portion."""
+    for rows in ([(4500, 1), (30, 1), (0, 1)], [(4200, 1), (6, 3), (4097, 1)]):
+        print(f"{heads} over {kv} of {d}, {rows}", flush=True)
+        q, pages, scales, table, attn, _ = _step(rows, heads, kv, d, 16, seed=heads, q8=q8, device="cuda")
+        got = hip.paged_attention_q8(q, pages, scales, table, attn, 16, d ** -0.5) if q8 else hip.prefix_attention(q, pages, table, attn, None, 16, d ** -0.5)
+        _check(got, q, pages, scales, table, attn, 16, d ** -0.5)
+
+
 BESIDE = [
     # (rows, heads, kv heads, head size, page, window): decode rows of short contexts and long beside portions, rows of a few queries between
     ([(5000, 1), (37, 1), (9000, 1), (10, 1), (200, 70)], 8, 2, 128, 16, 0),
