@@ -76,20 +76,41 @@ __device__ __forceinline__ int shared_keys(const CacheArgs& a, int row) {
   return before >= 1 && before <= a.n_groups ? max(a.group_lens[before - 1], 0) : 0;
 }
 
+__device__ __forceinline__ int wave_least(int v) {
+  v = min(v, lane_xor<32>(v));
+  v = min(v, lane_xor<16>(v));
+  v = min(v, lane_xor<8>(v));
+  v = min(v, lane_xor<4>(v));
+  v = min(v, lane_xor<2>(v));
+  return min(v, lane_xor<1>(v));
+}
+
 // Whose queries a block takes, and which keys: queries qs .. qs + nq - 1 against keys from .. n - 1 of a row, the last of them at
-// position n - 1; or all queries of a group's rows against the prefix of n keys, which every one of them sees whole.
+// position n - 1; or all queries of a group's rows (up to row `end`) against the prefix of n keys. Those see it whole but where a row is
+// no longer than the prefix, or begins with queries inside it: `lowest` is the smallest position of a group's query, n no more than the
+// largest and one. (Lengths and starts of 64 rows are loaded together, beside the group's own: no chain of loads gets longer.)
 struct Job {
-  int row, qs, nq, n, from;
+  int row, qs, nq, n, from, end, lowest;
+  __device__ __forceinline__ bool apart() const { return lowest < n - 1; }      // (of a group) some query does not see all n keys
 };
 __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) {
   Job j;
+  j.end = j.lowest = 0;
   if (by_group) {
     j.row = a.group_start[at];
-    const int end = a.group_start[at + 1];
+    j.end = a.group_start[at + 1];
     j.qs = a.qstart[j.row];
     j.n = a.group_lens[at];
-    j.nq = end > j.row && j.n > 0 ? a.qstart[end] - j.qs : 0;
+    j.nq = j.end > j.row && j.n > 0 ? a.qstart[j.end] - j.qs : 0;
     j.from = 0;
+    int low = 0x7fffffff, high = -1;
+    for (int at64 = j.row; at64 < j.end; at64 += WAVE) {
+      const int r = min(at64 + (int)(threadIdx.x % WAVE), j.end - 1), n = a.lens[r], queries = a.qstart[r + 1] - a.qstart[r];
+      low = min(low, queries > 0 ? n - queries : low);
+      high = max(high, queries > 0 ? n - 1 : high);
+    }
+    j.lowest = __builtin_amdgcn_readfirstlane(wave_least(low));
+    j.n = min(j.n, 1 - __builtin_amdgcn_readfirstlane(wave_least(-high)));
   } else {
     const bool in_order = a.row_ids == nullptr;            // rows of one query, one a token, from the first on
     j.row = in_order ? at : a.row_ids[at];
@@ -99,6 +120,17 @@ __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) 
     j.from = shared_keys(a, j.row);
   }
   return j;
+}
+
+// The position of a token of a group's rows: its row is the last that begins at it or in front of it.
+__device__ __forceinline__ int position_in_group(const CacheArgs& a, const Job& j, int token) {
+  int row = j.row, end = j.end;
+  while (end - row > 1) {
+    const int mid = row + (end - row) / 2;
+    if (a.qstart[mid] <= token) row = mid;
+    else end = mid;
+  }
+  return a.lens[row] - (a.qstart[row + 1] - token);
 }
 
 // Decode rows of different lengths: as many blocks for each as its keys are of all rows' keys, so that blocks have about the same to
@@ -234,20 +266,22 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
     slot = __builtin_amdgcn_readlane(shares.slot, ri);
     job.qs = a.row_ids == nullptr ? job.row : a.qstart[job.row];
     job.nq = a.row_ids == nullptr ? 1 : a.qstart[job.row + 1] - job.qs;
-    job.from = 0;
+    job.from = job.end = job.lowest = 0;
     if (piece == 0 && tile0 == 0 && hk == 0 && threadIdx.x == 0) a.row_parts[ri] = int2{nth, pieces};      // (for the merge)
   } else {
     job = job_of(a, by_group, ri);
   }
   const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
+  const bool apart = by_group && job.apart();
   if (tile0 * 16 >= nq * group || (!by_group && nq > max_query)) return;      // (the same for the whole block)
   Column col[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     col[t] = column_of(a, (tile0 + t) * 16 + c, hk, group, qs, nq, n);
-    if (by_group) col[t].pos = n - 1;
+    if (by_group && col[t].valid) col[t].pos = apart ? position_in_group(a, job, col[t].token) : n - 1;
   }
-  const int pos_first = by_group ? n - 1 : n - nq + tile0 * 16 / group;            // the tiles' first and last positions
+  // the tiles' first and last positions (of a group's queries: all tiles')
+  const int pos_first = by_group ? min(job.lowest, n - 1) : n - nq + tile0 * 16 / group;
   const int pos_last = by_group ? n - 1 : n - nq + min((tile0 + NT) * 16 - 1, nq * group - 1) / group;
   const int first = max(from, first_seen(pos_first, a.window)), whole_from = max(from, first_seen(pos_last, a.window));
   // a wave's keys: an equal share of the row's, or of its block's
@@ -424,7 +458,7 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
       }
       // Where queries of the tiles see different keys, a value that is not finite reaches those alone that see it: it leaves
       // the product (zero times it is no number) and sets their sums by itself.
-      if (!whole && nq > 1 && !by_group) {
+      if (!whole && nq > 1 && (!by_group || apart)) {
         bool odd = false;
 #pragma unroll
         for (int ds = 0; ds < D / 16; ++ds)
@@ -737,10 +771,10 @@ __device__ __forceinline__ void tiles_block(const CacheArgs& a, int by_group, in
   const int f0 = tile * COLUMNS + 32 * wave, f = f0 + c;
   Column col = column_of(a, f, hk, group, qs, nq, n);
   const int behind = n - nq;                               // the first query's position
-  const int pos_first = by_group ? n - 1 : behind + tile * COLUMNS / group;
+  const int pos_first = by_group ? min(job.lowest, n - 1) : behind + tile * COLUMNS / group;
   const int pos_last = by_group ? n - 1 : behind + min(tile * COLUMNS + COLUMNS - 1, columns - 1) / group;
-  if (by_group) col.pos = n - 1;
-  const int tile_first = by_group ? n - 1 : behind + f0 / group;
+  if (by_group && col.valid) col.pos = job.apart() ? position_in_group(a, job, col.token) : n - 1;
+  const int tile_first = by_group ? pos_first : behind + f0 / group;
   const int tile_last = f0 >= columns ? -1 : by_group ? n - 1 : behind + min(f0 + 31, columns - 1) / group;
   const int first = max(from, first_seen(pos_first, a.window)), whole_from = max(from, first_seen(tile_last, a.window));
   const int from_here = max(from, first_seen(col.pos, a.window));

@@ -45,7 +45,8 @@ class AttnRows:
 @dataclasses.dataclass
 class SharedPrefix:
     """Rows of a step that begin with the same tokens: group g is rows group_start[g] .. group_start[g + 1] - 1 (neighbours; a
-    row may be in none), whose first lens[g] tokens are the same ones in the same cache pages."""
+    row may be in none), whose first lens[g] tokens are the same ones in the same cache pages. A row may be shorter than that, or
+    begin with queries inside it: they see the prefix up to themselves. The block table of a group's first row names all of its pages."""
 
     group_start: torch.Tensor            # [G+1] int32, rising
     lens: torch.Tensor                   # [G] int32

@@ -767,6 +767,61 @@ def test_attention_over_a_shared_prefix(hip, step, q8):
         _check(got, q, pages, scales, table, attn, page, d ** -0.5, 0, s)
 
 
+INSIDE = [
+    # (rows, groups, lengths instead of theirs, heads, kv heads, head size): rows no longer than the prefix, queries inside it, rows of no key
+    ([(300, 1)] * 4, [(0, 3, 288)], {1: 288, 2: 100, 3: 0}, 8, 2, 128),                                # a block a row
+    ([(1100, 1)] * 6 + [(40, 1)], [(0, 5, 1056)], {1: 1057, 2: 1056, 3: 1055, 4: 33, 5: 0, 6: 0}, 8, 2, 128),
+    ([(300, 5)] * 5, [(0, 4, 288)], {1: 292, 2: 290, 3: 4, 4: 2}, 8, 2, 64),                            # drafted tokens
+    ([(1700, 1)] * 40 + [(20, 1)] * 3, [(0, 39, 1680), (40, 42, 16)], {i: 42 * i for i in range(1, 40)}, 10, 1, 128),   # many columns, two groups
+    ([(96, 200), (100, 40), (90, 3)], [(0, 2, 80)], {0: 230, 1: 60, 2: 3}, 4, 1, 128),                  # portions
+    ([(129, 70), (128, 2), (500, 1), (140, 1)], [(0, 3, 128)], {0: 150, 2: 64, 3: 0}, 4, 2, 256),        # all kinds of rows
+    ([(4000, 1)] * 3, [(0, 2, 3984)], {0: 7, 1: 0, 2: 2100}, 4, 1, 64),                                 # none sees the whole prefix
+    ([(1300, 1)] * 20, [(0, 19, 1280)], {i: 0 for i in range(20)}, 8, 2, 128),                          # none sees any of it
+]
+
+
+@gpu
+@pytest.mark.parametrize(("q8", "dtype"), [(False, torch.bfloat16), (True, torch.bfloat16), (True, torch.float32)])
+@pytest.mark.parametrize("step", range(len(INSIDE)))
+def test_queries_inside_a_shared_prefix(hip, step, q8, dtype):
+    """A query sees the keys up to its own, in the prefix as behind it; what it does not see may hold anything, what nobody sees too."""
+    rows, shared, lens, heads, kv, d = INSIDE[step]
+    print(f"step {step} 8-bit {q8} {dtype}", flush=True)
+    q, pages, scales, table, attn, prefix = _step(rows, heads, kv, d, 16, seed=step, shared=shared, q8=q8, dtype=dtype, device="cuda")
+    for i, n in lens.items():
+        attn.lens[i] = n
+    counts, held = attn.query_start.diff().tolist(), attn.lens.tolist()
+    got = hip.prefix_attention(q, pages, table, attn, prefix, 16, d ** -0.5, scales)
+    _check(got, q, pages, scales, table, attn, 16, d ** -0.5)
+    start = attn.query_start.tolist()
+    for i, (n, count) in enumerate(zip(held, counts)):
+        assert not got[start[i]: start[i] + max(0, count - n)].any()
+    # a value of the first group's prefix that is no number: it reaches those that see it, and changes nothing for the others
+    lo, hi, most = shared[0]
+    longest = max(held[i] for i in range(lo, hi + 1))
+    at = min(most, longest) - 1
+    if at < 0:
+        return
+    if q8:
+        pages.view(torch.uint8)[table[attn.slots[lo], at // 16].long(), 1, 0].view(d, 16)[5, at % 16] = 0x7f
+    else:
+        pages[table[attn.slots[lo], at // 16].long(), 1, 0].view(d, 16)[5, at % 16] = float("nan")
+    odd = hip.prefix_attention(q, pages, table, attn, prefix, 16, d ** -0.5, scales)
+    for i, (n, count) in enumerate(zip(held, counts)):
+        for x in range(count):
+            t, sees = start[i] + x, lo <= i <= hi and n - count + x >= at
+            mine = odd[t].clone()
+            if sees:
+                assert torch.isnan(mine[: heads // kv, 5]).all()
+                mine[: heads // kv, 5] = got[t, : heads // kv, 5]
+            assert torch.equal(mine, got[t]), (i, x)
+    if at + 1 < most:                                             # what lies behind the longest row: keys, values and scales of any bytes
+        pages.view(torch.uint8)[table[attn.slots[lo], (at + 16) // 16: most // 16].long()] = 0xff
+        if q8:
+            scales.view(torch.uint8)[table[attn.slots[lo], (at + 16) // 16: most // 16].long()] = 0xff
+        assert torch.equal(hip.prefix_attention(q, pages, table, attn, prefix, 16, d ** -0.5, scales).nan_to_num(7.0), odd.nan_to_num(7.0))
+
+
 @gpu
 @pytest.mark.parametrize("q8", [False, True])
 @pytest.mark.parametrize(("d", "rows"), [(64, [(49300, 8)] * 4), (128, [(49168, 8), (49500, 8), (49169, 8), (49200, 7), (60, 3)])])
