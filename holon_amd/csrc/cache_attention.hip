@@ -32,6 +32,7 @@ struct CacheArgs {
   const int32_t* slots;        // [B]
   const int32_t* lens;         // [B]
   const int32_t* qstart;       // [B + 1]
+  int rows;                    // B
   const int32_t* row_ids;      // the rows of this launch (null: they are decode rows alone, in order)
   int n_tokens;
   int heads, kv_heads, page_size;
@@ -1016,6 +1017,8 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
     const int qs = in_order ? ri : a.qstart[row], nq = in_order ? 1 : a.qstart[row + 1] - qs;
     if (qi >= nq || nq > max_query || nq <= less_than) return;      // (a row of more queries, or of fewer, is another kernel's)
     token = qs + qi;
+  } else if (!a.budget && (token < a.qstart[0] || token >= a.qstart[a.rows])) {
+    return;                                                // a token of no row: no kernel left anything of it
   }
   if (token < 0 || token >= a.n_tokens) return;
   const int64_t first = a.budget ? place * a.heads + head : (place * a.heads + head) * a.parts;
@@ -1298,7 +1301,7 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   a.q = q; a.out = out; a.pages = (const uint8_t*)c.pages; a.scales = (const uint8_t*)c.scales;
   a.page_stride = c.page_stride; a.scale_stride = c.scale_stride; a.num_pages = c.num_pages;
   a.table = c.table; a.table_stride = c.table_stride; a.n_slots = c.n_slots;
-  a.slots = c.slots; a.lens = c.lens; a.qstart = c.qstart; a.n_tokens = (int)c.tokens;
+  a.slots = c.slots; a.lens = c.lens; a.qstart = c.qstart; a.rows = c.rows; a.n_tokens = (int)c.tokens;
   a.heads = heads; a.kv_heads = c.kv_heads; a.page_size = c.page_size;
   a.page_magic = (uint32_t)magic;
   a.scale_log2 = c.scale * 1.4426950408889634f; a.window = c.window; a.sink = c.sink;

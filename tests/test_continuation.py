@@ -731,6 +731,26 @@ def test_rows_that_see_nothing(hip):
 
 
 @gpu
+@pytest.mark.parametrize("q8", [False, True])
+def test_tokens_of_no_row_are_left_alone(hip, q8, monkeypatch):
+    """Tokens in front of the first row's and behind the last one's, in every way of cutting a call: what the result held there stays."""
+    filled = lambda t, **kw: torch.full(t.shape, 7.0, dtype=t.dtype, device=t.device)              # noqa: E731
+    monkeypatch.setattr(torch, "empty_like", filled)
+    for rows, shared in (([(300, 1)] * 4, ()), ([(300, 1)] * 4, [(0, 3, 288)]), ([(1100, 1)] * 4, [(0, 3, 1056)]), ([(300, 4)] * 3, [(0, 2, 288)]),
+                         ([(6000, 1), (40, 1)], ()), ([(100, 70), (300, 1), (30, 3)], [(0, 1, 96)]), ([(100, 70), (300, 1), (30, 3)], ()),
+                         ([(100, 70), (1300, 70)], [(0, 1, 96)])):
+        print(rows, shared, q8, flush=True)
+        q, pages, scales, table, attn, prefix = _step(rows, 8, 2, 128, 16, seed=1, shared=shared, q8=q8, device="cuda")
+        want = hip.prefix_attention(q, pages, table, attn, prefix, 16, 128 ** -0.5, scales)
+        _check(want, q, pages, scales, table, attn, 16, 128 ** -0.5)
+        wide = torch.cat((q[:1].expand(2, -1, -1), q, q[:1].expand(3, -1, -1)))
+        attn.query_start += 2
+        attn.in_order = False
+        got = hip.prefix_attention(wide, pages, table, attn, prefix, 16, 128 ** -0.5, scales)
+        assert torch.equal(got[2:-3], want) and (got[:2] == 7).all() and (got[-3:] == 7).all()
+
+
+@gpu
 @pytest.mark.parametrize("step", range(len(STEPS)))
 def test_a_bfloat16_cache_without_a_prefix(hip, step):
     rows, heads, kv, d, page, window = STEPS[step]
