@@ -1203,7 +1203,7 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
   p.any_many = n_chunk > 0 && max_chunk_query > few;
   if (p.any_many && n_chunk == 1) p.any_few = false;       // (the one row is as long as the longest)
   p.decode = cut_keys(n_decode, group, seen_span(own_decode, 1, window), 1, kv_heads, head_dim, value_bytes, f32);
-  if (one_each) p.decode.splits = p.decode.waves = (int)std::min<int64_t>(most_waves(head_dim, f32, 1), (max_decode_len + 63) / 64);
+  if (one_each) p.decode.splits = p.decode.waves = std::max(1, (int)std::min<int64_t>(most_waves(head_dim, f32, 1), ((int64_t)max_decode_len + 63) / 64));
   p.few = cut_keys(n_chunk, (int64_t)few * group, seen_span(own_chunk, few, window), few, kv_heads, head_dim, value_bytes, f32);
   p.many = cut_keys(n_chunk, std::max<int64_t>((int64_t)max_chunk_query * group, FEW_COLUMNS + 1), seen_span(own_chunk, max_chunk_query, window),
                     max_chunk_query, kv_heads, head_dim, value_bytes, f32);

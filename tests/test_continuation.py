@@ -732,6 +732,16 @@ def test_rows_that_see_nothing(hip):
 
 @gpu
 @pytest.mark.parametrize("q8", [False, True])
+def test_a_group_of_rows_of_no_key(hip, q8):
+    """All of a step's rows are empty, and the bound on their lengths says so."""
+    q, pages, scales, table, attn, prefix = _step([(40, 1)] * 3, 4, 2, 64, 16, shared=[(0, 2, 32)], q8=q8, device="cuda")
+    attn.lens.zero_()
+    attn.max_decode_len = 0
+    assert not hip.prefix_attention(q, pages, table, attn, prefix, 16, 0.125, scales).any()
+
+
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
 def test_tokens_of_no_row_are_left_alone(hip, q8, monkeypatch):
     """Tokens in front of the first row's and behind the last one's, in every way of cutting a call: what the result held there stays."""
     filled = lambda t, **kw: torch.full(t.shape, 7.0, dtype=t.dtype, device=t.device)              # noqa: E731

@@ -35,3 +35,16 @@ def test_heads_that_go_to_the_kernel_of_many_columns_are_not_cut_by_lengths(lib,
             share = rows * heads * (dim + 2) * 4
             room = _room(lib, heads, kv, dim, decode=(rows, longest), q8=q8)
             assert room % share == 0 and room // share <= 32, (rows, longest, room)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("q8", [True, False])
+def test_every_bound_has_a_plan(lib, q8, f32):
+    """Bounds that the entry point takes: no rows, rows of no key, groups of no key or no query, and more than there is."""
+    if f32 and not q8:
+        return
+    for heads, kv, dim in ((1, 1, 64), (8, 2, 128), (20, 1, 256), (71, 1, 64)):
+        for decode in ((0, 0), (1, 0), (2, 0), (40, 0), (3, 1), (1, 1 << 30)):
+            for chunk in ((0, 0, 0), (1, 1, 0), (2, 2, 0), (3, 500, 1 << 30)):
+                for group in ((0, 0, 0), (1, 0, 0), (1, 2, 0), (1, 0, 16), (1, 2, 16), (2, 600, 1 << 30)):
+                    assert _room(lib, heads, kv, dim, decode=decode, chunk=chunk, group=group, q8=q8, f32=f32) >= 0
