@@ -1263,6 +1263,10 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
   return p;
 }
 
+// Floats of scratch for the partial sums of so many cells (and, where rows are cut by their lengths, `listed` rows' shares): whole
+// pieces of 16 bytes, so that what follows begins on a border for its vectors.
+int64_t room_of(int64_t cells, int head_dim, int listed) { return (cells * (head_dim + 2) + 2 * (int64_t)listed + 3) / 4 * 4; }
+
 }  // namespace
 
 static Plan plan_of(const HolonCacheAttention& c) {
@@ -1274,7 +1278,8 @@ extern "C" int64_t holon_cache_attention_room(const HolonCacheAttention* call) {
   const HolonCacheAttention& c = *call;
   if (c.kv_heads <= 0 || c.heads < c.kv_heads) return 0;   // (refused by the call that follows)
   const Plan p = plan_of(c);
-  return ((p.decode_cells + p.few_cells + p.many_cells) * (c.head_dim + 2) + (p.decode.budget ? 2 * (int64_t)c.n_decode : 0)) * (int64_t)sizeof(float);
+  return (room_of(p.decode_cells, c.head_dim, p.decode.budget ? c.n_decode : 0) + room_of(p.few_cells, c.head_dim, 0) +
+          room_of(p.many_cells, c.head_dim, 0)) * (int64_t)sizeof(float);
 }
 
 extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void* q, void* out, void* room, void* stream) {
@@ -1347,9 +1352,8 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
     if (p.by_token) return;
     a.parts = cut.parts(); a.cell_queries = most;
     a.part_o = at; a.part_ml = at + cells * head_dim;
-    at += cells * (head_dim + 2);
-    a.row_parts = (int2*)at;
-    if (cut.budget) at += 2 * n_rows;
+    a.row_parts = (int2*)(at + cells * (head_dim + 2));
+    at += room_of(cells, head_dim, cut.budget ? n_rows : 0);
   };
   const auto join = [&](int n_rows, int most, int less_than) {
     if (!p.by_token && a.parts > 1) merge(most, less_than, (int64_t)n_rows * most * heads);

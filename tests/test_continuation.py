@@ -497,6 +497,17 @@ def test_more_heads_on_one_behind_long_contexts(hip, heads, kv, d, q8):
         _check(got, q, pages, scales, table, attn, 16, d ** -0.5)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(("heads", "d"), [(5, 64), (3, 256)])
+def test_rows_of_every_kind_are_cut_in_one_call(hip, heads, d, dtype):
+    """Decode rows cut by their lengths and rows of a few queries, odd numbers of heads and rows: each kind's partial sums lie on borders."""
+    rows = [(5000, 1), (300, 3), (6000, 1), (4100, 5), (7000, 1), (37, 1), (2500, 2)]
+    q, pages, scales, table, attn, _ = _step(rows, heads, 1, d, 16, seed=heads, dtype=dtype, device="cuda")
+    got = hip.paged_attention_q8(q, pages, scales, table, attn, 16, d ** -0.5)
+    _check(got, q, pages, scales, table, attn, 16, d ** -0.5)
+
+
 BESIDE = [
     # (rows, heads, kv heads, head size, page, window): decode rows of short contexts and long beside portions, rows of a few queries between
     ([(5000, 1), (37, 1), (9000, 1), (10, 1), (200, 70)], 8, 2, 128, 16, 0),

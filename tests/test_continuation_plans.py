@@ -34,7 +34,7 @@ def test_heads_that_go_to_the_kernel_of_many_columns_are_not_cut_by_lengths(lib,
         for longest in (4096, 4097, 8192, 100000):
             share = rows * heads * (dim + 2) * 4
             room = _room(lib, heads, kv, dim, decode=(rows, longest), q8=q8)
-            assert room % share == 0 and room // share <= 32, (rows, longest, room)
+            assert room % share < 16 and room // share <= 32, (rows, longest, room)       # (whole pieces of 16 bytes)
 
 
 @pytest.mark.parametrize("f32", [False, True])
@@ -48,3 +48,15 @@ def test_every_bound_has_a_plan(lib, q8, f32):
             for chunk in ((0, 0, 0), (1, 1, 0), (2, 2, 0), (3, 500, 1 << 30)):
                 for group in ((0, 0, 0), (1, 0, 0), (1, 2, 0), (1, 0, 16), (1, 2, 16), (2, 600, 1 << 30)):
                     assert _room(lib, heads, kv, dim, decode=decode, chunk=chunk, group=group, q8=q8, f32=f32) >= 0
+
+
+def test_scratch_is_in_whole_pieces_of_16_bytes(lib):
+    """Partial sums are vectors of 16 bytes: those of a step's further kinds of rows begin behind the others', on a border."""
+    rooms = set()
+    for heads, kv, dim in ((1, 1, 64), (5, 1, 64), (3, 3, 128), (7, 1, 256)):
+        for rows in (1, 3, 5):
+            for longest in (5000, 7000, 9000, 30000):
+                rooms |= {_room(lib, heads, kv, dim, decode=(rows, longest), q8=q8, f32=f32) for q8, f32 in ((True, False), (False, False), (True, True))}
+                rooms |= {_room(lib, heads, kv, dim, decode=(rows, longest), chunk=(rows, most, longest)) for most in (3, 5, 400)}
+                rooms.add(_room(lib, heads, kv, dim, decode=(rows, longest), group=(1, rows, longest)))
+    assert len(rooms) > 50 and all(room % 16 == 0 for room in rooms)
