@@ -2,11 +2,12 @@
 // start[b + 1] - 1 of the logits; row i judges drafted[i], the last one has none behind it. With p = softmax(logits / T) and q the
 // distribution that the draft came from (given, or certainty):
 //
-//   row i takes its draft x when accept[i] q(x) <= p(x);   after the first that does not (or the last row) one token is drawn:
+//   row i takes its draft x when accept[i] q(x) < p(x);   after the first that does not (or the last row) one token is drawn:
 //   from max(p - q, 0), renormalised, where a draft was turned down, from p where none was judged,
 //   the first x with sum_{y <= x} mass(y) > draw[b] * sum mass.
 //
-// So a token's law is p whatever q is. T = 0 takes the largest logit for p. The draw compares a running sum over up to hundreds
+// So a token's law is p whatever q is: accept lies in [0, 1), where it is below p(x) / q(x) with that probability (1 at most), and never
+// where p(x) = 0, at accept[i] = 0 and q(x) = 0 too: what a mask has set to -inf does not come out. T = 0 takes the largest logit for p. The draw compares a running sum over up to hundreds
 // of thousands of masses with a given number: exponentials and sums are in 64 bits, where the order of a sum moves a border
 // between two tokens by 1e-16 of the whole, not by more than a token's own mass as in 32.
 //
@@ -259,7 +260,7 @@ __device__ __forceinline__ Judged judge(const Request& r, int b) {
     const int64_t at = (int64_t)row * r.vocab + (may ? x : 0);
     const float lx = r.logits[at], qx = r.draft_probs != nullptr ? r.draft_probs[at] : 1.f, u = r.accept[row];
     const RowPart w = whole_row(r.parts + (int64_t)row * r.pieces, r.pieces, c);
-    const bool good = c > 0.0 ? (double)u * (double)qx * w.sum <= Weight(w.max, c)(lx) : x == (w.at == NONE ? 0 : w.at);
+    const bool good = c > 0.0 ? (double)u * (double)qx * w.sum < Weight(w.max, c)(lx) : x == (w.at == NONE ? 0 : w.at);
     if (lane == 0) {
       whole[i] = w;
       verdict[i] = may ? (good ? 1 : 0) : -1;

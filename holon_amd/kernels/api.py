@@ -244,12 +244,13 @@ class Kernels(Protocol):
         """Drafted tokens judged against the target's probabilities from given random numbers. Request b (of B) owns rows start[b]
         .. start[b + 1] - 1 (start [B+1] int32) of logits [N, V] float32: row i judges drafted[i] ([N] int32), the last row none.
         p = softmax(logits / temperature[b]), q = draft_probs[i] ([N, V] float32; None: the drafts were certain). Row i takes its
-        draft x when accept[i] q(x) <= p(x); behind the drafts taken one more token is drawn: from max(p - q, 0) where a draft was
-        turned down (where that leaves nothing: from p), from p otherwise: the first whose running sum exceeds draw[b] times the
-        whole. accept [N] and draw [B] float32 lie in [0, 1). Temperature 0 (or less): p is the first largest logit. A drafted id
-        outside the vocabulary is no draft: the row draws from p. Sums and exponentials in 64 bits; a logit that is NaN has no
-        mass; a row without any gives token 0. -> (tokens [B, most + 1] int32: those taken, the drawn one, then -1; how many were
-        taken [B] int32); a request of no rows gets -1 and 0, of its rows only the first most + 1 (at most 64) count."""
+        draft x when accept[i] q(x) < p(x) (never one of probability 0); behind the drafts taken one more token is drawn: from
+        max(p - q, 0) where a draft was turned down (where that leaves nothing: from p), from p otherwise: the first whose running
+        sum exceeds draw[b] times the whole. accept [N] and draw [B] float32 lie in [0, 1). Temperature 0 (or less): p is the first
+        largest logit. A drafted id outside the vocabulary is no draft: the row draws from p. Sums and exponentials in 64 bits; a
+        logit that is NaN has no mass; a row without any gives token 0. -> (tokens [B, most + 1] int32: those taken, the drawn
+        one, then -1; how many were taken [B] int32); a request of no rows gets -1 and 0, of its rows only the first most + 1 (at
+        most 64) count."""
 
     def scatter_rows(self, dst: torch.Tensor, idx: torch.Tensor, src: torch.Tensor) -> None:
         """dst[idx[r]] = src[r] for int32 rows: dst [N, W], idx [n], src n * W values."""

@@ -317,7 +317,7 @@ class TorchKernels:
                 judged = i + 1 < rows.stop and 0 <= draft < vocab
                 q = draft_probs[i].double() if draft_probs is not None else torch.nn.functional.one_hot(
                     torch.tensor(max(0, min(draft, vocab - 1))), vocab).to(p)
-                good = judged and (float(accept[i]) * float(q[draft]) <= float(p[draft]) if heat > 0 else float(p[draft]) == 1)
+                good = judged and (float(accept[i]) * float(q[draft]) < float(p[draft]) if heat > 0 else float(p[draft]) == 1)
                 if good:
                     tokens[b, taken] = draft
                     taken += 1

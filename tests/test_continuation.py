@@ -931,6 +931,35 @@ def test_verify_at_the_borders(hip):
     assert _verify(hip, same)[1].sum() >= 14
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("probs", [True, False])
+def test_a_draft_of_probability_0_is_never_taken(request, device, probs):
+    """Tokens that a mask has set to -inf, that are no number, or lie in a row without mass are turned down whatever was drawn against
+    them, 0 too and where the draft's own probability is 0; what comes out instead has mass. A draft of probability 0 that the target
+    allows is taken. Held to the definition: accept is uniform in [0, 1), so P(accept q < p) = min(1, p / q)."""
+    ops = PLAIN if device == "cpu" else request.getfixturevalue("hip")
+    vocab, n = 5000, 8
+    logits = torch.randn(2 * n, vocab, generator=torch.Generator().manual_seed(3))
+    drafted = torch.arange(2 * n, dtype=torch.int32) * 311
+    q = torch.full((2 * n, vocab), 1.0 / vocab)
+    accept, rows = torch.zeros(2 * n), torch.arange(n) * 2        # request b judges row 2 b
+    accept[rows[1]] = accept[rows[4]] = accept[rows[5]] = 0.5
+    for b in (0, 1, 2):
+        logits[rows[b], drafted[rows[b]]] = float("-inf")
+    q[rows[1], drafted[rows[1]]] = q[rows[2], drafted[rows[2]]] = 0.0
+    logits[rows[3], drafted[rows[3]]] = float("nan")
+    logits[rows[4]], logits[rows[5]] = float("-inf"), float("nan")                       # no mass at all
+    q[rows[6], drafted[rows[6]]] = 0.0                                                   # rows 6, 7: allowed, and drawn against with 0
+    case = dict(logits=logits, drafted=drafted, draft_probs=q if probs else None, accept=accept, draw=torch.rand(n, generator=torch.Generator().manual_seed(4)),
+                temperature=torch.ones(n), start=torch.arange(0, 2 * n + 1, 2, dtype=torch.int32), most=1)
+    tokens, taken = (x.cpu().tolist() for x in ops.verify_drafts(**{k: x.to(device) if torch.is_tensor(x) else x for k, x in case.items()}))
+    assert taken == [0] * 6 + [1, 1]
+    for b in range(4):
+        assert tokens[b][0] != int(drafted[rows[b]]) and logits[rows[b], tokens[b][0]] > float("-inf") and tokens[b][1] == -1
+    assert tokens[4] == tokens[5] == [0, -1]
+    assert [tokens[b][0] for b in (6, 7)] == drafted[rows[6:]].tolist()
+
+
 @gpu
 @pytest.mark.parametrize("probs", [True, False])
 def test_verify_where_little_is_left(hip, probs):
