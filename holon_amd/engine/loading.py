@@ -60,9 +60,11 @@ def build_from_spec(spec: ModelSpec, *, device: torch.device, dtype: torch.dtype
                   cache_format=cache_format)
     model = build_model(spec, build)
     if cache_format == "q8":
-        others = sorted({d.name for decls in model.state_decls() for d in decls if hasattr(d, "elems") and d.dtype is not torch.uint8})
-        if others:
-            raise ValueError(f"cache_format q8 is served by grouped-query attention alone: this model also keeps {', '.join(others)}")
+        paged = [d for decls in model.state_decls() for d in decls if hasattr(d, "elems")]
+        others = sorted({d.name for d in paged if d.dtype is not torch.uint8})
+        if others or not paged:
+            raise ValueError("cache_format q8 is served by grouped-query attention alone: this model "
+                             + (f"also keeps {', '.join(others)}" if others else "keeps no keys and values"))
     return model, build
 
 

@@ -138,3 +138,19 @@ def test_what_it_refuses():
     for config in (dopirax_models.CONFIG_A, falisun_models.CONFIG_A):                # other attention keeps its own state, in its own types
         with pytest.raises(ValueError, match="cache_format q8 is served by grouped-query attention alone"):
             load_model("", device="cpu", dtype="float32", kernels=TorchKernels(), cache_format="q8", random_config=config)
+
+
+def test_models_without_keys_and_values_are_refused():
+    """A model that keeps nothing by token has no cache whose format could be asked for."""
+    from holon_amd.registry import register_architecture, register_part, unregister_architecture, unregister_part
+    from tests.toy_parts import GridRunningMean, ToyConfig, toy_recipe
+    config = {"architectures": ["ToyGridModel"], "width": 48, "tokens": 61, "depth": 2, "grid": 8, "eps": 1e-5}
+    register_part("mixer", "test-grid-mean")(GridRunningMean)
+    register_architecture("ToyGridModel", ToyConfig, toy_recipe)
+    try:
+        load_model("", device="cpu", dtype="float32", kernels=TorchKernels(), random_config=config)
+        with pytest.raises(ValueError, match="keeps no keys and values"):
+            load_model("", device="cpu", dtype="float32", kernels=TorchKernels(), cache_format="q8", random_config=config)
+    finally:
+        unregister_part("mixer", "test-grid-mean")
+        unregister_architecture("ToyGridModel")
