@@ -203,11 +203,14 @@ class ContinuationOps:
             groups, most, longest = prefix.n_groups, prefix.max_queries, prefix.max_len
             starts_at = _ints(what, "group_start", prefix.group_start, groups + 1, device)
             lens_at = _ints(what, "prefix lens", prefix.lens, groups, device)
-        packed = _ATTENTION.pack(
-            at, to or 0, table.data_ptr(), _ints(what, "slots", slots, b, device), _ints(what, "lens", rows.lens, b, device),
-            _ints(what, "query_start", rows.query_start, b + 1, device), decode, chunk, starts_at, lens_at, sink_at, step, gap, t,
-            n, held[1], held[0], b, n_decode, rows.max_decode_len, n_chunk, rows.max_chunk_query, rows.max_chunk_len, groups, most, longest,
-            heads, kv, dim, page_size, int(window), _DT[dtype], scale)
+        try:
+            packed = _ATTENTION.pack(
+                at, to or 0, table.data_ptr(), _ints(what, "slots", slots, b, device), _ints(what, "lens", rows.lens, b, device),
+                _ints(what, "query_start", rows.query_start, b + 1, device), decode, chunk, starts_at, lens_at, sink_at, step, gap, t,
+                n, held[1], held[0], b, n_decode, rows.max_decode_len, n_chunk, rows.max_chunk_query, rows.max_chunk_len, groups, most, longest,
+                heads, kv, dim, page_size, int(window), _DT[dtype], scale)
+        except (struct.error, OverflowError) as error:
+            _fail(f"{what}: sizes, bounds and the window are whole numbers of 32 bits, the scale a float32 ({error})")
         out = torch.empty_like(q)
         room = self.lib.holon_cache_attention_room(packed)
         space = torch.empty((room,), dtype=torch.uint8, device=q.device) if room else None

@@ -263,6 +263,23 @@ def test_refused_caches_and_rows():
     assert len(ops.launched) == 5
 
 
+def test_refused_bounds_past_32_bits():
+    ops = Refusing()
+    q, pages, scales, table, rows, prefix = _step([(40, 1), (41, 3)], 4, 2, 64, 16, shared=[(0, 1, 32)])
+    more = lambda x, **kw: type(x)(**{**vars(x), **kw})                                             # noqa: E731
+    ops.paged_attention_q8(q, pages, scales, table, rows, 16, 0.1, 2 ** 31 - 1)
+    for bad in (lambda: ops.paged_attention_q8(q, pages, scales, table, rows, 16, 0.1, 2 ** 31),
+                lambda: ops.paged_attention_q8(q, pages, scales, table, rows, 16, 0.1, -2 ** 31 - 1),
+                lambda: ops.paged_attention_q8(q, pages, scales, table, rows, 16, 1e39),
+                lambda: ops.paged_attention_q8(q, pages, scales, table, more(rows, max_decode_len=2 ** 31), 16, 0.1),
+                lambda: ops.paged_attention_q8(q, pages, scales, table, more(rows, max_chunk_query=2 ** 40), 16, 0.1),
+                lambda: ops.prefix_attention(q, pages, table, rows, more(prefix, max_len=2 ** 31), 16, 0.1, scales),
+                lambda: ops.prefix_attention(q, pages, table, rows, more(prefix, max_queries=2.5), 16, 0.1, scales)):
+        with pytest.raises(KernelError, match="32 bits"):
+            bad()
+    assert len(ops.launched) == 1
+
+
 def test_refused_caches_without_scales():
     """A bfloat16 cache has pages of the same shape: without scales it is no 8-bit cache."""
     ops, at = Refusing(), torch.zeros(5, dtype=torch.int32)
