@@ -1309,7 +1309,9 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   a.slots = c.slots; a.lens = c.lens; a.qstart = c.qstart; a.rows = c.rows; a.n_tokens = (int)c.tokens;
   a.heads = heads; a.kv_heads = c.kv_heads; a.page_size = c.page_size;
   a.page_magic = (uint32_t)magic;
-  a.scale_log2 = c.scale * 1.4426950408889634f; a.window = c.window; a.sink = c.sink;
+  a.scale_log2 = c.scale * 1.4426950408889634f; a.sink = c.sink;
+  // (a query may lie up to 65,534 positions in front of the sequence, and what it sees begins a window before that: see first_seen)
+  a.window = std::min(std::max(c.window, -0x7fffffff), 0x7fffffff - 0x10000);
   const Plan p = plan_of(c);
   float* at = (float*)room;
   const Launch w{(hipStream_t)stream, q8, dtype};

@@ -759,6 +759,19 @@ def test_rows_that_see_nothing(hip):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_windows_and_chunks_as_wide_as_there_are(hip, dtype):
+    """The widest windows hide nothing, from queries in front of the sequence and their neighbours neither."""
+    q, pages, scales, table, attn, _ = _step([(9, 1), (12, 8), (30, 90)], 4, 2, 64, 16, dtype=dtype, device="cuda")
+    attn.lens[1], attn.lens[2] = 2, 40                            # eight queries of a sequence of two tokens, 90 of one of 40
+    want = hip.paged_attention_q8(q, pages, scales, table, attn, 16, 0.125)
+    assert not want[1:7].any() and want[7:9].any() and not want[9:59].any() and want[59:].any()
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, -2 ** 30, 1 - 2 ** 31, -2 ** 31):
+        print(window, flush=True)
+        assert torch.equal(hip.paged_attention_q8(q, pages, scales, table, attn, 16, 0.125, window), want)
+
+
+@gpu
 @pytest.mark.parametrize("q8", [False, True])
 def test_a_group_of_rows_of_no_key(hip, q8):
     """All of a step's rows are empty, and the bound on their lengths says so."""
