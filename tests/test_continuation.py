@@ -838,6 +838,34 @@ def test_attention_over_a_shared_prefix(hip, step, q8):
         _check(got, q, pages, scales, table, attn, page, d ** -0.5, 0, s)
 
 
+@gpu
+@pytest.mark.parametrize("step", range(len(SHARED)))
+def test_float32_queries_over_a_shared_prefix(hip, step):
+    rows, shared, heads, kv, d, page = SHARED[step]
+    print(f"step {step}", flush=True)
+    q, pages, scales, table, attn, prefix = _step(rows, heads, kv, d, page, seed=step, shared=shared, dtype=torch.float32, device="cuda")
+    sink = torch.linspace(-2, 3, heads).cuda()
+    for s in (None, sink):
+        got = hip.prefix_attention(q, pages, table, attn, prefix, page, d ** -0.5, scales, s)
+        _check(got, q, pages, scales, table, attn, page, d ** -0.5, 0, s)
+
+
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize(("groups", "queries"), [(63, 1), (64, 1), (65, 1), (140, 1), (70, 3)])
+def test_many_groups(hip, groups, queries, q8):
+    """More groups than a wave has lanes: a row finds its own, one that is in none finds none."""
+    rows, shared = [], []
+    for i in range(groups):
+        whole = 16 * (1 + i % 3)
+        rows += [(whole + j + i % 5, queries) for j in range(2 + i % 3)]
+        shared.append((len(rows) - 2 - i % 3, len(rows) - 1, whole))
+    rows.append((33, queries))
+    q, pages, scales, table, attn, prefix = _step(rows, 4, 4, 64, 16, seed=groups, shared=shared, q8=q8, device="cuda")
+    got = hip.prefix_attention(q, pages, table, attn, prefix, 16, 0.125, scales)
+    _check(got, q, pages, scales, table, attn, 16, 0.125)
+
+
 INSIDE = [
     # (rows, groups, lengths instead of theirs, heads, kv heads, head size): rows no longer than the prefix, queries inside it, rows of no key
     ([(300, 1)] * 4, [(0, 3, 288)], {1: 288, 2: 100, 3: 0}, 8, 2, 128),                                # a block a row
@@ -1013,6 +1041,24 @@ def test_verify_where_little_is_left(hip, probs):
                 draw=torch.tensor([0.0, 1.0 - 2.0 ** -24] * len(others)), temperature=torch.ones(2 * len(others)), start=start, most=1)
     want = _verify(hip, case)
     assert (want[1] == 0).all() and (want[0][:, 0] != drafted[0]).all()
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [262145, 262208, 600001])
+@pytest.mark.parametrize("probs", [True, False])
+def test_verify_over_many_pieces(hip, vocab, probs):
+    """Vocabularies of more than 64 pieces of 4,096: tokens drawn from the first of them, from behind 64 and from the very last, and rows
+    whose largest logit lies there."""
+    for seed, draw in ((0, (0.0, 0.5, 0.999, 1.0 - 2.0 ** -24)), (1, (0.97, 0.3, 1.0 - 2.0 ** -24, 0.9))):
+        case = _drafts([3, 1, 2, 3], vocab, seed, probs=probs, spread=1.0)
+        case["draw"][:] = torch.tensor(draw)
+        _verify(hip, case)
+        case["logits"][:, 64 * 4096:] += 30.0                      # all that matters lies behind 64 pieces
+        case["temperature"][2] = 0.0
+        want = _verify(hip, case)[0][case["draw"] > 0]               # (a number of 0 draws the first token of any mass)
+        assert ((want >= 64 * 4096) | (want == -1)).all()
+        case["logits"][:, : vocab - 2] = float("-inf")
+        assert set(_verify(hip, case)[0].flatten().tolist()) <= {-1, vocab - 2, vocab - 1}
 
 
 @gpu
