@@ -1144,9 +1144,11 @@ Cut cut_keys(int jobs, int64_t columns, int64_t span, int64_t queries, int kv_he
   if (columns > FEW_COLUMNS && !f32) {
     // Blocks of 256 columns (a stage is brought in once for twice the columns; one block a compute unit) where there is one for every
     // unit and the first ones' walks are not much shorter than the last ones', or two. Heads 32 over 8 of 128, us, 128 columns | 256:
-    // 4,096 tokens behind 28,672 3,000 | 2,783, 2,048 behind 6,144 359 | 347, a whole prompt of 2,048 81 | 91.
+    // 4,096 tokens behind 28,672 2,710 | 2,492 (bfloat16 2,506 | 2,192), 2,048 behind 6,144 332 | 339 (306 | 296), a whole prompt of 2,048
+    // 82 | 93 (73 | 82), of 8,192 737 | 716 (679 | 625). Heads of 64: over codes 4,096 behind 28,672 1,923 | 1,715, 2,048 behind 6,144 234 |
+    // 233, a whole prompt of 8,192 528 | 491; over bfloat16, whose stages cost no widening, never: 1,600 | 1,722, 213 | 234, 394 | 490.
     const int64_t wide = units * ((columns + 255) / 256);
-    r.waves = head_dim <= 128 && (wide >= 512 || (wide >= 256 && 2 * queries <= span)) ? 8 : 4;
+    r.waves = head_dim <= 128 && (head_dim > 64 || value_bytes == 1) && (wide >= 512 || (wide >= 256 && 2 * queries <= span)) ? 8 : 4;
     r.tiles = (int)((columns + 32 * r.waves - 1) / (32 * r.waves));
     const int64_t want = std::max<int64_t>(1, 2048 / r.waves / (units * r.tiles));      // two waves a SIMD
     r.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (span + 127) / 128));
