@@ -1245,10 +1245,19 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
     // Rows of long contexts are cut by their lengths. In equal numbers of shares | by lengths, us in a graph, 32 heads over 8 of 128, 8
     // bits: 32,768 and seven of 500 keys 40 | 29, 32,768 and fifteen of 500 67 | 31, 16,384 and 47 of 700 83 | 33, eight of 11,000 to 32,768 80 |
     // 79; all alike, eight of 32,768 109 | 112, 32 of 4,096 51 | 51; where rows are short, 900 to 4,096, 12 | 16.
-    // A portion's blocks and the decode rows in one launch. Two | one, us in a graph, 8 bits, 32 heads over 8 of 128: a portion of 2,048 behind
-    // 6,144 and seven rows of 8,000 364 | 341, 512 behind 28,672 and 16 of 4,096 373 | 351, 256 and 32 of 1,000 36 | 27, 128 and one of 300
-    // 19 | 12; where the decode rows are most of the step, 512 behind 2,000 and 64 of 4,096 167 | 172 (16 over 8 of 64, bfloat16 135 | 144).
-    p.beside = p.any_decode && p.any_many && group <= 16 && !f32;
+    // A portion's blocks and the decode rows in one launch, but where the decode rows are most of a long step (their blocks then run at a
+    // portion's occupancy). Two | one, us in a graph, over codes: 32 heads over 8 of 128, a portion of 2,048 behind 6,144 and seven rows of
+    // 8,000 364 | 341, 512 behind 28,672 and 16 of 4,096 373 | 351, 256 and 32 of 1,000 36 | 27, 128 and one of 300 19 | 12; 128 behind 8,000
+    // and 64 of 4,096 155 | 161, 16 over 8 of 64, 32 of 16,384 136 | 150. No line in a step's bytes and operations is much sooner there: 0.5%
+    // from the best on average over 192 steps, 10% at most. Over bfloat16 (32 over 8 of 128, then of 64): 512 behind 28,672 and 16 of 4,096
+    // 370 | 344, 243 | 222; 128 behind 8,000 and 64 of 4,096 235 | 247, 131 | 143, behind 2,000 220 | 231, 120 | 141. At heads of 256 (16 over 2)
+    // the joined kernel's tiles are slower: 2,048 behind 28,672 and eight of 1,000 1,514 | 1,608, a whole prompt of 2,048 and 16 of 4,096
+    // 148 | 128. By this rule 0.4 and 0.6% from the best on average over 216 and 48 steps, 9% at most; always joined 1.2 and 2.9%, 21%.
+    const double keys = 2.0 * value_bytes * n_decode * kv_heads * head_dim * seen_span(max_decode_len, 1, window);       // bytes
+    const double work = 4.0 * n_chunk * max_chunk_query * heads * head_dim *                                             // operations
+                        std::min(seen_span(max_chunk_len, max_chunk_query, window), std::max((int64_t)max_chunk_len - max_chunk_query / 2, (int64_t)1));
+    const bool pays = value_bytes == 1 || (head_dim < 256 ? keys <= std::max(3e8, work / 15) : keys <= 1.5e8 && work <= 4e10);
+    p.beside = p.any_decode && p.any_many && group <= 16 && !f32 && pays;
     if (p.beside) {                                        // (in blocks of the portion's size)
       p.decode.splits = p.decode.parts() * p.many.waves;
       p.decode.waves = p.many.waves;

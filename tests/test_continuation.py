@@ -553,6 +553,31 @@ def test_decode_rows_beside_portions(hip, case):
 
 
 @gpu
+def test_kinds_of_rows_in_launches_of_their_own(hip):
+    """Steps whose decode rows and portions are not joined (heads of 256 over a bfloat16 cache, a long portion): each kind of rows gets
+    what it gets alone, and they are joined where that is little."""
+    for portion, together in (((8000, 700), False), ((100, 70), True)):
+        rows = [(4000, 1), (37, 1), portion, (900, 1)]
+        print(rows, flush=True)
+        q, pages, _, table, attn, _ = _step(rows, 16, 2, 256, 16, seed=1, q8=False, device="cuda")
+        run = lambda q, attn: hip.prefix_attention(q, pages, table, attn, None, 16, 256 ** -0.5)     # noqa: E731
+        got, alone = run(q, attn), []
+        starts = attn.query_start.tolist()
+        for kind in ([0, 1, 3], [2]):
+            at = torch.tensor(kind, device="cuda")
+            tokens = torch.cat([torch.arange(starts[i], starts[i + 1]) for i in kind]).cuda()
+            count = attn.query_start.diff()[at]
+            start, order = torch.cat((count[:1] * 0, count.cumsum(0))).int(), torch.arange(len(kind), dtype=torch.int32, device="cuda")
+            none, decode = order[:0], len(kind) == 3
+            mine = AttnRows(attn.slots[at], attn.lens[at], start, order if decode else none, none if decode else order, 3 * decode, 1 - decode,
+                            attn.max_decode_len * decode, attn.max_chunk_query * (1 - decode), attn.max_chunk_len * (1 - decode))
+            alone.append((got[tokens], run(q[tokens], mine)))
+        assert all(torch.equal(x, y) for x, y in alone) or together
+        if together:
+            _check(got, q, pages, None, table, attn, 16, 256 ** -0.5)
+
+
+@gpu
 def test_nothing_to_do(hip):
     """Calls of no token, no row, no request: results of their shapes, and nothing is touched."""
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
