@@ -1190,9 +1190,13 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
   Plan p;
   const int group = heads / kv_heads;
   p.any_shared = n_groups > 0 && max_group_query > 0 && max_group_len > 0;
-  // Decode rows that one block each serves read their prefix themselves, from L2, while the GPU has room for all blocks: one launch
-  // for two. (A wave has half as much more than above: the other side has a merge in any case.)
-  const int64_t alone = (int64_t)16384 * most_waves(head_dim, f32, 1) * 3 / 2;
+  // Decode rows that one block each serves read their prefix themselves, from L2, while the GPU has room for all blocks and a row's keys
+  // are 192 KB at most: one launch for two. Two (the groups' and the rows', the merge) | one, four rows, us in a graph, where the merge's own
+  // launch costs least (not recorded, two take 15 us at least); keys behind | us: 32 heads over 8 of 128, codes 256 9.8 | 7.5, 768 10.8 | 10.8,
+  // 1,536 12.1 | 16.4, float32 queries 256 17 | 9, 1,536 23 | 22, bfloat16 256 10.9 | 8.1, 768 11.9 | 13.2; 16 over 8 of 64, codes 256 8.4 | 5.8,
+  // 1,536 10.4 | 10.2, 2,560 11.7 | 13.3, float32 queries 1,536 21 | 14, bfloat16 1,024 10.3 | 9.8, 1,536 11.0 | 12.0; 16 over 2 of 256, codes
+  // 256 18.6 | 10.5, 768 19.2 | 18.1, 1,024 19.9 | 21.7, float32 queries 512 22 | 19, 1,024 24 | 29, bfloat16 384 18.0 | 15.5, 640 19.2 | 21.4.
+  const int64_t alone = 192 * 1024;
   const bool one_each = p.any_shared && n_chunk == 0 && group <= 16 && (int64_t)n_decode * kv_heads <= 256 &&
                         (int64_t)max_decode_len * head_dim * value_bytes <= alone;
   if (one_each) p.any_shared = false;
@@ -1221,7 +1225,8 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
       const int64_t units = (int64_t)n_groups * kv_heads;
       if (p.shared.tiles) {                                // one block a compute unit, the rows' blocks beside them
         // Blocks of 256 columns, if they are full, over long prefixes. 128 columns | 256, us, 64 rows of 32 heads over 8 of 128 with 256 keys of
-        // their own, bfloat16: behind 16,384 61 | 71, 32,768 89 | 93, 65,536 151 | 121, 131,072 276 | 215.
+        // their own, bfloat16: behind 16,384 55 | 67, 32,768 82 | 85, 49,152 110 | 107, 65,536 141 | 127, 131,072 253 | 211; of heads of 64
+        // 44 | 51, 62 | 65, 81 | 79, 102 | 92, 180 | 150, over codes 45 | 52, 66 | 66, 88 | 80, 110 | 94, 198 | 150.
         const int64_t columns = (int64_t)max_group_query * group;
         p.shared.waves = max_group_len >= 49152 && (columns + 255) / 256 * 2 == (columns + 127) / 128 ? 8 : 4;
         p.shared.tiles = (int)((columns + 32 * p.shared.waves - 1) / (32 * p.shared.waves));
