@@ -32,7 +32,6 @@ struct CacheArgs {
   const int32_t* slots;        // [B]
   const int32_t* lens;         // [B]
   const int32_t* qstart;       // [B + 1]
-  int rows;                    // B
   const int32_t* row_ids;      // the rows of this launch (null: they are decode rows alone, in order)
   int n_tokens;
   int heads, kv_heads, page_size;
@@ -51,6 +50,7 @@ struct CacheArgs {
   const int32_t* group_start;
   const int32_t* group_lens;
   int n_groups;
+  int rows;                    // B. (Here, where the struct ended in a gap: eight more bytes of it took the merge of 64 rows from 8 to 13 us.)
 };
 
 // The page that a position lies in: position / page_size, by a product (a division is forty vector instructions, also where every
@@ -91,7 +91,7 @@ __device__ __forceinline__ int wave_least(int v) {
 // no longer than the prefix, or begins with queries inside it: `lowest` is the smallest position of a group's query, n no more than the
 // largest and one. (Lengths and starts of 64 rows are loaded together, beside the group's own: no chain of loads gets longer.)
 struct Job {
-  int row, qs, nq, n, from, end, lowest;
+  int row, slot, qs, nq, n, from, end, lowest;             // slot: the block table's row
   __device__ __forceinline__ bool apart() const { return lowest < n - 1; }      // (of a group) some query does not see all n keys
 };
 __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) {
@@ -102,6 +102,7 @@ __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) 
     j.end = a.group_start[at + 1];
     j.qs = a.qstart[j.row];
     j.n = a.group_lens[at];
+    j.slot = a.slots[min(j.row, a.rows - 1)];              // (asked for with the rest: the walk's chain of loads begins at it)
     j.nq = j.end > j.row && j.n > 0 ? a.qstart[j.end] - j.qs : 0;
     j.from = 0;
     int low = 0x7fffffff, high = -1;
@@ -118,6 +119,7 @@ __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) 
     j.qs = in_order ? at : a.qstart[j.row];
     j.nq = in_order ? 1 : a.qstart[j.row + 1] - j.qs;
     j.n = a.lens[j.row];
+    j.slot = a.slots[j.row];
     j.from = shared_keys(a, j.row);
   }
   return j;
@@ -253,7 +255,6 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
   int piece = at % out_splits, pieces = a.parts, per = 0;
   const int nth = piece;
   Job job;
-  int slot = -1;
   if (a.budget) {
     const RowShares shares(a);
     const uint64_t rows_to_go = __ballot(shares.upto > nth);
@@ -264,7 +265,7 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
     per = shares.per;
     job.row = __builtin_amdgcn_readlane(shares.row, ri);
     job.n = __builtin_amdgcn_readlane(shares.n, ri);
-    slot = __builtin_amdgcn_readlane(shares.slot, ri);
+    job.slot = __builtin_amdgcn_readlane(shares.slot, ri);
     job.qs = a.row_ids == nullptr ? job.row : a.qstart[job.row];
     job.nq = a.row_ids == nullptr ? 1 : a.qstart[job.row + 1] - job.qs;
     job.from = job.end = job.lowest = 0;
@@ -272,7 +273,7 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
   } else {
     job = job_of(a, by_group, ri);
   }
-  const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
+  const int qs = job.qs, nq = job.nq, n = job.n, from = job.from;
   const bool apart = by_group && job.apart();
   if (tile0 * 16 >= nq * group || (!by_group && nq > max_query)) return;      // (the same for the whole block)
   Column col[NT];
@@ -298,7 +299,7 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
   Tiles<D, NT> tl;
   tl.clear();
   if (key_lo <= key_hi) {
-    const int32_t* trow = table_at(a, a.budget ? slot : a.slots[row]);
+    const int32_t* trow = table_at(a, job.slot);
     const int max_page = a.table_stride - 1;
     const int bytes = Q8 ? 1 : 2;
     const int64_t plane = (int64_t)P * D * bytes;
@@ -766,7 +767,7 @@ __device__ __forceinline__ void tiles_block(const CacheArgs& a, int by_group, in
   const int tiles = blocks / a.splits, nth = at / a.splits;
   const int tile = folded && nth >= (tiles + 1) / 2 ? nth - (tiles + 1) / 2 : tiles - 1 - nth;
   const Job job = job_of(a, by_group, ri);
-  const int row = job.row, qs = job.qs, nq = job.nq, n = job.n, from = job.from;
+  const int qs = job.qs, nq = job.nq, n = job.n, from = job.from;
   const int columns = nq * group;
   if (tile * COLUMNS >= columns || (!by_group && nq <= less_than)) return;
   const int f0 = tile * COLUMNS + 32 * wave, f = f0 + c;
@@ -798,7 +799,7 @@ __device__ __forceinline__ void tiles_block(const CacheArgs& a, int by_group, in
       if (col.valid) x = *reinterpret_cast<const u32x4_t*>(qp + 16 * ds);
       qf[ds] = __builtin_bit_cast(bf16x8_t, x);
     }
-    const int32_t* trow = table_at(a, a.slots[row]);
+    const int32_t* trow = table_at(a, job.slot);
     // queries of the block see different keys from here on, or up to here
     const int seen_last = first_seen(pos_last, a.window), seen_tile = a.window ? first_seen(tile_first, a.window) : 0;
     const auto differs = [&](int kb) { return kb + 31 > pos_first || kb < seen_last; };
@@ -1003,6 +1004,8 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
   int64_t token = at / a.heads, place = token, apart = 1;  // its parts lie `apart` cells from one another
   int parts = a.parts;
   if (at >= cells) return;
+  // (cells by token: of no row's tokens a kernel left anything; what they hold is read beside the rows' bounds, and not written)
+  const bool nobodys = !a.budget && a.cell_queries == 0 && (token < a.qstart[0] || token >= a.qstart[a.rows]);
   if (a.budget) {
     const int2 mine = a.row_parts[token];
     parts = mine.y;
@@ -1017,8 +1020,6 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
     const int qs = in_order ? ri : a.qstart[row], nq = in_order ? 1 : a.qstart[row + 1] - qs;
     if (qi >= nq || nq > max_query || nq <= less_than) return;      // (a row of more queries, or of fewer, is another kernel's)
     token = qs + qi;
-  } else if (!a.budget && (token < a.qstart[0] || token >= a.qstart[a.rows])) {
-    return;                                                // a token of no row: no kernel left anything of it
   }
   if (token < 0 || token >= a.n_tokens) return;
   const int64_t first = a.budget ? place * a.heads + head : (place * a.heads + head) * a.parts;
@@ -1040,6 +1041,7 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheArgs a, int max_q
   }
   if (a.sink != nullptr && big != -INFINITY) l += exp2f(a.sink[head] * 1.4426950408889634f - big);
   const float inv = l == 0.f ? 0.f : 1.0f / l;
+  if (nobodys) return;
   QT* op = (QT*)a.out + (token * a.heads + head) * D + d0;
   if constexpr (std::is_same<QT, float>::value) {
     *reinterpret_cast<f32x4_t*>(op) = o * inv;
