@@ -1319,7 +1319,7 @@ extern "C" int holon_cache_attention(const HolonCacheAttention* call, const void
   HOLON_CHECK((int64_t)c.table_stride * c.page_size < (1ll << 31) - 256 && ((uint64_t)c.table_stride * c.page_size + 256) * excess < (1ull << 32),
               "attention: a table row of %d pages of %d tokens is too long", c.table_stride, c.page_size);
   HOLON_CHECK(c.page_stride < (1ll << 32) && c.scale_stride < (1ll << 32), "attention: pages lie too far apart");
-  if (c.tokens == 0) return 0;
+  if (c.tokens == 0 || c.rows <= 0) return 0;              // (tokens of no row are left alone)
   CacheArgs a{};
   a.q = q; a.out = out; a.pages = (const uint8_t*)c.pages; a.scales = (const uint8_t*)c.scales;
   a.page_stride = c.page_stride; a.scale_stride = c.scale_stride; a.num_pages = c.num_pages;

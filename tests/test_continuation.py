@@ -798,6 +798,23 @@ def test_windows_and_chunks_as_wide_as_there_are(hip, dtype):
 
 @gpu
 @pytest.mark.parametrize("q8", [False, True])
+def test_groups_of_no_row(hip, q8, monkeypatch):
+    """Groups without rows, behind the last row too; and a call of tokens, groups and no row at all, which leaves its result alone."""
+    q, pages, scales, table, attn, prefix = _step([(1100, 1)] * 3, 8, 2, 128, 16, shared=[(0, 2, 1056)], q8=q8, device="cuda")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")                              # noqa: E731
+    want = hip.prefix_attention(q, pages, table, attn, prefix, 16, 128 ** -0.5, scales)
+    more = SharedPrefix(i32(0, 0, 3, 3, 3), i32(1056, 1056, 1056, 16), 4, 3, 1056)
+    got = hip.prefix_attention(q, pages, table, attn, more, 16, 128 ** -0.5, scales)
+    _check(got, q, pages, scales, table, attn, 16, 128 ** -0.5)
+    assert (got.float() - want.float()).abs().max() <= 2 ** -6 * want.float().abs().max()
+    monkeypatch.setattr(torch, "empty_like", lambda t, **kw: torch.full(t.shape, 7.0, dtype=t.dtype, device=t.device))
+    none = AttnRows(i32(), i32(), i32(0), i32(), i32(), 0, 0, 0, 0, 0)
+    for shared in (None, SharedPrefix(i32(0, 0), i32(1056), 1, 3, 1056)):
+        assert (hip.prefix_attention(q, pages, table, none, shared, 16, 128 ** -0.5, scales) == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("q8", [False, True])
 def test_a_group_of_rows_of_no_key(hip, q8):
     """All of a step's rows are empty, and the bound on their lengths says so."""
     q, pages, scales, table, attn, prefix = _step([(40, 1)] * 3, 4, 2, 64, 16, shared=[(0, 2, 32)], q8=q8, device="cuda")
