@@ -1144,13 +1144,18 @@ Cut cut_keys(int jobs, int64_t columns, int64_t span, int64_t queries, int kv_he
   span = std::max<int64_t>(span, 1);
   columns = std::max<int64_t>(columns, 1);
   if (columns > FEW_COLUMNS && !f32) {
-    // Blocks of 256 columns (a stage is brought in once for twice the columns; one block a compute unit) where there is one for every
-    // unit and the first ones' walks are not much shorter than the last ones', or two. Heads 32 over 8 of 128, us, 128 columns | 256:
-    // 4,096 tokens behind 28,672 2,710 | 2,492 (bfloat16 2,506 | 2,192), 2,048 behind 6,144 332 | 339 (306 | 296), a whole prompt of 2,048
-    // 82 | 93 (73 | 82), of 8,192 737 | 716 (679 | 625). Heads of 64: over codes 4,096 behind 28,672 1,923 | 1,715, 2,048 behind 6,144 234 |
-    // 233, a whole prompt of 8,192 528 | 491; over bfloat16, whose stages cost no widening, never: 1,600 | 1,722, 213 | 234, 394 | 490.
+    // Blocks of 256 columns (a stage is brought in once for twice the columns; one block a compute unit) where there are about two for every
+    // unit; where there is one, if the first ones' walks are not much shorter than the last ones'; where there is one and a part, if what
+    // is left behind the first round is short. 32 heads over 8 of 128, us over codes (over bfloat16), 128 columns | 256: 4,096 tokens
+    // behind 28,672 2,669 | 2,456 (2,499 | 2,183), a whole prompt of 8,192 724 | 708 (674 | 630); 2,048, one block a unit, behind 2,048 155 | 173
+    // (141 | 153), 6,144 327 | 334 (301 | 295), 28,672 1,321 | 1,227 (1,212 | 1,075), a whole prompt of 2,048 83 | 92 (73 | 82); of 40 heads, 1.25
+    // blocks a unit, behind 2,048 243 | 224 (225 | 198), 4,096 371 | 384 (340 | 339), 28,672 2,158 | 2,337 (1,999 | 2,075). Heads of 64: over
+    // codes 4,096 behind 28,672 1,936 | 1,734, 2,048 behind 6,144 235 | 235, a whole prompt of 8,192 532 | 495; over bfloat16, whose stages cost
+    // no widening, 1,585 | 1,678, 213 | 228, 385 | 477: not there.
     const int64_t wide = units * ((columns + 255) / 256);
-    r.waves = head_dim <= 128 && (head_dim > 64 || value_bytes == 1) && (wide >= 512 || (wide >= 256 && 2 * queries <= span)) ? 8 : 4;
+    const bool pays = wide >= 448 || (wide >= 256 && wide <= 288 && 4 * queries <= span) ||
+                      (wide > 288 && 4 * queries <= 3 * span && 2 * span <= 5 * queries);
+    r.waves = head_dim <= 128 && (head_dim > 64 || value_bytes == 1) && pays ? 8 : 4;
     r.tiles = (int)((columns + 32 * r.waves - 1) / (32 * r.waves));
     const int64_t want = std::max<int64_t>(1, 2048 / r.waves / (units * r.tiles));      // two waves a SIMD
     r.splits = (int)std::min<int64_t>(std::min<int64_t>(want, 32), std::max<int64_t>(1, (span + 127) / 128));
@@ -1194,10 +1199,10 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
   p.any_shared = n_groups > 0 && max_group_query > 0 && max_group_len > 0;
   // Decode rows that one block each serves read their prefix themselves, from L2, while the GPU has room for all blocks and a row's keys
   // are 192 KB at most: one launch for two. Two (the groups' and the rows', the merge) | one, four rows, us in a graph, where the merge's own
-  // launch costs least (not recorded, two take 15 us at least); keys behind | us: 32 heads over 8 of 128, codes 256 9.8 | 7.5, 768 10.8 | 10.8,
-  // 1,536 12.1 | 16.4, float32 queries 256 17 | 9, 1,536 23 | 22, bfloat16 256 10.9 | 8.1, 768 11.9 | 13.2; 16 over 8 of 64, codes 256 8.4 | 5.8,
-  // 1,536 10.4 | 10.2, 2,560 11.7 | 13.3, float32 queries 1,536 21 | 14, bfloat16 1,024 10.3 | 9.8, 1,536 11.0 | 12.0; 16 over 2 of 256, codes
-  // 256 18.6 | 10.5, 768 19.2 | 18.1, 1,024 19.9 | 21.7, float32 queries 512 22 | 19, 1,024 24 | 29, bfloat16 384 18.0 | 15.5, 640 19.2 | 21.4.
+  // launch costs least (not recorded, two take 15 us at least); keys behind | us: 32 heads over 8 of 128, codes 256 9.6 | 7.3, 768 10.6 | 10.5,
+  // 1,536 11.9 | 15.8, float32 queries 256 17 | 9, 1,536 18 | 21, bfloat16 256 10.9 | 8.1, 768 11.9 | 13.3; 16 over 8 of 64, codes 256 8.2 | 5.7,
+  // 1,536 10.3 | 10.2, 2,560 10.2 | 13.3, float32 queries 1,536 16 | 14, bfloat16 1,024 10.1 | 9.7, 1,536 11.0 | 11.8; 16 over 2 of 256, codes
+  // 256 18.2 | 10.4, 512 15.6 | 14.3, 768 17.3 | 17.9, float32 queries 512 20 | 19, 768 22 | 24, bfloat16 384 17.7 | 15.4, 512 16.5 | 18.3.
   const int64_t alone = 192 * 1024;
   const bool one_each = p.any_shared && n_chunk == 0 && group <= 16 && (int64_t)n_decode * kv_heads <= 256 &&
                         (int64_t)max_decode_len * head_dim * value_bytes <= alone;
@@ -1227,8 +1232,8 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
       const int64_t units = (int64_t)n_groups * kv_heads;
       if (p.shared.tiles) {                                // one block a compute unit, the rows' blocks beside them
         // Blocks of 256 columns, if they are full, over long prefixes. 128 columns | 256, us, 64 rows of 32 heads over 8 of 128 with 256 keys of
-        // their own, bfloat16: behind 16,384 55 | 67, 32,768 82 | 85, 49,152 110 | 107, 65,536 141 | 127, 131,072 253 | 211; of heads of 64
-        // 44 | 51, 62 | 65, 81 | 79, 102 | 92, 180 | 150, over codes 45 | 52, 66 | 66, 88 | 80, 110 | 94, 198 | 150.
+        // their own, bfloat16: behind 16,384 50 | 60, 32,768 77 | 78, 49,152 106 | 100, 65,536 136 | 120, 131,072 249 | 205; of heads of 64
+        // 38 | 43, 57 | 57, 76 | 71, 96 | 85, 174 | 144, over codes 40 | 45, 61 | 58, 81 | 73, 103 | 87, 190 | 144.
         const int64_t columns = (int64_t)max_group_query * group;
         p.shared.waves = max_group_len >= 49152 && (columns + 255) / 256 * 2 == (columns + 127) / 128 ? 8 : 4;
         p.shared.tiles = (int)((columns + 32 * p.shared.waves - 1) / (32 * p.shared.waves));
@@ -1253,13 +1258,13 @@ Plan plan_of(int n_decode, int max_decode_len, int n_chunk, int max_chunk_query,
     // bits: 32,768 and seven of 500 keys 40 | 29, 32,768 and fifteen of 500 67 | 31, 16,384 and 47 of 700 83 | 33, eight of 11,000 to 32,768 80 |
     // 79; all alike, eight of 32,768 109 | 112, 32 of 4,096 51 | 51; where rows are short, 900 to 4,096, 12 | 16.
     // A portion's blocks and the decode rows in one launch, but where the decode rows are most of a long step (their blocks then run at a
-    // portion's occupancy). Two | one, us in a graph, over codes: 32 heads over 8 of 128, a portion of 2,048 behind 6,144 and seven rows of
-    // 8,000 364 | 341, 512 behind 28,672 and 16 of 4,096 373 | 351, 256 and 32 of 1,000 36 | 27, 128 and one of 300 19 | 12; 128 behind 8,000
-    // and 64 of 4,096 155 | 161, 16 over 8 of 64, 32 of 16,384 136 | 150. No line in a step's bytes and operations is much sooner there: 0.5%
-    // from the best on average over 192 steps, 10% at most. Over bfloat16 (32 over 8 of 128, then of 64): 512 behind 28,672 and 16 of 4,096
-    // 370 | 344, 243 | 222; 128 behind 8,000 and 64 of 4,096 235 | 247, 131 | 143, behind 2,000 220 | 231, 120 | 141. At heads of 256 (16 over 2)
-    // the joined kernel's tiles are slower: 2,048 behind 28,672 and eight of 1,000 1,514 | 1,608, a whole prompt of 2,048 and 16 of 4,096
-    // 148 | 128. By this rule 0.4 and 0.6% from the best on average over 216 and 48 steps, 9% at most; always joined 1.2 and 2.9%, 21%.
+    // portion's occupancy). Two | one, us in a graph, over codes: 32 heads over 8 of 128, a portion of 512 behind 28,672 and 16 of 4,096
+    // 372 | 352, a whole prompt of 2,048 and as many 111 | 88, 128 and one of 300 18 | 11; 128 behind 8,000 and 64 of 4,096 154 | 158, 16 over 8 of
+    // 64, 32 of 16,384 133 | 140. No line in a step's bytes and operations is sooner there: 0.3% from the best on average over 264 steps, 5%
+    // at most. Over bfloat16 (32 over 8 of 128, then of 64): 512 behind 28,672 and 16 of 4,096 378 | 352, 249 | 226; 128 behind 8,000 and 64 of
+    // 4,096 235 | 241, 130 | 138, behind 2,000 220 | 226, 119 | 138. At heads of 256 (16 over 2) the joined kernel's tiles are slower: 2,048
+    // behind 28,672 and eight of 1,000 1,531 | 1,614, a whole prompt of 2,048 and 16 of 4,096 146 | 126. By this rule 0.3 and 0.5% from the best
+    // on average over 216 and 48 steps, 9% at most; always joined 1.0 and 2.5%, 19%.
     const double keys = 2.0 * value_bytes * n_decode * kv_heads * head_dim * seen_span(max_decode_len, 1, window);       // bytes
     const double work = 4.0 * n_chunk * max_chunk_query * heads * head_dim *                                             // operations
                         std::min(seen_span(max_chunk_len, max_chunk_query, window), std::max((int64_t)max_chunk_len - max_chunk_query / 2, (int64_t)1));
