@@ -585,8 +585,8 @@ __device__ __forceinline__ void rows_block(const CacheArgs& a, int by_group, int
 //     of the stage's first 16 and of its last: the B operands of
 //   O^T (32 dims x 32 columns) += V^T P^T: A = 32 dims x 16 keys, the values transposed as in the pages.
 // Rows of LDS are swizzled by pieces of 16 bytes, so that 16 lanes that read one piece of 16 rows touch every bank once.
-// A wave's own chain bounds it, scores, softmax, products, with two waves a SIMD: 32 heads over 8 of 128, 2,048 tokens behind 6,144 354
-// us over codes and 331 over bfloat16 (0.68, 0.73 PFLOP/s), 4,096 behind 28,672 0.78 and 0.88. The next stage's scores beside this one's
+// A wave's own chain bounds it, scores, softmax, products, with two waves a SIMD: 32 heads over 8 of 128, 2,048 tokens behind 6,144 335
+// us over codes and 296 over bfloat16 (0.72, 0.81 PFLOP/s), 4,096 behind 28,672 0.83 and 0.94. The next stage's scores beside this one's
 // softmax would need more registers than there are (spilled: 498 us), and a second stage ahead in registers brings nothing (407).
 constexpr float SLACK = 8.f;   // see where it is used
 

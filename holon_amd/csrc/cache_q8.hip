@@ -154,9 +154,10 @@ __device__ __forceinline__ void write_block(const Target& w, int hk, const Place
 
 // A block takes 16 tokens of one head: 16 lanes a token, D / 16 values of its key and of its value a lane. Values go through LDS
 // where their tokens lie in two stretches, so that what a stretch has of a dim's 16 bytes is written at once; tokens anywhere else
-// have theirs written one by one. Memory bounds it: 8 heads of 128 in bfloat16, 4,096 tokens from a page's begin on (25 MB) 9.0 us a
-// call, from its sixth place on 10.6, anywhere 27; 32,768 tokens 46, 54 and 169 (4.4, 3.7 and 1.2 TB/s). With one stretch alone, a byte
-// at a time from the sixth place on, the second of these took 14.9 and 87. Below some 1,000 tokens the host's 8 us.
+// have theirs written one by one. Memory bounds it: 8 heads of 128 in bfloat16, over inputs that change from call to call 4,096 tokens
+// from a page's begin on 11.6 us a call, 16,384 35, 32,768 63 (202 MB, 3.2 TB/s). Over the same again and again, which the Infinity
+// Cache holds: 4,096 tokens (25 MB) from a page's begin on 9.0, from its sixth place on 10.6, anywhere 27; 32,768 tokens 46, 54 and 169. With
+// one stretch alone, a byte at a time from the sixth place on, the second of these took 14.9 and 87. Below some 1,000 tokens the host's 8 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t stride, int wide, Target w) {
   constexpr int E = D / 16;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(256) kv_write_q8_kernel(const T* __restrict__ 
 // The merged projection's heads: queries and keys normed and turned, queries to q_out, keys and values into the cache. A block takes
 // 16 tokens of one kv head, or of one query head; a value's partner in the rotation is eight lanes away.
 // 32 heads over 8 of 128 in bfloat16: 8 tokens 4.7 us (a chain of loads: position, angles; place, stores), 64 5.6, 2,048 15.3 (46 MB, 3.0
-// TB/s); into the 16-bit cache, by blocks of a token each, 3.4, 3.8 and 12.6.
+// TB/s), 8,192 50 (189 MB, 3.8); into the 16-bit cache, by blocks of a token each, which read angles and places once, 3.4, 3.8, 12.1 and 40.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) qk_norm_rope_write_q8_kernel(const T* __restrict__ qkv, T* __restrict__ q_out, int heads,
                                                                     const T* __restrict__ q_weight, const T* __restrict__ k_weight,
@@ -238,8 +239,8 @@ __device__ __forceinline__ void widen4(uint32_t w, float power, float (&f)[4]) {
   f[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * power;
 }
 // The same blocks the other way round: 16 lanes a token, D / 16 of its codes a lane. Two thirds of what it moves are the values it
-// writes: 32,768 tokens of 8 heads of 128 into bfloat16 (202 MB) 36 us from a page's begin on, 40 from its sixth place on, 84 anywhere;
-// into 32 bits (336 MB) 92, 97 and 147.
+// writes: over inputs that change from call to call 32,768 tokens of 8 heads of 128 into bfloat16 (202 MB) 46 us, into 32 bits (336 MB) 86 (4.4
+// and 3.9 TB/s); over the same again and again 36 us from a page's begin on, 40 from its sixth place on, 84 anywhere, into 32 bits 92, 97, 147.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_read_q8_kernel(T* __restrict__ k, T* __restrict__ v, const uint8_t* __restrict__ pages,
                                                          const uint8_t* __restrict__ scales, int64_t page_stride,

@@ -7,16 +7,16 @@
 //   the first x with sum_{y <= x} mass(y) > draw[b] * sum mass.
 //
 // So a token's law is p whatever q is: accept lies in [0, 1), where it is below p(x) / q(x) with that probability (1 at most), and never
-// where p(x) = 0, at accept[i] = 0 and q(x) = 0 too: what a mask has set to -inf does not come out. T = 0 takes the largest logit for p. The draw compares a running sum over up to hundreds
-// of thousands of masses with a given number: exponentials and sums are in 64 bits, where the order of a sum moves a border
-// between two tokens by 1e-16 of the whole, not by more than a token's own mass as in 32.
+// where p(x) = 0, at accept[i] = 0 and q(x) = 0 too: what a mask has set to -inf does not come out. T = 0 takes the largest logit for p.
+// The draw compares a running sum over up to hundreds of thousands of masses with a given number: exponentials and sums are in 64 bits,
+// where the order of a sum moves a border between two tokens by 1e-16 of the whole, not by more than a token's own mass as in 32.
 //
 // Two launches over pieces of 4,096 values: every row's largest value and sum of exponentials; the judgement and the walk through the
 // one piece that the drawn number falls into, by a block a request. The masses of p are the pieces' sums, those of p without a certain
 // draft too but for its own piece; where drafts came with probabilities, a launch between judges (every block for itself) and sums
 // max(p - q, 0) of the rows whose draft was turned down. 151,936 tokens, 64 requests of four drafts: 45 us (177 MB of logits, 3.9 TB/s:
 // memory, and beside it 64-bit arithmetic, 34 us by its count), 22 and 11; one request of three 4.4, 6.4 and 9.0, each a chain of loads.
-// Without probabilities 85 us a call of 64 requests with the launch between, 72 without it, 18.4 and 17.2 a call of one.
+// Without probabilities 44 and 16 (its launch between took 13 us more a call), 4.4 and 11.5.
 // (The walk by the last block to leave its masses, which saves a launch, took the judgement's launch over 64 requests from 28 to 111 us:
 // to see the others' masses across the XCDs each block writes back and drops what its L2 holds of the logits.)
 #include "common.h"
