@@ -66,6 +66,9 @@ __device__ __forceinline__ const int32_t* table_at(const CacheArgs& a, int32_t s
   return a.table + (int64_t)min((uint32_t)slot, (uint32_t)(a.n_slots - 1)) * a.table_stride;
 }
 
+// A row's length, as far as its block table goes (so that every walk ends: a table's row holds fewer than 2^31 - 256 keys).
+__device__ __forceinline__ int length_of(const CacheArgs& a, int row) { return min(a.lens[row], a.table_stride * a.page_size); }
+
 // The keys a row shares with its group (0: it is in none), by the lanes of a wave side by side.
 __device__ __forceinline__ int shared_keys(const CacheArgs& a, int row) {
   if (a.n_groups == 0) return 0;
@@ -107,7 +110,7 @@ __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) 
     j.from = 0;
     int low = 0x7fffffff, high = -1;
     for (int at64 = j.row; at64 < j.end; at64 += WAVE) {
-      const int r = min(at64 + (int)(threadIdx.x % WAVE), j.end - 1), n = a.lens[r], queries = a.qstart[r + 1] - a.qstart[r];
+      const int r = min(at64 + (int)(threadIdx.x % WAVE), j.end - 1), n = length_of(a, r), queries = a.qstart[r + 1] - a.qstart[r];
       low = min(low, queries > 0 ? n - queries : low);
       high = max(high, queries > 0 ? n - 1 : high);
     }
@@ -118,7 +121,7 @@ __device__ __forceinline__ Job job_of(const CacheArgs& a, int by_group, int at) 
     j.row = in_order ? at : a.row_ids[at];
     j.qs = in_order ? at : a.qstart[j.row];
     j.nq = in_order ? 1 : a.qstart[j.row + 1] - j.qs;
-    j.n = a.lens[j.row];
+    j.n = length_of(a, j.row);
     j.slot = a.slots[j.row];
     j.from = shared_keys(a, j.row);
   }
@@ -133,7 +136,7 @@ __device__ __forceinline__ int position_in_group(const CacheArgs& a, const Job& 
     if (a.qstart[mid] <= token) row = mid;
     else end = mid;
   }
-  return a.lens[row] - (a.qstart[row + 1] - token);
+  return length_of(a, row) - (a.qstart[row + 1] - token);
 }
 
 // Decode rows of different lengths: as many blocks for each as its keys are of all rows' keys, so that blocks have about the same to
@@ -146,7 +149,7 @@ struct RowShares {
   __device__ __forceinline__ explicit RowShares(const CacheArgs& a) {
     const int r = threadIdx.x % WAVE, here = min(r, a.n_rows - 1);
     row = a.row_ids == nullptr ? here : a.row_ids[here];
-    n = a.lens[row];
+    n = length_of(a, row);
     slot = a.slots[row];
     const int units = r < a.n_rows && n > 0 ? (n - 1) / 64 - max(0, first_seen(n - 1, a.window)) / 64 + 1 : 0;
     // (A sum past 2^24 is rounded; one step makes `per` large enough then: never more than budget + n_rows blocks, the launch's.)

@@ -200,7 +200,8 @@ class Kernels(Protocol):
         """`paged_attention` over an 8-bit cache (see `kv_write_q8`): the softmax and its sums in float32 over the values that the
         cache stands for. q [T, Hq, D] bfloat16 or float32 -> a new tensor of its type; heads of 64, 128 and 256, pages of a
         multiple of 16 tokens; `scale` > 0. A query that sees no key gets zeros; what a query does not see, finite or not, does
-        not reach it. Tokens of no row are not written. A page or slot number out of range is not followed."""
+        not reach it. Tokens of no row are not written. A page or slot number out of range is not followed, a length past the end
+        of its block table's row is taken as that."""
 
     def prefix_attention(self, q: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, rows: AttnRows, prefix: SharedPrefix,
                          page_size: int, scale: float, scales: torch.Tensor | None = None, sink: torch.Tensor | None = None

@@ -797,6 +797,29 @@ def test_windows_and_chunks_as_wide_as_there_are(hip, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [[(200, 1)], [(5000, 1), (37, 1), (300, 1)], [(100, 3), (200, 5)], [(70, 90), (20, 1)]])
+def test_lengths_past_the_block_table(hip, rows, dtype):
+    """A row's walk ends where its table does, whatever its length says: 2^31 - 1 is the table's last key."""
+    q, pages, scales, table, attn, _ = _step(rows, 4, 2, 64, 16, seed=1, dtype=dtype, device="cuda")
+    pages.view(torch.uint8)[(pages.view(torch.uint8) & 0x7f) == 0x7f] = 0x30          # (the null page's keys are seen here)
+    attn.lens[0] = 16 * table.shape[1]
+    attn.max_decode_len = 16 * table.shape[1]
+    want = hip.paged_attention_q8(q, pages, scales, table, attn, 16, 0.125)
+    _check(want, q, pages, scales, table, attn, 16, 0.125)
+    for more in (16 * table.shape[1] + 1, 2 ** 31 - 200, 2 ** 31 - 1):
+        print(rows, more, flush=True)
+        attn.lens[0] = more
+        assert torch.equal(hip.paged_attention_q8(q, pages, scales, table, attn, 16, 0.125), want)
+    attn.lens[0] = 2 ** 31 - 1
+    prefix = SharedPrefix(torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda"), 1,
+                          rows[0][1], 16 * table.shape[1])
+    got = hip.prefix_attention(q, pages, table, attn, prefix, 16, 0.125, scales)
+    attn.lens[0] = 16 * table.shape[1]
+    _check(got, q, pages, scales, table, attn, 16, 0.125)
+
+
+@gpu
 @pytest.mark.parametrize("q8", [False, True])
 def test_groups_of_no_row(hip, q8, monkeypatch):
     """Groups without rows, behind the last row too; and a call of tokens, groups and no row at all, which leaves its result alone."""
